@@ -7,7 +7,7 @@
 // Kernels
 //  mask_logits_rows_kernel  logits[slot][y][x] = sum_k coef[slot][k] * proto[b][k][y][x], only for the rows and
 //                        columns of the letterbox crop window that the survivor's box can read, as a k-ordered
-//                        fmaf chain on the vector ALU (v_pk_fma_f32); proto is read once.
+//                        fmaf chain on the vector ALU; proto is read once.
 //  mask_gemm_kernel      the same product as dense 32-survivor tiles on the exact-fp32 MFMA
 //                        (v_mfma_f32_32x32x2_f32); kept for odd prototype widths.
 //  The upsample is HBM-write-bound (m*H0*W0 bytes of uint8 per image, ~97 % of them zeros outside the boxes) and

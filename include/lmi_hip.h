@@ -40,7 +40,7 @@ enum lmi_status {
   LMI_ERR_NO_DEVICE = -6
 };
 
-enum lmi_dtype { LMI_F32 = 0, LMI_F16 = 1, LMI_U8 = 2 };
+enum lmi_dtype { LMI_F32 = 0, LMI_F16 = 1, LMI_U8 = 2, LMI_BF16 = 3, LMI_I32 = 4, LMI_I64 = 5, LMI_MXFP4 = 6 };
 
 /* resampler of the letterbox entry: the fixed-point cv2.INTER_LINEAR (default) */
 enum lmi_resize_mode { LMI_RESIZE_CV2_LINEAR = 0, LMI_RESIZE_TORCH_BILINEAR = 1, LMI_RESIZE_TORCH_BILINEAR_1T = 2 };
@@ -60,6 +60,8 @@ enum lmi_resize_mode { LMI_RESIZE_CV2_LINEAR = 0, LMI_RESIZE_TORCH_BILINEAR = 1,
 #define LMI_MAX_MASK_DIM 32    /* number of prototype channels (nm) the mask kernels are built for */
 #define LMI_MAX_POINT_OPS 16   /* longest operator list lmi_revert_points_f32 accepts */
 #define LMI_NMS_STATIC_BYTES (4 << 20) /* built-in workspace of lmi_nms_v8_static, per GPU */
+#define LMI_MAX_TOP 32         /* most alternatives lmi_class_logprobs returns per row */
+#define LMI_MX_BLOCK 32        /* elements that share one MXFP4 scale */
 
 int lmi_version(void);
 const char *lmi_status_string(int status);
@@ -453,6 +455,83 @@ int lmi_pack_mask_boxes(const void *masks, int dtype, int64_t m, int img_h, int 
 int64_t lmi_trace_contours_host(const uint64_t *words, int64_t m, const int32_t *boxes,
                                 const int64_t *word_offset, int strategy_all, int threads,
                                 int32_t *out_xy, int64_t capacity_points, int64_t *points_per_mask);
+
+/* ------------------------------------------------------------------------------------------
+ * Class evidence -- log probability of a given class, entropy, and the best alternatives of rows of `classes` values.
+ * The reference keeps the best class's score only (object_detectors/yolov8_lmi/model.py:223-232); this is what the
+ * other classes of the same row say.
+ *   LMI_PROB_SOFTMAX  x are logits: logp_c = x_c - log sum_j e^(x_j); entropy = -sum_c p_c logp_c.
+ *                     A row whose values are all -inf holds no class: every logp is -inf, the entropy 0.
+ *   LMI_PROB_SIGMOID  x are logits of independent classes: logp_c = log sigmoid(x_c); entropy = the sum over the
+ *                     classes of the entropy of a yes / no answer with that probability.
+ *   LMI_PROB_NONE     x are such probabilities themselves (what the detection head emits): logp_c = log x_c.
+ * Rows: (n0, n1) of them, row (o, i) at x + o*stride0 + i*stride1, class c another c*class_stride on (elements).
+ * With `index` [device] int32 (n0, n1) row (o, m) is read at i = index[o][m] of `index_range` positions (the anchors
+ * NMS kept); with `count` [device] int32 (n0) rows m >= count[o] are skipped and their outputs left as they are.  An
+ * index outside its range gives NaN (alternatives: -1).
+ * labels [device] LMI_F32 | LMI_I32 | LMI_I64, strides in elements, may be NULL with logprob; a label outside
+ * [0, classes) gives NaN.
+ * Outputs [device], any of them NULL if not wanted, contiguous: logprob (n0,n1), entropy (n0,n1) fp32; top_logprob fp32 and
+ * top_index int32 (n0,n1,top), best first, equal values in the order of their classes, NaN before everything else.
+ * 0 <= top <= min(classes, LMI_MAX_TOP).  `workspace` [device] of lmi_class_logprobs_workspace_bytes (0: none needed).
+ */
+enum lmi_prob_activation { LMI_PROB_SOFTMAX = 0, LMI_PROB_SIGMOID = 1, LMI_PROB_NONE = 2 };
+typedef struct lmi_logprob_args {
+  const void *x;
+  int32_t x_dtype, activation; /* LMI_F32 | LMI_F16 | LMI_BF16; enum lmi_prob_activation */
+  int64_t classes, class_stride, n0, n1, stride0, stride1;
+  const int32_t *index;
+  int64_t index_range;
+  const int32_t *count;
+  const void *labels;
+  int64_t label_stride0, label_stride1;
+  int32_t label_dtype, top;
+  float *logprob, *entropy, *top_logprob;
+  int32_t *top_index;
+  void *workspace;
+  int64_t workspace_bytes;
+} lmi_logprob_args;
+int64_t lmi_class_logprobs_workspace_bytes(int64_t rows, int64_t classes, int64_t class_stride, int top);
+int lmi_class_logprobs(const lmi_logprob_args *args, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * MXFP4 -- microscaled 4-bit floating point (OCP MX v1.0): blocks of LMI_MX_BLOCK elements along a row share the scale
+ * 2^(byte - 127), byte 255 = NaN; elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two per byte, the
+ * earlier one in the low half.  A row of k elements takes B = ceil(k / 32) scale bytes and 16*B element bytes; the last
+ * block is filled up with zeros.
+ * lmi_mx_quantize: scale exponent floor(log2(max |x|)) - 2 of each block, at least -127 (also for a block of zeros);
+ *   elements rounded to nearest, ties to even, beyond 6 to 6.  A block that holds an infinity or a NaN gets byte 255.
+ *   x LMI_F32 | LMI_F16 | LMI_BF16, k contiguous elements a row, rows row_stride elements apart.
+ * lmi_mx_dequantize: the values, as out_dtype (LMI_F32 | LMI_F16 | LMI_BF16), rows contiguous.
+ * lmi_mx_product: y[m][n] = act(sum_k Q(x)[m][k] * w[n][k] + bias[n]) with fp32 sums, Q = lmi_mx_quantize along k,
+ *   w quantised.  The positions m are (batch, pixels).  layout LMI_MX_ROWS (a linear layer, channels-last maps): x
+ *   element (b, p, k) at b*x_batch + p*x_stride + k, y contiguous (batch, pixels, n).  LMI_MX_PLANES (NCHW maps): x
+ *   element at b*x_batch + k*x_stride + p, y contiguous (batch, n, pixels).
+ *   x_dtype LMI_MXFP4: x points at packed rows, x_scales at their scales (rows, batch 1, x_stride unused).
+ *   y_dtype LMI_F32 | LMI_F16 | LMI_BF16, the type of x unless that is MXFP4.  bias [device] fp32 (n) or NULL.  workspace [device] of lmi_mx_product_workspace_bytes (0: none).
+ *   This is a 1x1 convolution of the network with its folded batch norm (bias) and SiLU.
+ */
+enum lmi_mx_act { LMI_ACT_NONE = 0, LMI_ACT_SILU = 1 };
+enum lmi_mx_layout { LMI_MX_ROWS = 0, LMI_MX_PLANES = 1 };
+typedef struct lmi_mx_product_args {
+  const void *x;
+  const uint8_t *x_scales;
+  int32_t x_dtype, act;
+  int64_t batch, pixels, k, n;
+  int64_t x_batch, x_stride;
+  const uint8_t *w_packed, *w_scales;
+  const float *bias;
+  void *y;
+  int32_t y_dtype, layout;
+  void *workspace;
+  int64_t workspace_bytes;
+} lmi_mx_product_args;
+int lmi_mx_quantize(const void *x, int dtype, int64_t rows, int64_t k, int64_t row_stride, uint8_t *packed,
+                    uint8_t *scales, void *stream);
+int lmi_mx_dequantize(const uint8_t *packed, const uint8_t *scales, int64_t rows, int64_t k, void *out, int out_dtype,
+                      void *stream);
+int64_t lmi_mx_product_workspace_bytes(const lmi_mx_product_args *args);
+int lmi_mx_product(const lmi_mx_product_args *args, void *stream);
 
 #ifdef __cplusplus
 }

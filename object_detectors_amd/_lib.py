@@ -10,7 +10,7 @@ import torch  # noqa: F401  -- must come first: the library has to bind to the H
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "liblmi_hip.so")
 
-LMI_F32, LMI_F16, LMI_U8 = 0, 1, 2
+LMI_F32, LMI_F16, LMI_U8, LMI_BF16, LMI_I32, LMI_I64, LMI_MXFP4 = 0, 1, 2, 3, 4, 5, 6
 LMI_MAX_DET_CAP = 1024
 LMI_NMS_STATIC_BYTES = 4 << 20
 
@@ -47,6 +47,31 @@ LMI_NMS_SWEEP_ONLY = 0x100
 
 class lmi_point_op(C.Structure):
     _fields_ = [("kind", C.c_int32), ("x", C.c_float), ("y", C.c_float)]
+
+
+LMI_PROB_SOFTMAX, LMI_PROB_SIGMOID, LMI_PROB_NONE = 0, 1, 2
+LMI_MAX_TOP = 32
+
+
+class lmi_logprob_args(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_dtype", C.c_int32), ("activation", C.c_int32), ("classes", C.c_int64), ("class_stride", C.c_int64),
+                ("n0", C.c_int64), ("n1", C.c_int64), ("stride0", C.c_int64), ("stride1", C.c_int64), ("index", C.c_void_p),
+                ("index_range", C.c_int64), ("count", C.c_void_p), ("labels", C.c_void_p), ("label_stride0", C.c_int64),
+                ("label_stride1", C.c_int64), ("label_dtype", C.c_int32), ("top", C.c_int32), ("logprob", C.c_void_p),
+                ("entropy", C.c_void_p), ("top_logprob", C.c_void_p), ("top_index", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
+LMI_MX_BLOCK = 32
+LMI_ACT_NONE, LMI_ACT_SILU = 0, 1
+LMI_MX_ROWS, LMI_MX_PLANES = 0, 1
+
+
+class lmi_mx_product_args(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_scales", C.c_void_p), ("x_dtype", C.c_int32), ("act", C.c_int32), ("batch", C.c_int64),
+                ("pixels", C.c_int64), ("k", C.c_int64), ("n", C.c_int64), ("x_batch", C.c_int64), ("x_stride", C.c_int64),
+                ("w_packed", C.c_void_p), ("w_scales", C.c_void_p), ("bias", C.c_void_p), ("y", C.c_void_p), ("y_dtype", C.c_int32),
+                ("layout", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
 LMI_POINT_DIV, LMI_POINT_SUB, LMI_POINT_FLIP_X, LMI_POINT_FLIP_Y, LMI_POINT_FLIP_XY = 1, 2, 3, 4, 5
@@ -114,6 +139,12 @@ SIGNATURES = {
     "lmi_pack_mask_boxes": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "lmi_trace_contours_host": (C.c_int64, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int64,
                                             C.c_void_p]),
+    "lmi_class_logprobs_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int]),
+    "lmi_class_logprobs": (C.c_int, [C.POINTER(lmi_logprob_args), C.c_void_p]),
+    "lmi_mx_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "lmi_mx_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_void_p]),
+    "lmi_mx_product_workspace_bytes": (C.c_int64, [C.POINTER(lmi_mx_product_args)]),
+    "lmi_mx_product": (C.c_int, [C.POINTER(lmi_mx_product_args), C.c_void_p]),
     "lmi_revert_points_f32": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
     "lmi_revert_masks_stage": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),

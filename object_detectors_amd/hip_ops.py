@@ -6,8 +6,10 @@ unless they say so.  There is no CPU fallback: tensors must live on a HIP device
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
+import math
 import struct
 import threading
 from typing import List, Optional, Sequence, Tuple, Union
@@ -704,3 +706,318 @@ def paste_masks(masks: torch.Tensor, boxes: torch.Tensor, image_shape: Tuple[int
     check(_L.lmi_paste_masks(m.data_ptr(), n, m.shape[1], m.shape[2], b.data_ptr(), b.shape[1], h, w, float(threshold),
                              out.data_ptr(), _stream(m.device)))
     return out if soft else out.view(torch.bool)
+
+
+_FLOAT_DTYPES = {torch.float32: LMI_F32, torch.float16: LMI_F16, torch.bfloat16: _lib.LMI_BF16}
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Makes `device` the current one for a launch (nothing to do in the usual case)."""
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _no_gradient(what: str, *tensors) -> None:
+    """The operators below serve inference: a graph they would silently cut is refused."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() / inference_mode(), or detach its inputs")
+
+
+_ACTIVATIONS = {"softmax": _lib.LMI_PROB_SOFTMAX, "sigmoid": _lib.LMI_PROB_SIGMOID, "none": _lib.LMI_PROB_NONE}
+_LABEL_DTYPES = {torch.float32: LMI_F32, torch.int32: _lib.LMI_I32, torch.int64: _lib.LMI_I64}
+
+
+def _two_strides(t: torch.Tensor, nd: int):
+    """Leading `nd` dimensions of t as (n0, n1, stride0, stride1), or None where two strides cannot say it."""
+    n, st = [], []
+    for size, stride in zip(t.shape[:nd], t.stride()[:nd]):
+        if size == 1:
+            continue
+        if n and st[-1] == stride * size:      # folds into the dimension before it
+            n[-1], st[-1] = n[-1] * size, stride
+        else:
+            n.append(size)
+            st.append(stride)
+    if len(n) > 2:
+        return None
+    while len(n) < 2:
+        n.insert(0, 1)
+        st.insert(0, 0)
+    return n[0], n[1], st[0], st[1]
+
+
+def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: int = 0, activation: str = "softmax",
+                   index: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None, out: Optional[dict] = None) -> dict:
+    """Log probability of given classes, entropy, and the `top` best classes of every row of x (..., C), classes last,
+    fp32 / fp16 / bf16.  x is read where it lies: a transposed view of the head's class planes
+    (`pred[:, 4:4 + nc].transpose(1, 2)`) or of the distance bins costs no copy.
+
+    activation 'softmax': x are logits, one class per row (a row of -inf alone has log probabilities -inf, entropy 0);
+    'sigmoid': logits of independent classes, the entropy summed over the yes / no answers; 'none': such
+    probabilities themselves, as the detection head emits them.
+    labels (...): int64, int32 or float32 (the class column of NMS rows, `det[:, :, 5]`, as it is); outside [0, C): NaN.
+    index (B, M) int32: row (b, m) is read at x[b, index[b, m]] of x (B, A, C) -- `anchor` of nms_v8; labels and results are
+    (B, M) then.  count (B,) int32: rows m >= count[b] are skipped and the results there left as they are (unspecified in
+    fresh ones).
+    out: a previous result of the same shapes to write into instead of allocating.
+    Returns dict(logprob (...) if labels are given, entropy (...), and for top > 0 top_logprob, top_index (..., top)): fp32 and int32, best
+    first, equal values in class order, NaN first.  Inference only: inputs that require a gradient are refused."""
+    _need_cuda(x, "x")
+    _no_gradient("class_logprobs", x)
+    if x.dtype not in _FLOAT_DTYPES:
+        raise TypeError("class_logprobs: x must be float32, float16 or bfloat16")
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"class_logprobs: unknown activation {activation!r}")
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError("class_logprobs: x must hold at least one class in its last dimension")
+    dev, c, top = x.device, x.shape[-1], int(top)
+    if not 0 <= top <= min(c, _lib.LMI_MAX_TOP):
+        raise ValueError(f"class_logprobs: top={top} must lie in 0..{min(c, _lib.LMI_MAX_TOP)}")
+    lead = tuple(x.shape[:-1])
+    if index is not None:
+        if x.ndim != 3 or index.ndim != 2 or index.shape[0] != x.shape[0]:
+            raise ValueError("class_logprobs: index (B,M) needs x (B,A,C)")
+        if index.dtype != torch.int32 or not index.is_contiguous() or index.device != dev:
+            raise ValueError("class_logprobs: index must be a contiguous int32 tensor on x's device")
+        lead = tuple(index.shape)
+    if count is not None:
+        if len(lead) != 2 or tuple(count.shape) != lead[:1] or count.dtype != torch.int32 or not count.is_contiguous() or count.device != dev:
+            raise ValueError("class_logprobs: count must be a contiguous int32 tensor (B,) on x's device, rows (B,M)")
+    if labels is not None:
+        if labels.dtype not in _LABEL_DTYPES or labels.device != dev:
+            raise TypeError("class_logprobs: labels must be int64, int32 or float32 on x's device")
+        if tuple(labels.shape) != lead:
+            raise ValueError(f"class_logprobs: labels must have shape {lead}")
+    want = {"logprob": (lead, torch.float32)} if labels is not None else {}
+    want["entropy"] = (lead, torch.float32)
+    if top:
+        want["top_logprob"], want["top_index"] = (lead + (top,), torch.float32), (lead + (top,), torch.int32)
+    if out is None:
+        out = {k: torch.empty(s, dtype=d, device=dev) for k, (s, d) in want.items()}
+    else:
+        for k, (s, d) in want.items():
+            t = out.get(k)
+            if t is None or tuple(t.shape) != s or t.dtype != d or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"class_logprobs: out[{k!r}] must be a contiguous {d} tensor of shape {s} on x's device")
+        out = {k: out[k] for k in want}
+    rows = math.prod(lead)
+    if rows == 0:
+        return out
+    if index is not None or count is not None:   # the two leading dimensions mean what they say
+        if x.ndim != 3:
+            raise ValueError("class_logprobs: count needs x (B,M,C)")
+        n0, n1, s0, s1 = lead[0], lead[1], x.stride(0), x.stride(1)
+    else:
+        split = _two_strides(x, x.ndim - 1)
+        if split is None:
+            x = x.contiguous()
+            split = _two_strides(x, x.ndim - 1)
+        n0, n1, s0, s1 = split
+    cs = x.stride(-1) if c > 1 else 1
+    if cs == 0 or any(v < 0 for v in (s0, s1, cs)):   # classes broadcast from one value
+        x = x.contiguous()
+        n0, n1, s0, s1 = (n0, n1, x.stride(0), x.stride(1)) if x.ndim == 3 and (index is not None or count is not None) else _two_strides(x, x.ndim - 1)
+        cs = x.stride(-1)
+    l0 = l1 = 0
+    if labels is not None:
+        if (n0, n1) == lead:
+            l0, l1 = labels.stride()
+        else:
+            if not labels.is_contiguous():
+                labels = labels.contiguous()
+            l0, l1 = n1, 1
+    a = _lib.lmi_logprob_args(
+        x.data_ptr(), _FLOAT_DTYPES[x.dtype], act, c, cs, n0, n1, s0, s1, None if index is None else index.data_ptr(),
+        0 if index is None else x.shape[1], None if count is None else count.data_ptr(), None if labels is None else labels.data_ptr(), l0, l1,
+        0 if labels is None else _LABEL_DTYPES[labels.dtype], top, out["logprob"].data_ptr() if labels is not None else None,
+        out["entropy"].data_ptr(), out["top_logprob"].data_ptr() if top else None, out["top_index"].data_ptr() if top else None, None, 0)
+    need = int(_L.lmi_class_logprobs_workspace_bytes(n0 * n1, c, cs, top))
+    ws = None
+    if need:   # not from the shared cache: two captured graphs that run side by side must not share it
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    with _on(dev):
+        check(_L.lmi_class_logprobs(C.byref(a), _stream(dev)))
+    return out
+
+
+class MxTensor:
+    """A tensor (..., k) in MXFP4: blocks of 32 elements along the last dimension share a power-of-two scale.
+    packed uint8 (rows, 16*B): two 4-bit elements per byte, the earlier one in the low half; scales uint8 (rows, B):
+    2^(byte - 127), 255 = NaN; B = ceil(k / 32), the last block filled up with zeros.  4.25 bits per element."""
+
+    __slots__ = ("packed", "scales", "shape")
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, shape):
+        self.packed, self.scales, self.shape = packed, scales, torch.Size(shape)
+        rows, blocks = math.prod(self.shape[:-1]), -(-self.shape[-1] // _lib.LMI_MX_BLOCK)
+        for t, s, name in ((packed, (rows, 16 * blocks), "packed"), (scales, (rows, blocks), "scales")):
+            if t.dtype != torch.uint8 or tuple(t.shape) != s or not t.is_contiguous() or t.device != packed.device:
+                raise ValueError(f"MxTensor: {name} must be a contiguous uint8 tensor of shape {s}")
+
+    @property
+    def device(self) -> torch.device:
+        return self.packed.device
+
+    def __repr__(self):
+        return f"MxTensor(shape={tuple(self.shape)}, device={self.device})"
+
+
+def _rows_of(x: torch.Tensor):
+    """x (..., k) as (tensor, rows, row stride): the elements of a row side by side, rows a fixed distance apart."""
+    if x.ndim == 1:
+        x = x.unsqueeze(0)
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    split = _two_strides(x, x.ndim - 1)
+    if split is None or split[0] != 1:
+        x = x.contiguous()
+        split = _two_strides(x, x.ndim - 1)
+    return x, math.prod(x.shape[:-1]), split[3]
+
+
+def mx_quantize(x: torch.Tensor) -> MxTensor:
+    """x (..., k), fp32 / fp16 / bf16 -> MXFP4 along the last dimension: scale 2^(floor(log2 max|x|) - 2) of each block of 32, elements
+    rounded to nearest (ties to even) and held at 6 at most.  A block with an infinity or a NaN becomes NaN as a whole."""
+    _need_cuda(x, "x")
+    _no_gradient("mx_quantize", x)
+    if x.dtype not in _FLOAT_DTYPES:
+        raise TypeError("mx_quantize: x must be float32, float16 or bfloat16")
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError("mx_quantize: x must hold at least one element in its last dimension")
+    shape, k, dev = x.shape, x.shape[-1], x.device
+    blocks, rows = -(-k // _lib.LMI_MX_BLOCK), math.prod(x.shape[:-1])
+    packed = torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=dev)
+    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=dev)
+    if rows:
+        x, _, stride = _rows_of(x)
+        with _on(dev):
+            check(_L.lmi_mx_quantize(x.data_ptr(), _FLOAT_DTYPES[x.dtype], rows, k, stride, packed.data_ptr(), scales.data_ptr(), _stream(dev)))
+    return MxTensor(packed, scales, shape)
+
+
+def _need_mx(q, name: str) -> None:
+    if not isinstance(q, MxTensor):
+        raise TypeError(f"{name} must be an MxTensor (mx_quantize)")
+    _need_cuda(q.packed, name)
+
+
+def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values an MxTensor stands for (exact in fp32 and, within its range, bf16; fp16 rounds what lies outside its range)."""
+    _need_mx(q, "q")
+    if dtype not in _FLOAT_DTYPES:
+        raise TypeError("mx_dequantize: dtype must be float32, float16 or bfloat16")
+    y = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if y.numel():
+        with _on(q.device):
+            check(_L.lmi_mx_dequantize(q.packed.data_ptr(), q.scales.data_ptr(), math.prod(q.shape[:-1]), q.shape[-1], y.data_ptr(),
+                                       _FLOAT_DTYPES[dtype], _stream(q.device)))
+    return y
+
+
+_MX_ACTS = {None: _lib.LMI_ACT_NONE, "silu": _lib.LMI_ACT_SILU}
+
+
+def _mx_product(what, x_ptr, x_scales, x_dtype, batch, pixels, k, x_batch, x_stride, weight, bias, act, y, layout):
+    """Checks what mx_linear and mx_pointwise share, and enqueues the product."""
+    dev = y.device
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (weight.shape[0],) or not bias.is_contiguous() or bias.device != dev):
+        raise ValueError(f"{what}: bias must be a contiguous float32 tensor ({weight.shape[0]},) on x's device")
+    if y.numel() == 0:
+        return y
+    a = _lib.lmi_mx_product_args(x_ptr, x_scales, x_dtype, _MX_ACTS[act], batch, pixels, k, weight.shape[0], x_batch, x_stride,
+                                 weight.packed.data_ptr(), weight.scales.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
+                                 _FLOAT_DTYPES[y.dtype], layout, None, 0)
+    need = int(_L.lmi_mx_product_workspace_bytes(C.byref(a)))
+    ws = None
+    if need:   # not from the shared cache: two captured graphs that run side by side must not share it
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    with _on(dev):
+        check(_L.lmi_mx_product(C.byref(a), _stream(dev)))
+    return y
+
+
+def _mx_common(what, x, weight, act, k):
+    _need_mx(weight, "weight")
+    _no_gradient(what, x)
+    if len(weight.shape) != 2 or weight.shape[1] != k or weight.shape[0] < 1:
+        raise ValueError(f"{what}: weight {tuple(weight.shape)} does not fit inputs of {k} channels (out, in)")
+    if weight.device != x.device:
+        raise ValueError(f"{what}: weight must be on x's device")
+    if act not in _MX_ACTS:
+        raise ValueError(f"{what}: unknown activation {act!r} (None or 'silu')")
+
+
+def _mx_out(what, out, shape, dtype, device, memory_format=torch.contiguous_format):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device, memory_format=memory_format)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device or not out.is_contiguous(memory_format=memory_format):
+        raise ValueError(f"{what}: `out` must be a {dtype} tensor of shape {tuple(shape)} in {memory_format} on x's device")
+    return out
+
+
+def mx_linear(x: Union[torch.Tensor, MxTensor], weight: MxTensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
+              dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x weight^T + bias) with both factors in MXFP4 and fp32 sums: x (..., k) is quantised as `mx_quantize` does it, on the
+    fly, or comes quantised (MxTensor); weight MxTensor (n, k); bias fp32 (n,); act None | 'silu'.
+    dtype: of the result, x's own (which it must be if given) or, for an MxTensor, float32 unless said otherwise.  Inference only."""
+    quantised = isinstance(x, MxTensor)
+    if quantised:
+        _need_mx(x, "x")
+        dtype = dtype or torch.float32
+        if dtype not in _FLOAT_DTYPES:
+            raise TypeError("mx_linear: dtype must be float32, float16 or bfloat16")
+    else:
+        _need_cuda(x, "x")
+        if x.dtype not in _FLOAT_DTYPES:
+            raise TypeError("mx_linear: x must be float32, float16, bfloat16 or an MxTensor")
+        if dtype not in (None, x.dtype):
+            raise ValueError("mx_linear: the result has x's dtype unless x is an MxTensor")
+        dtype = x.dtype
+    if len(x.shape) < 1:
+        raise ValueError("mx_linear: x must be (..., k)")
+    k = x.shape[-1]
+    _mx_common("mx_linear", x.packed if quantised else x, weight, act, k)
+    y = _mx_out("mx_linear", out, tuple(x.shape[:-1]) + (weight.shape[0],), dtype, x.device)
+    m = math.prod(x.shape[:-1])
+    if quantised:
+        return _mx_product("mx_linear", x.packed.data_ptr(), x.scales.data_ptr(), _lib.LMI_MXFP4, 1, m, k, 0, 0, weight, bias, act, y, _lib.LMI_MX_ROWS)
+    stride = k
+    if m:
+        x, _, stride = _rows_of(x)
+    return _mx_product("mx_linear", x.data_ptr(), None, _FLOAT_DTYPES[dtype], 1, m, k, 0, stride, weight, bias, act, y, _lib.LMI_MX_ROWS)
+
+
+def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A 1x1 convolution in MXFP4: x (B, k, H, W) fp32 / fp16 / bf16, quantised on the fly in blocks of 32 channels of a pixel,
+    weight MxTensor (n, k), bias fp32 (n,), act None | 'silu', fp32 sums.  Returns (B, n, H, W) of x's dtype, channels-last
+    if x is.  Channel slices of a larger map (`chunk` along dim 1) are read in place.  Inference only."""
+    _need_cuda(x, "x")
+    if x.dtype not in _FLOAT_DTYPES:
+        raise TypeError("mx_pointwise: x must be float32, float16 or bfloat16")
+    if x.ndim != 4:
+        raise ValueError("mx_pointwise: x must be (B, k, H, W)")
+    b, k, h, w = x.shape
+    _mx_common("mx_pointwise", x, weight, act, k)
+    n = weight.shape[0]
+    sb, sk, sh, sw = x.stride()
+    planes = (w == 1 or sw == 1) and (h == 1 or sh == w * (sw if w > 1 else 1)) and h * w > 1
+    if planes and w == 1 and h > 1:
+        planes = sh == 1
+    rows = (k == 1 or sk == 1) and not planes and (h == 1 or w == 1 or sh == w * sw)
+    if not planes and not rows:
+        x = x.contiguous()
+        sb, sk, sh, sw = x.stride()
+        planes, rows = h * w > 1, h * w <= 1
+    if planes:
+        y = _mx_out("mx_pointwise", out, (b, n, h, w), x.dtype, x.device)
+        return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], b, h * w, k, sb, sk, weight, bias, act, y, _lib.LMI_MX_PLANES)
+    fmt = torch.channels_last if h * w > 1 else torch.contiguous_format   # one pixel: both are the same memory
+    y = _mx_out("mx_pointwise", out, (b, n, h, w), x.dtype, x.device, fmt)
+    if h * w == 1:       # an image per row
+        return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], 1, b, k, 0, sb, weight, bias, act, y, _lib.LMI_MX_ROWS)
+    return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], b, h * w, k, sb, sw if w > 1 else sh, weight, bias, act, y,
+                       _lib.LMI_MX_ROWS)

@@ -1,0 +1,249 @@
+"""class_logprobs against the fp64 oracle: types, layouts, lengths, masked rows, ties, gathered rows."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import class_logprobs as OC
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+ULP = 2.0 ** -24
+
+
+def _ops():
+    from object_detectors_amd import hip_ops
+    return hip_ops
+
+
+def _check(res, x, labels, top, activation, sequential=160):
+    """Tolerances, from the arithmetic: every sum runs over at most `sequential` terms one after another (a lane's share plus the
+    tree over the lanes), each of them with a relative error of a few units (2^-24); the exponential's argument is rounded
+    once (relative error 2 |z| units of e^z, and sum p|z| <= ln C over a row)."""
+    x = x.detach().float().cpu().numpy()
+    ref = OC.evidence(x, None if labels is None else labels.cpu().numpy(), top, activation)
+    c = x.shape[-1]
+    lnc = np.log(c) + 1
+    with np.errstate(all="ignore"):
+        if activation == "softmax":
+            unit = (sequential + 8 + 4 * lnc) * ULP
+            tol_h = unit * (2 + 2 * lnc)
+            tol_lp = lambda v: unit + 4 * ULP * np.abs(v)
+        else:
+            # an answer's entropy has a relative error of some units, |x| more of them through e^-|x| (fp64 of x: the score's logit)
+            a = np.abs(x.astype(np.float64)) if activation == "sigmoid" else np.zeros_like(x, np.float64)
+            h = OC.evidence(x[..., None], None, 0, activation)["entropy"]
+            tol_h = np.where(np.isfinite(a), h * (2 * a + 12 + sequential) * ULP, 0).sum(-1)
+            tol_lp = lambda v: 8 * ULP * np.abs(v) + 2.0 ** -140
+    got = {k: v.cpu().numpy() for k, v in res.items()}
+    assert set(got) == set(ref)
+
+    def close(a, b, tol):
+        same = (a == b) | (np.isnan(a) & np.isnan(b))
+        with np.errstate(all="ignore"):
+            err = np.where(same, 0, np.abs(a.astype(np.float64) - b))
+        assert not np.isnan(err).any() and (err <= np.where(same, 0, tol)).all(), np.nanmax(err - tol)
+
+    close(got["entropy"], ref["entropy"], tol_h)
+    if labels is not None:
+        close(got["logprob"], ref["logprob"], tol_lp(ref["logprob"]))
+    if top:
+        assert np.array_equal(got["top_index"], ref["top_index"])
+        close(got["top_logprob"], ref["top_logprob"], tol_lp(ref["top_logprob"]))
+
+
+def _rows(seed, n, c, dtype, activation, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, c, generator=g) * scale
+    if activation == "none":
+        x = torch.sigmoid(x)
+    return x.to(dtype).cuda(), torch.randint(0, c, (n,), generator=g).cuda()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", ["softmax", "sigmoid", "none"])
+@pytest.mark.parametrize("n,c,top", [(1, 1, 1), (3, 2, 2), (7, 8, 0), (5, 9, 9), (300, 80, 5), (2, 1000, 32), (4, 1021, 7), (3, 1025, 3),
+                                     (5, 4099, 16), (3, 8192, 0), (130, 8193, 1), (129, 16500, 10), (2, 40003, 32), (1, 270001, 20)])
+def test_rows(n, c, top, activation, dtype):
+    x, labels = _rows(n * 1000 + c, n, c, DTYPES[dtype], activation)
+    _check(_ops().class_logprobs(x, labels, top=top, activation=activation), x, labels, top, activation)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", ["softmax", "sigmoid", "none"])
+@pytest.mark.parametrize("b,g,c,a,top", [(1, 1, 1, 1, 1), (2, 4, 16, 525, 2), (3, 1, 80, 1701, 5), (1, 2, 63, 4097, 32), (2, 1, 300, 2100, 8),
+                                         (1, 1, 200, 70, 4)])
+def test_planes(b, g, c, a, top, activation, dtype):
+    """Class planes (the head's layout, distance bins): classes lie `a` apart."""
+    gen = torch.Generator().manual_seed(c)
+    planes = torch.randn(b, g * c, a, generator=gen) * 2
+    if activation == "none":
+        planes = torch.sigmoid(planes)
+    x = planes.to(DTYPES[dtype]).cuda().view(b, g, c, a).transpose(2, 3)
+    labels = torch.randint(0, c, (b, g, a), generator=gen).to(torch.int32).cuda()
+    _check(_ops().class_logprobs(x, labels, top=min(top, c), activation=activation), x, labels, min(top, c), activation, sequential=c + 8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,nc,a,m,top,activation", [(1, 80, 8400, 300, 5, "none"), (4, 3, 525, 17, 3, "sigmoid"), (2, 131, 1701, 64, 32, "softmax"),
+                                                     (2, 1, 40, 5, 1, "none")])
+def test_gathered(b, nc, a, m, top, activation, dtype):
+    """Rows at NMS anchors, labels from the class column of the NMS rows, per-image counts; rows behind a count stay."""
+    gen = torch.Generator().manual_seed(nc)
+    head = torch.randn(b, 4 + nc + 3, a, generator=gen) * 2
+    if activation == "none":
+        head = torch.sigmoid(head)
+    head = head.to(DTYPES[dtype]).cuda()
+    index = torch.randint(0, a, (b, m), generator=gen).to(torch.int32).cuda()
+    index[:, -1] = index[:, 0]     # the same anchor twice
+    count = torch.tensor([m, 0, m // 2, 1][:b], dtype=torch.int32).cuda()
+    det = torch.randn(b, m, 9, generator=gen).cuda()
+    det[:, :, 5] = torch.randint(0, nc, (b, m), generator=gen).float().cuda()
+    out = {"logprob": torch.full((b, m), 7.0).cuda(), "entropy": torch.full((b, m), 7.0).cuda(),
+           "top_logprob": torch.full((b, m, top), 7.0).cuda(), "top_index": torch.full((b, m, top), 7, dtype=torch.int32).cuda()}
+    res = _ops().class_logprobs(head[:, 4:4 + nc].transpose(1, 2), det[:, :, 5], top=top, activation=activation, index=index, count=count, out=out)
+    assert all(res[k] is out[k] for k in out)
+    for i in range(b):
+        n = int(count[i])
+        x = head[i, 4:4 + nc].t()[index[i, :n].long()]
+        if n:
+            _check({k: v[i, :n] for k, v in res.items()}, x, det[i, :n, 5].long(), top, activation)
+        for v in res.values():
+            assert (v[i, n:] == 7).all()
+
+
+@pytest.mark.parametrize("c", [5, 100, 1500, 20000, 70000])
+@pytest.mark.parametrize("layout", ["rows", "planes"])
+def test_masked_and_odd_values(c, layout):
+    """Masked classes, rows with nothing left, the type's lowest value as a mask, equal values, infinities and NaN."""
+    gen = torch.Generator().manual_seed(c)
+    x = torch.randn(12, c, generator=gen)
+    x[1, torch.rand(c, generator=gen) < 0.9] = -float("inf")
+    x[2] = -float("inf")                                  # nothing left
+    x[3] = torch.finfo(torch.float32).min                 # masked by the lowest value, all of it
+    x[4, 1:] = torch.finfo(torch.float32).min
+    x[5] = 1.5                                            # all equal
+    x[6] = torch.randint(0, 3, (c,), generator=gen).float()
+    x[7, c // 2] = float("nan")
+    x[8, c // 2] = float("inf")
+    x[9] = torch.tensor([0.0, -0.0]).repeat((c + 1) // 2)[:c]
+    x[10] = -float("inf")
+    x[10, c - 1] = 3.0                                    # one class left
+    x[11] = torch.arange(c).flip(0) * 0.001               # sorted
+    x = x.cuda()
+    if layout == "planes":
+        x = x.t().contiguous().t()
+    labels = torch.randint(0, c, (12,), generator=gen).cuda()
+    for top in (0, min(c, 4), min(c, 32)):
+        _check(_ops().class_logprobs(x, labels, top=top), x, labels, top, "softmax", sequential=160 if layout == "rows" or c > 64 else c + 8)
+    _check(_ops().class_logprobs(x, labels, top=2, activation="sigmoid"), x, labels, 2, "sigmoid")
+
+
+def test_probabilities_at_the_borders():
+    x = torch.tensor([[0.0, 1.0, 0.5, 2.0 ** -24, 1 - 2.0 ** -24, 6e-8], [0.0] * 6, [1.0] * 6, [0.5, float("nan"), 0.25, 0.1, 0.2, 0.3]]).cuda()
+    for label in range(6):
+        labels = torch.full((4,), label).cuda()
+        _check(_ops().class_logprobs(x, labels, top=6, activation="none"), x, labels, 6, "none")
+
+
+def test_many_best_in_few_lanes():
+    """The best values sit where a few lanes hold them all (every 64th group of a tile): the candidate table overflows."""
+    for n, c in ((1, 8000), (2, 16000), (3, 900)):
+        x = torch.randn(n, c)
+        at = torch.arange(c)
+        x[:, (at // 8) % 64 == 5] += 100.0
+        x = x.bfloat16().cuda()
+        labels = torch.zeros(n, dtype=torch.int64).cuda()
+        _check(_ops().class_logprobs(x, labels, top=32), x, labels, 32, "softmax")
+
+
+def test_labels_and_shapes():
+    ops = _ops()
+    x, labels = _rows(1, 6, 50, torch.float32, "softmax")
+    bad = torch.tensor([-1, 50, 3, 1 << 40, -(1 << 40), 0]).cuda()
+    _check(ops.class_logprobs(x, bad), x, bad, 0, "softmax")
+    lp = ops.class_logprobs(x, torch.tensor([float("nan"), 1.0, -3.0, 1e20, 49.0, 50.0]).cuda())["logprob"].cpu()
+    assert torch.isnan(lp[[0, 2, 3, 5]]).all() and not torch.isnan(lp[[1, 4]]).any()
+    assert set(ops.class_logprobs(x)) == {"entropy"}
+    one = ops.class_logprobs(x[0], labels[0], top=3)                      # a single row without leading dimensions
+    assert one["entropy"].shape == () and one["top_index"].shape == (3,)
+    empty = ops.class_logprobs(x[:0], labels[:0], top=3)
+    assert empty["entropy"].shape == (0,) and empty["top_index"].shape == (0, 3)
+    wide = torch.randn(4, 3, 5, 64).cuda().permute(2, 0, 1, 3)            # strides two of which cannot say: copied
+    lab = torch.randint(0, 64, (5, 4, 3)).cuda()
+    _check(ops.class_logprobs(wide, lab, top=2), wide, lab, 2, "softmax")
+    same = x[:1].expand(6, 50)                                            # broadcast rows, broadcast classes
+    _check(ops.class_logprobs(same, labels, top=2), same, labels, 2, "softmax")
+    flat = x[:, :1].expand(6, 50)
+    _check(ops.class_logprobs(flat, labels, top=2), flat, labels, 2, "softmax")
+    every = x[:, ::3]                                                     # a class stride that is neither 1 nor a plane
+    _check(ops.class_logprobs(every, labels % 17, top=2), every, labels % 17, 2, "softmax")
+
+
+def test_offset_rows_keep_alignment_rules():
+    """Rows that start at every offset inside 16 bytes."""
+    base = torch.randn(40000).half().cuda()
+    for off in range(9):
+        for c in (1, 7, 513, 2049, 9001):
+            x = base[off:off + 3 * c].view(3, c)
+            labels = torch.tensor([0, c - 1, c // 2]).cuda()
+            _check(_ops().class_logprobs(x, labels, top=min(c, 4)), x, labels, min(c, 4), "softmax")
+
+
+def test_bad_index_gives_nan():
+    ops = _ops()
+    x = torch.randn(1, 30, 6).cuda()
+    index = torch.tensor([[-1, 30, 29, 2 ** 31 - 1, 0]], dtype=torch.int32).cuda()
+    r = ops.class_logprobs(x, torch.zeros(1, 5, dtype=torch.int64).cuda(), top=2, index=index)
+    for k in ("logprob", "entropy"):
+        assert torch.isnan(r[k][0, [0, 1, 3]]).all() and not torch.isnan(r[k][0, [2, 4]]).any()
+    assert (r["top_index"][0, [0, 1, 3]] == -1).all() and (r["top_index"][0, [2, 4]] >= 0).all()
+
+
+def test_far_rows_of_a_large_tensor():
+    """Offsets beyond 2^32 bytes and 2^31 elements."""
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    c, n = 1 << 16, (1 << 15) + 40
+    x = torch.zeros(n, c, dtype=torch.float16, device="cuda")
+    x[-3:].copy_(torch.randn(3, c))
+    labels = torch.arange(3).cuda()
+    _check(_ops().class_logprobs(x[-3:], labels, top=3), x[-3:], labels, 3, "softmax")
+    r = _ops().class_logprobs(x, torch.zeros(n, dtype=torch.int64, device="cuda"))
+    _check({k: v[-3:] for k, v in r.items()}, x[-3:], torch.zeros(3, dtype=torch.int64), 0, "softmax")
+
+
+def test_captured_and_replayed():
+    ops = _ops()
+    x, labels = _rows(3, 2, 50001, torch.float32, "softmax")
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ops.class_logprobs(x, labels, top=5)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = ops.class_logprobs(x, labels, top=5)
+    for i in range(3):
+        x.copy_(torch.randn(2, 50001) * (i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(res, x, labels, 5, "softmax")
+        eager = ops.class_logprobs(x, labels, top=5)
+        assert all(torch.equal(res[k], eager[k]) for k in res)
+
+
+def test_two_streams_agree():
+    """A long row on two streams at once: the parts' workspaces are the calls' own; the results have the same bits every time."""
+    ops = _ops()
+    data = [_rows(s, 3, 100003, torch.bfloat16, "softmax") for s in (1, 2)]
+    want = [ops.class_logprobs(x, l, top=8) for x, l in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    got = [[], []]
+    for _ in range(10):
+        for i, (x, l) in enumerate(data):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.class_logprobs(x, l, top=8))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(r[k], want[i][k]) for k in r)

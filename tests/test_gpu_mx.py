@@ -1,0 +1,195 @@
+"""MXFP4: quantising against the fp64 oracle bit for bit, products within the error bound of an fp32 sum."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx as OM
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _ops():
+    from object_detectors_amd import hip_ops
+    return hip_ops
+
+
+def _np(t):
+    return t.detach().float().cpu().numpy().astype(np.float64)
+
+
+def _same_blocks(q, x):
+    """Scales equal everywhere, codes wherever the scale is a number."""
+    codes, scales = OM.quantize(_np(x).reshape(-1, x.shape[-1]))
+    assert np.array_equal(q.scales.cpu().numpy(), scales)
+    live = np.repeat(scales != 255, 32, axis=1)
+    assert np.array_equal(OM.unpack(q.packed.cpu().numpy())[live], codes[live])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 31), (2, 32), (5, 33), (64, 80), (7, 400), (130, 2560), (1, 5000), (2049, 96)])
+def test_quantize(rows, k, dtype):
+    g = torch.Generator().manual_seed(rows * 7 + k)
+    x = torch.randn(rows, k, generator=g) * torch.exp2(torch.randint(-8, 9, (rows, 1), generator=g).float())
+    x = x.to(DTYPES[dtype]).cuda()
+    q = _ops().mx_quantize(x)
+    _same_blocks(q, x)
+    want = OM.values(_np(x))
+    for out in DTYPES.values():       # scale 2^e x {0 .. 6}: exact in every type here (fp16: exponents within its range)
+        assert np.array_equal(_np(_ops().mx_dequantize(q, out)), torch.from_numpy(want).to(out).double().numpy())
+
+
+def test_quantize_every_step():
+    """Every midpoint and its neighbours at several scales, subnormals, the ends of the range, zeros, non-finite blocks."""
+    u = np.concatenate([np.arange(0, 8, 0.25), np.nextafter(np.arange(0.25, 8, 0.25, dtype=np.float32), np.float32(9)),
+                        np.nextafter(np.arange(0.25, 8, 0.25, dtype=np.float32), np.float32(0))]).astype(np.float32)
+    rows = []
+    for e in (-126, -125, -60, -1, 0, 1, 90, 125):
+        v = (u * np.float32(2.0) ** e).astype(np.float32)
+        for i in range(0, len(v), 30):
+            part = v[i:i + 30]
+            rows.append(np.concatenate([part, -part[:32 - len(part)], np.zeros(max(0, 32 - 2 * len(part)), np.float32)])[:32])
+    tiny = np.full(32, np.float32(1e-45)); tiny[3] = -7e-45
+    odd = [np.zeros(32), -np.zeros(32), tiny, np.full(32, 2.0 ** -127), np.full(32, 3.4028235e38), np.r_[np.inf, np.ones(31)],
+           np.r_[np.ones(31), np.nan], np.full(32, -np.inf)]
+    x = torch.from_numpy(np.stack(rows + [np.asarray(o, np.float32) for o in odd]).astype(np.float32)).cuda()
+    q = _ops().mx_quantize(x)
+    _same_blocks(q, x)
+    y = _ops().mx_dequantize(q).cpu().numpy()
+    want = OM.values(_np(x)).astype(np.float32)
+    assert np.array_equal(y, want, equal_nan=True)
+    assert np.isnan(y[-3:]).all()
+
+
+def test_quantize_strides_and_shapes():
+    ops = _ops()
+    x = torch.randn(6, 10, 100).cuda()
+    for v in (x[:, :, 5:77], x[::2], x.transpose(0, 1), x.transpose(1, 2), x[:, 3], x[0, 0], x[:, :, ::2], x[:0]):
+        q = ops.mx_quantize(v)
+        assert q.shape == v.shape
+        if v.numel():
+            _same_blocks(q, v)
+        assert ops.mx_dequantize(q).shape == v.shape
+
+
+def _close(got, want, size, k, dtype, act):
+    """fp32 sums of k products of at most `size` in all: k + 8 roundings of 2^-24 each at most (2^-23 where the matrix
+    instruction cuts instead of rounding); SiLU's slope is below 1.1 and its own error some units; then one rounding to the type."""
+    tol = (k + 8) * 2.0 ** -23 * size * (1.1 if act else 1.0)
+    if act:
+        tol = tol + 8 * 2.0 ** -24 * np.abs(want)
+    tol = tol + (np.abs(want) + tol) * torch.finfo(dtype).eps / 2 + (6e-8 if dtype == torch.float16 else 1e-37)
+    got = _np(got)
+    assert got.shape == want.shape
+    both = np.isnan(got) & np.isnan(want)
+    assert (np.isnan(got) == np.isnan(want)).all()
+    err = np.where(both, 0, np.abs(got - want))
+    assert (err <= np.where(both, 0, tol)).all(), (np.nanmax(err), np.nanmax(err / np.maximum(tol, 1e-300)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 1280, 1000), (2, 33, 5), (5, 80, 80), (17, 400, 160), (64, 64, 32), (65, 96, 33), (300, 2560, 64),
+                                   (1000, 160, 75), (3, 9000, 40), (129, 5000, 130), (700, 640, 640)])
+def test_linear(m, k, n, act, dtype):
+    ops, dt = _ops(), DTYPES[dtype]
+    g = torch.Generator().manual_seed(m + k + n)
+    x = (torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-3, 4, (m, 1), generator=g).float())).to(dt).cuda()
+    w = torch.randn(n, k, generator=g).cuda() / k ** 0.5
+    bias = torch.randn(n, generator=g).cuda() if k % 2 == 0 else None
+    wq = ops.mx_quantize(w)
+    want, size = OM.product(_np(x), _np(w), None if bias is None else _np(bias), act)
+    y = ops.mx_linear(x, wq, bias, act=act)
+    assert y.dtype == dt
+    _close(y, want, size, k, dt, act)
+    z = ops.mx_linear(ops.mx_quantize(x), wq, bias, act=act, dtype=dt)
+    _close(z, want, size, k, dt, act)
+    out = torch.empty_like(y)
+    assert ops.mx_linear(x, wq, bias, act=act, out=out) is out and torch.equal(out, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["planes", "channels_last", "slice"])
+@pytest.mark.parametrize("b,k,n,h,w,act", [(1, 1, 1, 1, 1, None), (1, 640, 640, 20, 20, "silu"), (3, 400, 75, 7, 13, "silu"), (2, 48, 16, 1, 5, None),
+                                           (2, 33, 40, 9, 1, "silu"), (4, 96, 64, 40, 24, None), (1, 80, 32, 160, 96, "silu"), (5, 64, 80, 1, 1, "silu"),
+                                           (1, 2600, 70, 3, 11, None), (2, 5000, 33, 4, 4, "silu")])
+def test_pointwise(b, k, n, h, w, act, layout, dtype):
+    ops, dt = _ops(), DTYPES[dtype]
+    g = torch.Generator().manual_seed(k + n)
+    x = torch.randn(b, k, h, w, generator=g).to(dt).cuda()
+    if layout == "channels_last":
+        x = x.contiguous(memory_format=torch.channels_last)
+    elif layout == "slice":           # channels k.. of a map twice as deep, as `chunk` leaves them
+        x = torch.cat([torch.full_like(x, float("nan")), x], 1)[:, k:]
+    wt = torch.randn(n, k, generator=g).cuda() / k ** 0.5
+    bias = torch.randn(n, generator=g).cuda()
+    y = ops.mx_pointwise(x, ops.mx_quantize(wt), bias, act=act)
+    assert y.shape == (b, n, h, w) and y.dtype == dt
+    if layout == "channels_last" and h * w > 1 and k > 1:
+        assert y.is_contiguous(memory_format=torch.channels_last)
+    want, size = OM.product(_np(x.permute(0, 2, 3, 1)).reshape(-1, k), _np(wt), _np(bias), act)
+    _close(y.permute(0, 2, 3, 1).reshape(-1, n), want, size, k, dt, act)
+
+
+def test_pointwise_odd_strides():
+    ops = _ops()
+    w = torch.randn(24, 40).cuda()
+    wq = ops.mx_quantize(w)
+    base = torch.randn(3, 44, 12, 18).half().cuda()
+    for x in (base[:, :40, :, 1:], base[:, :40, ::2], base[:, 2:42].transpose(2, 3), base[:, :40, :, :1], base[:, :40, 3:4], base.transpose(0, 1)[:40].transpose(0, 1),
+              base[:, :40].flip(3)):
+        want, size = OM.product(_np(x.permute(0, 2, 3, 1)).reshape(-1, 40), _np(w))
+        _close(ops.mx_pointwise(x, wq).permute(0, 2, 3, 1).reshape(-1, 24), want, size, 40, torch.float16, None)
+
+
+def test_non_finite_blocks_stay_in_their_row():
+    """A NaN or an infinity makes the results of its own position NaN, and no other's."""
+    ops = _ops()
+    x = torch.randn(70, 100)
+    x[3, 50] = float("nan")
+    x[40, 99] = float("inf")
+    w = torch.randn(50, 100)
+    y = ops.mx_linear(x.cuda(), ops.mx_quantize(w.cuda()))
+    bad = torch.isnan(y).cpu()
+    assert bad[[3, 40]].all() and bad.sum() == 100
+    w[7, 0] = float("-inf")
+    bad = torch.isnan(ops.mx_linear(x.cuda(), ops.mx_quantize(w.cuda()))).cpu()
+    assert bad[:, 7].all() and bad.sum() == 100 + 68
+    p = ops.mx_pointwise(x.t().reshape(1, 100, 70, 1).half().cuda(), ops.mx_quantize(w.cuda()))
+    assert torch.isnan(p[0, 7]).all() and int(torch.isnan(p).sum()) == 100 + 68
+
+
+def test_empty_and_out():
+    ops = _ops()
+    wq = ops.mx_quantize(torch.randn(8, 32).cuda())
+    assert ops.mx_linear(torch.empty(0, 32).cuda(), wq).shape == (0, 8)
+    assert ops.mx_linear(ops.mx_quantize(torch.empty(0, 32).cuda()), wq).shape == (0, 8)
+    assert ops.mx_pointwise(torch.empty(2, 32, 0, 4).cuda(), wq).shape == (2, 8, 0, 4)
+    x = torch.randn(2, 32, 6, 6).cuda()
+    guard = torch.full((2 * 8 * 36 + 64,), 5.0).cuda()          # nothing is written beside the result
+    out = guard[32:32 + 2 * 8 * 36].view(2, 8, 6, 6)
+    ops.mx_pointwise(x, wq, out=out)
+    assert (guard[:32] == 5).all() and (guard[-32:] == 5).all()
+    assert torch.equal(out, ops.mx_pointwise(x, wq))
+
+
+def test_captured_and_replayed():
+    ops = _ops()
+    wq = ops.mx_quantize(torch.randn(64, 96).cuda())
+    big = ops.mx_quantize(torch.randn(640, 1280).cuda())
+    x, r = torch.randn(2, 96, 10, 10).half().cuda(), torch.randn(1, 1280).half().cuda()
+
+    def step():
+        return ops.mx_pointwise(x, wq, act="silu"), ops.mx_linear(r, big), ops.mx_linear(ops.mx_quantize(x.permute(0, 2, 3, 1)), wq)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for i in range(3):
+        x.copy_(torch.randn(2, 96, 10, 10))
+        r.copy_(torch.randn(1, 1280))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(res, step()):
+            assert torch.equal(a, b)

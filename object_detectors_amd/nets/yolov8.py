@@ -32,6 +32,39 @@ class ConvBNAct(nn.Module):
         return self.act(self.bn(self.conv(x)))
 
 
+class MxPointwise(nn.Module):
+    """A 1x1 convolution with its batch norm (folded) and SiLU, weights and activations in MXFP4 (hip_ops.mx_pointwise):
+    4.25 bits per weight, one pass over the activations instead of the three of convolution, norm and activation.
+    GPU only, inference only."""
+
+    def __init__(self, weight, bias, act):
+        super().__init__()
+        from .. import hip_ops
+        q = hip_ops.mx_quantize(weight)
+        self.register_buffer("packed", q.packed)
+        self.register_buffer("scales", q.scales)
+        self.register_buffer("bias", bias.float().contiguous())
+        self.size, self.act = tuple(weight.shape), act
+
+    @classmethod
+    def of(cls, m):
+        """From a ConvBNAct or an nn.Conv2d with a 1x1 kernel."""
+        conv = m.conv if isinstance(m, ConvBNAct) else m
+        w = conv.weight.detach().float().flatten(1)
+        bias = torch.zeros(w.shape[0], device=w.device) if conv.bias is None else conv.bias.detach().float()
+        act = None
+        if isinstance(m, ConvBNAct):
+            gain = m.bn.weight.detach().float() / torch.sqrt(m.bn.running_var.float() + m.bn.eps)
+            w, bias = w * gain.unsqueeze(1), (bias - m.bn.running_mean.float()) * gain + m.bn.bias.detach().float()
+            act = "silu" if isinstance(m.act, nn.SiLU) else None
+        return cls(w, bias, act)
+
+    def forward(self, x):
+        from .. import hip_ops
+        bias = self.bias if self.bias.dtype == torch.float32 else self.bias.float()   # .half() of the whole model reaches buffers too
+        return hip_ops.mx_pointwise(x, hip_ops.MxTensor(self.packed, self.scales, self.size), bias, act=self.act)
+
+
 class Bottleneck(nn.Module):
     def __init__(self, c, shortcut=True):
         super().__init__()
@@ -180,6 +213,26 @@ class YoloV8(nn.Module):
         self.names = names or {i: f"class{i}" for i in range(nc)}
         self.fp16 = False
         self.stride = 32
+
+    @torch.no_grad()
+    def quantize_pointwise(self, head=False):
+        """Replaces the 1x1 convolutions of backbone and neck (head=True: the head's last layers too) by their MXFP4 form, in
+        place.  The model must be in eval mode and on the GPU.  Returns how many were replaced."""
+        if self.training:
+            raise RuntimeError("quantize_pointwise folds the batch norms: call eval() first")
+        todo = []
+        for name, parent in self.named_modules():
+            if not head and (name == "head" or name.startswith("head.")):
+                continue
+            if isinstance(parent, ConvBNAct):
+                continue
+            for key, m in parent.named_children():
+                conv = m.conv if isinstance(m, ConvBNAct) else m
+                if isinstance(conv, nn.Conv2d) and conv.kernel_size == (1, 1) and conv.stride == (1, 1) and conv.groups == 1:
+                    todo.append((parent, key, m))
+        for parent, key, m in todo:
+            setattr(parent, key, MxPointwise.of(m))
+        return len(todo)
 
     def forward(self, x):
         x = self.b2(self.b1(self.b0(x)))

@@ -78,6 +78,12 @@ class Yolov8Core:
     # forward pass still running).  Set sync_time_info = True to synchronise at every stage boundary: the figures are
     # then the stages' real durations, at the cost of the overlap between host and device.
     sync_time_info = False
+    # > 0: results also carry, per detection, 'logprobs' (log probability of its class), 'entropy' (summed over the classes'
+    # yes / no answers) and 'alternatives' (that many best classes as (name, log probability), best first) -- one more
+    # kernel on the rows NMS kept (hip_ops.class_logprobs).
+    alternatives = 0
+    # True: the network's 1x1 convolutions (backbone and neck) run in MXFP4 (this package's own networks; set before construction)
+    mx_weights = False
 
     def _init(self, weights: str, device='gpu', data=None, fp16=False):
         if not os.path.isfile(weights):
@@ -90,6 +96,10 @@ class Yolov8Core:
                 self.logger.warning('GPU not available, using CPU')
         self.model = load_backend(weights, self.device, data=data, fp16=fp16)
         self.model.eval()
+        if self.mx_weights:
+            if not hasattr(self.model, 'quantize_pointwise'):
+                raise TypeError(f'mx_weights needs one of this package\'s networks, not {type(self.model).__name__}')
+            self.model.quantize_pointwise()
         self.names = self.model.names
         self._thres_cache = {}
 
@@ -245,6 +255,32 @@ class Yolov8Core:
             self._thres_cache = {key: t}
         return t
 
+    # ---- additive: evidence of the kept detections ----------------------------------------------
+    _EVIDENCE = ('logprobs', 'entropy', 'alternatives')
+
+    def _evidence(self, preds, det, count, anchor, nc):
+        """[logprob, entropy, top_logprob, top_index] of the NMS rows on the device, [] unless `alternatives` is set."""
+        k = min(int(self.alternatives), nc)
+        if k <= 0:
+            return []
+        r = _hip_ops().class_logprobs(preds[:, 4:4 + nc].transpose(1, 2), det[:, :, 5], top=k, activation='none', index=anchor, count=count)
+        return [r["logprob"], r["entropy"], r["top_logprob"], r["top_index"]]
+
+    def _add_evidence(self, results, ev_dev, ev_h, i, n, M, return_tensor):
+        """Entries of image i (rows M of its n) for what `_evidence` returned and its host copies."""
+        if not ev_dev:
+            return
+        if return_tensor:
+            sel = torch.from_numpy(np.nonzero(M)[0]).to(ev_dev[0].device)
+            lp, h = (t[i, :n][sel] for t in ev_dev[:2])
+        else:
+            lp, h = (t[i, :n][M] for t in ev_h[:2])
+        results['logprobs'].append(lp)
+        results['entropy'].append(h)
+        names = self.model.names
+        results['alternatives'].append([[(names[int(c)], float(v)) for c, v in zip(cs, vs)]
+                                        for cs, vs in zip(ev_h[3][i, :n][M], ev_h[2][i, :n][M])])
+
     # ---- postprocess (model.py:178-252) ----------------------------------------------------------
     @torch.inference_mode()
     def postprocess(self, preds, img, orig_imgs, conf: Union[float, dict], iou=0.45, agnostic=False, max_det=300, return_segments=True,
@@ -280,13 +316,15 @@ class Yolov8Core:
         # its epilogue (-> the slot prefix when masks follow); an fp16 head is read as it is
         any_tensor = any(isinstance(orig_of(i), torch.Tensor) for i in range(B))
         with_slots = predict_mask or any_tensor    # the dense survivor order also serves the one-gather tensor output
-        det, count, _, fin = ops.nms_v8(preds, float(conf2), float(iou), agnostic=bool(agnostic), max_det=int(max_det), nc=nc,
-                                        finalize=dict(model_hw=model_hw, orig_hw=ohw, thres=thres, with_slots=with_slots))
+        det, count, anchor, fin = ops.nms_v8(preds, float(conf2), float(iou), agnostic=bool(agnostic), max_det=int(max_det), nc=nc,
+                                             finalize=dict(model_hw=model_hw, orig_hw=ohw, thres=thres, with_slots=with_slots))
+        evidence = self._evidence(preds, det, count, anchor, nc)
         # ONE synchronisation: counts, keep flags, the six box columns (and the mask slots) land in pinned host
         # buffers by asynchronous copies, then the stream is waited for once
         fetch = [count, fin["keep"], det[:, :, :6]] + ([fin["slot_base"]] if with_slots else [])
-        host = self._to_host(fetch)
+        host = self._to_host(fetch + evidence)
         count_h, keep_h, det_h = host[0], host[1].astype(bool), host[2]
+        evidence = (evidence, host[len(fetch):])
         masks_by_image = [None] * B
         slot_base = host[3] if with_slots else None
         rows_dev = None
@@ -302,7 +340,7 @@ class Yolov8Core:
                 masks_by_image = ops.process_mask_ragged(proto.to(self.device), det, fin["slot_map"], fin["slot_base"], shapes,
                                                          [int(slot_base[i + 1] - slot_base[i]) for i in range(B)], self.mask_dtype)
         return self._assemble(rows_dev, slot_base, det_h, count_h, keep_h, masks_by_image, orig_imgs, predict_mask, return_segments,
-                              _masks_on_device, _with_index)
+                              _masks_on_device, _with_index, evidence)
 
     def _now(self) -> float:
         if self.sync_time_info and self.device.type == 'cuda':
@@ -339,7 +377,7 @@ class Yolov8Core:
         return [b.numpy() for b in out]
 
     def _assemble(self, rows_dev, slot_base, det_h, count_h, keep_h, masks_by_image, orig_imgs, predict_mask, return_segments,
-                  masks_on_device=False, with_index=False):
+                  masks_on_device=False, with_index=False, evidence=([], [])):
         """Result dict exactly as model.py:214-252 builds it (images with no NMS survivor add no entry).
         masks_on_device: leave the masks of numpy-input images on the GPU (predict reverts them there first).
         with_index: add the key 'image_index' (batch position of every entry), which the skip-empty rule loses."""
@@ -374,6 +412,7 @@ class Yolov8Core:
                 results['boxes'].append(det_h[i, :n, :4][M])
                 results['scores'].append(det_h[i, :n, 4][M])
             results['classes'].append(classes[M].tolist())
+            self._add_evidence(results, *evidence, i, n, M, return_tensor)
         return results
 
     # ---- predict (model.py:256-324) --------------------------------------------------------------
@@ -412,6 +451,7 @@ class Yolov8Core:
         results_dict['boxes'] = pipeline_utils.revert_to_origin(boxes, operators)
         results_dict['scores'] = scores
         results_dict['classes'] = classes
+        results_dict.update({k: results[k][0] for k in self._EVIDENCE if k in results})
         time_info['postproc'] = self._now() - t0
         return results_dict, time_info
 
@@ -498,9 +538,10 @@ class Yolov8PoseCore(Yolov8Core):
         ohw = shapes[0] if all(s == shapes[0] for s in shapes) else torch.tensor(shapes, dtype=torch.int32, device=self.device)
         # ONE launch chain, like det / seg: scale_boxes + clip, the class threshold and scale_coords on the keypoint columns
         # run in the suppression kernel's epilogue (reference: three passes over the rows, model.py:555-569)
-        det, count, _, fin = ops.nms_v8(preds, float(conf2), float(iou), agnostic=bool(agnostic), max_det=int(max_det), nc=nc,
-                                        finalize=dict(model_hw=model_hw, orig_hw=ohw, thres=thres, with_slots=False, kpt=(6, nkpt, ndim)))
-        count_h, keep_h, det_h = self._to_host([count, fin["keep"], det])   # pinned, asynchronous, ONE synchronisation
+        det, count, anchor, fin = ops.nms_v8(preds, float(conf2), float(iou), agnostic=bool(agnostic), max_det=int(max_det), nc=nc,
+                                             finalize=dict(model_hw=model_hw, orig_hw=ohw, thres=thres, with_slots=False, kpt=(6, nkpt, ndim)))
+        evidence = self._evidence(preds, det, count, anchor, nc)
+        count_h, keep_h, det_h, *evidence_h = self._to_host([count, fin["keep"], det] + evidence)   # pinned, asynchronous, ONE synchronisation
         keep_h = keep_h.astype(bool)
         results = collections.defaultdict(list)
         names = self.model.names
@@ -523,6 +564,7 @@ class Yolov8PoseCore(Yolov8Core):
                 results['scores'].append(rows[:, 4])
                 results['points'].append(rows[:, 6:].reshape(len(rows), nkpt, ndim))
             results['classes'].append(classes[M].tolist())
+            self._add_evidence(results, evidence, evidence_h, i, n, M, isinstance(orig_img, torch.Tensor))
         return results
 
     @torch.inference_mode()
@@ -553,6 +595,7 @@ class Yolov8PoseCore(Yolov8Core):
         results_dict['boxes'] = pipeline_utils.revert_to_origin(boxes, operators)
         results_dict['scores'] = scores
         results_dict['classes'] = classes
+        results_dict.update({k: results[k][0] for k in self._EVIDENCE if k in results})
         time_info['postproc'] = self._now() - t0
         return results_dict, time_info
 
@@ -580,10 +623,11 @@ class Yolov8ObbCore(Yolov8Core):
         model_hw = tuple(img.shape[2:])
         shapes = [tuple((orig_imgs[i] if isinstance(orig_imgs, list) else orig_imgs).shape[:2]) for i in range(B)]
         ohw = shapes[0] if all(s == shapes[0] for s in shapes) else torch.tensor(shapes, dtype=torch.int32, device=self.device)
-        det, count, _ = ops.nms_v8(preds, float(conf2), float(iou), agnostic=bool(agnostic), max_det=int(max_det), nc=nc, rotated=True)
+        det, count, anchor = ops.nms_v8(preds, float(conf2), float(iou), agnostic=bool(agnostic), max_det=int(max_det), nc=nc, rotated=True)
+        evidence = self._evidence(preds, det, count, anchor, nc)
         fin = ops.finalize_obb(det, count, nc, model_hw, ohw, thres)
         corners = fin["corners"]
-        count_h, keep_h, det_h, corners_h = self._to_host([count, fin["keep"], det[:, :, :6], corners])   # ONE synchronisation
+        count_h, keep_h, det_h, corners_h, *evidence_h = self._to_host([count, fin["keep"], det[:, :, :6], corners] + evidence)   # ONE synchronisation
         keep_h = keep_h.astype(bool)
         results = collections.defaultdict(list)
         names = self.model.names
@@ -602,6 +646,7 @@ class Yolov8ObbCore(Yolov8Core):
                 results['boxes'].append(corners_h[i, :n][M])
                 results['scores'].append(det_h[i, :n, 4][M])
             results['classes'].append(classes[M].tolist())
+            self._add_evidence(results, evidence, evidence_h, i, n, M, isinstance(orig_img, torch.Tensor))
         return results
 
     @torch.inference_mode()
@@ -629,5 +674,6 @@ class Yolov8ObbCore(Yolov8Core):
         results_dict['boxes'] = boxes
         results_dict['scores'] = scores
         results_dict['classes'] = classes
+        results_dict.update({k: results[k][0] for k in self._EVIDENCE if k in results})
         time_info['postproc'] = self._now() - t0
         return results_dict, time_info

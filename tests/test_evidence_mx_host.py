@@ -1,0 +1,116 @@
+"""Refusals of class_logprobs and the MXFP4 operators that need no GPU, and the oracles against hand-made values."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import class_logprobs as OC, mx as OM
+
+
+@pytest.fixture(scope="module")
+def L():
+    from object_detectors_amd import _lib
+    return _lib
+
+
+def test_cpu_tensors_are_refused():
+    from object_detectors_amd import hip_ops as ops
+    from object_detectors_amd.nets.yolov8 import YoloV8
+    with pytest.raises(TypeError, match="GPU"):
+        ops.class_logprobs(torch.zeros(2, 3))
+    with pytest.raises(TypeError, match="GPU"):
+        ops.mx_quantize(torch.zeros(2, 32))
+    q = ops.MxTensor(torch.zeros(2, 16, dtype=torch.uint8), torch.zeros(2, 1, dtype=torch.uint8), (2, 30))
+    with pytest.raises(TypeError, match="GPU"):
+        ops.mx_dequantize(q)
+    with pytest.raises(TypeError, match="GPU"):
+        ops.mx_linear(torch.zeros(1, 30), q)
+    with pytest.raises(TypeError, match="GPU"):
+        ops.mx_pointwise(torch.zeros(1, 30, 2, 2), q)
+    with pytest.raises(RuntimeError, match="eval"):
+        YoloV8("n", 2).quantize_pointwise()
+    with pytest.raises(TypeError, match="GPU"):
+        YoloV8("n", 2).eval().quantize_pointwise()
+
+
+@pytest.mark.parametrize("packed,scales,shape", [((2, 16), (2, 1), (2, 33)), ((2, 32), (2, 1), (2, 33)), ((2, 32), (2, 2), (3, 33)),
+                                                 ((1, 32), (2, 2), (2, 33))])
+def test_mx_tensor_checks_its_parts(packed, scales, shape):
+    from object_detectors_amd import hip_ops as ops
+    with pytest.raises(ValueError, match="MxTensor"):
+        ops.MxTensor(torch.zeros(packed, dtype=torch.uint8), torch.zeros(scales, dtype=torch.uint8), shape)
+
+
+def _probs(L, **kw):
+    a = L.lmi_logprob_args()
+    a.x, a.x_dtype, a.activation, a.classes, a.class_stride, a.n0, a.n1, a.stride0, a.stride1 = 4096, 0, 0, 10, 1, 1, 4, 40, 10
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return L.load().lmi_class_logprobs(C.byref(a), None)
+
+
+def test_class_logprobs_arguments(L):
+    lib = L.load()
+    assert lib.lmi_class_logprobs(None, None) == -1
+    assert _probs(L, n1=0) == 0                      # no rows: nothing to do, nothing is read
+    for bad in (dict(classes=0), dict(n0=-1), dict(activation=3), dict(top=-1), dict(top=11), dict(top=33, classes=100), dict(x=None),
+                dict(x_dtype=2), dict(class_stride=0), dict(stride1=-1), dict(labels=4096, label_dtype=2), dict(index=4096)):
+        assert _probs(L, **bad) == -1, bad
+    assert _probs(L, classes=1 << 31) == -4 and _probs(L, n0=1 << 20, n1=1 << 12) == -4
+    need = lib.lmi_class_logprobs_workspace_bytes(2, 200001, 1, 5)
+    assert need > 0 and lib.lmi_class_logprobs_workspace_bytes(2, 80, 1, 5) == 0
+    assert _probs(L, classes=200001, n1=2) == -3
+    assert _probs(L, classes=200001, n1=2, workspace=4096, workspace_bytes=need - 1) == -3
+    assert _probs(L, classes=200001, n1=2, workspace=4104, workspace_bytes=need) == -2
+
+
+def _product(L, **kw):
+    a = L.lmi_mx_product_args()
+    a.x, a.x_dtype, a.act, a.batch, a.pixels, a.k, a.n, a.x_stride = 4096, 0, 0, 1, 4, 64, 8, 64
+    a.w_packed, a.w_scales, a.y, a.y_dtype = 4096, 4096, 4096, 0
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return L.load().lmi_mx_product(C.byref(a), None)
+
+
+def test_mx_arguments(L):
+    lib = L.load()
+    assert lib.lmi_mx_quantize(4096, 0, 0, 32, 32, 4096, 4096, None) == 0 and lib.lmi_mx_dequantize(4096, 4096, 0, 32, 4096, 0, None) == 0
+    for bad in ((None, 0, 1, 32, 32, 4096, 4096), (4096, 2, 1, 32, 32, 4096, 4096), (4096, 0, -1, 32, 32, 4096, 4096), (4096, 0, 1, 0, 32, 4096, 4096),
+                (4096, 0, 1, 32, 32, None, 4096)):
+        assert lib.lmi_mx_quantize(*bad, None) == -1, bad
+    assert lib.lmi_mx_quantize(4096, 0, 1, 32, 32, 4104, 4096, None) == -2
+    assert lib.lmi_mx_quantize(4096, 0, 1 << 41, 32, 32, 4096, 4096, None) == -4
+    assert lib.lmi_mx_dequantize(4096, 4096, 1, 32, 4096, 2, None) == -1 and lib.lmi_mx_dequantize(4096, None, 1, 32, 4096, 0, None) == -1
+    assert lib.lmi_mx_product(None, None) == -1
+    assert _product(L, pixels=0) == 0
+    for bad in (dict(k=0), dict(n=0), dict(batch=-1), dict(act=2), dict(x_dtype=2), dict(y_dtype=1), dict(x=None), dict(y=None), dict(w_packed=None),
+                dict(layout=2), dict(x_stride=-1), dict(x_dtype=6, x_scales=None), dict(x_dtype=6, x_scales=4096, batch=2),
+                dict(x_dtype=6, x_scales=4096, layout=1)):
+        assert _product(L, **bad) == -1, bad
+    assert _product(L, w_packed=4104) == -2
+
+
+def test_oracle_mx_by_hand():
+    x = np.zeros((1, 33))
+    x[0, :8] = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9]      # largest 7.9: scale 2^0, midpoints go to the even code
+    x[0, 32] = -48.0                                              # a block of its own: 2^(5 - 2), 48 = 6 * 8
+    codes, scales = OM.quantize(x)
+    assert scales.tolist() == [[127, 130]]
+    assert codes[0, :8].tolist() == [0, 2, 2, 4, 4, 6, 6, 7] and codes[0, 32] == 15
+    assert OM.values(x)[0, :8].tolist() == [0, 1, 1, 2, 2, 4, 4, 6] and OM.values(x)[0, 32] == -48
+    assert OM.unpack(np.array([[0x21, 0xf0]], np.uint8)).tolist() == [[1, 2, 0, 15]]
+    codes, scales = OM.quantize(np.array([[np.nan] + [1.0] * 31, [0.0] * 32]))
+    assert scales.tolist() == [[255], [0]] and np.isnan(OM.dequantize(codes, scales, 32)[0]).all()
+
+
+def test_oracle_evidence_by_hand():
+    r = OC.evidence([[0.0, 0.0, -np.inf], [-np.inf] * 3, [np.log(3), 0.0, np.nan]], [1, 2, 0], 2)
+    assert np.allclose(r["logprob"][0], -np.log(2)) and r["logprob"][1] == -np.inf and np.isnan(r["logprob"][2])
+    assert np.allclose(r["entropy"][0], np.log(2)) and r["entropy"][1] == 0 and np.isnan(r["entropy"][2])
+    assert r["top_index"].tolist() == [[0, 1], [0, 1], [2, 0]]
+    r = OC.evidence([[0.5, 0.0, 1.0]], [0], 3, "none")
+    assert np.allclose(r["entropy"], np.log(2)) and np.allclose(r["logprob"], np.log(0.5)) and r["top_index"].tolist() == [[2, 0, 1]]
+    r = OC.evidence([[0.0, 1000.0]], [1], 1, "sigmoid")
+    assert np.allclose(r["entropy"], np.log(2)) and r["logprob"][0] == 0 and r["top_index"].tolist() == [[1]]

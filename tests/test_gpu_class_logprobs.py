@@ -247,3 +247,24 @@ def test_two_streams_agree():
     for i in range(2):
         for r in got[i]:
             assert all(torch.equal(r[k], want[i][k]) for k in r)
+
+
+def test_refusals():
+    ops = _ops()
+    x = torch.randn(4, 6, 9).cuda()
+    lab = torch.zeros(4, 6, dtype=torch.int64).cuda()
+    idx, cnt = torch.zeros(4, 3, dtype=torch.int32).cuda(), torch.zeros(4, dtype=torch.int32).cuda()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.class_logprobs(x.clone().requires_grad_(), lab)
+    for err, call in ((TypeError, lambda: ops.class_logprobs(x.int(), lab)), (ValueError, lambda: ops.class_logprobs(x, lab, top=10)),
+                      (ValueError, lambda: ops.class_logprobs(x, lab, top=-1)), (ValueError, lambda: ops.class_logprobs(x, lab, activation="relu")),
+                      (ValueError, lambda: ops.class_logprobs(x, lab[:3])), (TypeError, lambda: ops.class_logprobs(x, lab.short())),
+                      (TypeError, lambda: ops.class_logprobs(x, lab.cpu())), (ValueError, lambda: ops.class_logprobs(x[..., :0])),
+                      (ValueError, lambda: ops.class_logprobs(torch.randn(2, 40).cuda(), top=33)),
+                      (ValueError, lambda: ops.class_logprobs(x, index=idx.long())), (ValueError, lambda: ops.class_logprobs(x, index=idx[:3])),
+                      (ValueError, lambda: ops.class_logprobs(x[0], index=idx)), (ValueError, lambda: ops.class_logprobs(x, index=idx.t())),
+                      (ValueError, lambda: ops.class_logprobs(x, count=cnt[:3])), (ValueError, lambda: ops.class_logprobs(x, count=cnt.long())),
+                      (ValueError, lambda: ops.class_logprobs(x, out={})), (ValueError, lambda: ops.class_logprobs(x[0], count=cnt)),
+                      (ValueError, lambda: ops.class_logprobs(x, out={"entropy": torch.empty(6, 4).cuda().t()}))):
+        with pytest.raises(err):
+            call()

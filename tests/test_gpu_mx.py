@@ -193,3 +193,24 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for a, b in zip(res, step()):
             assert torch.equal(a, b)
+
+
+def test_refusals():
+    ops = _ops()
+    x, w = torch.randn(4, 64).cuda(), ops.mx_quantize(torch.randn(8, 64).cuda())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.mx_linear(x.clone().requires_grad_(), w)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.mx_quantize(x.clone().requires_grad_())
+    with torch.no_grad():
+        ops.mx_linear(x.clone().requires_grad_(), w)
+    for err, call in ((TypeError, lambda: ops.mx_quantize(x.int())), (TypeError, lambda: ops.mx_linear(x.double(), w)),
+                      (TypeError, lambda: ops.mx_linear(x, torch.randn(8, 64).cuda())), (ValueError, lambda: ops.mx_linear(x[:, :63], w)),
+                      (ValueError, lambda: ops.mx_linear(x, w, act="relu")), (ValueError, lambda: ops.mx_linear(x, w, dtype=torch.float16)),
+                      (ValueError, lambda: ops.mx_linear(x, w, torch.zeros(7).cuda())), (ValueError, lambda: ops.mx_linear(x, w, torch.zeros(8).cuda().half())),
+                      (ValueError, lambda: ops.mx_linear(x, w, torch.zeros(8))), (ValueError, lambda: ops.mx_linear(x, w, out=torch.empty(4, 9).cuda())),
+                      (ValueError, lambda: ops.mx_pointwise(x, w)), (ValueError, lambda: ops.mx_pointwise(torch.randn(1, 32, 4, 4).cuda(), w)),
+                      (ValueError, lambda: ops.mx_linear(x, w, out=torch.empty(8, 4).cuda().t())), (ValueError, lambda: ops.mx_quantize(x[:, :0])),
+                      (TypeError, lambda: ops.mx_dequantize(x)), (TypeError, lambda: ops.mx_dequantize(w, torch.int8))):
+        with pytest.raises(err):
+            call()

@@ -497,8 +497,11 @@ int lmi_class_logprobs(const lmi_logprob_args *args, void *stream);
 /* ------------------------------------------------------------------------------------------
  * MXFP4 -- microscaled 4-bit floating point (OCP MX v1.0): blocks of LMI_MX_BLOCK elements along a row share the scale
  * 2^(byte - 127), byte 255 = NaN; elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two per byte, the
- * earlier one in the low half.  A row of k elements takes B = ceil(k / 32) scale bytes and 16*B element bytes; the last
- * block is filled up with zeros.
+ * earlier one in the low half.  Blocks are kept in the order the matrix instruction takes them, rows in groups of 32, k in
+ * steps of 64 = two blocks:
+ *   packed uint8 [G][S][2][32][16]  group of rows, step, which block of the step, row of the group, 16 bytes = 32 elements
+ *   scales uint8 [G][Q][2][32][4]   group, four steps, block, row, step of the four
+ * with G = ceil(rows / 32), S = ceil(ceil(k / 32) / 2), Q = ceil(S / 4); rows and blocks beyond the tensor are zeros (scale byte 0).
  * lmi_mx_quantize: scale exponent floor(log2(max |x|)) - 2 of each block, at least -127 (also for a block of zeros);
  *   elements rounded to nearest, ties to even, beyond 6 to 6.  A block that holds an infinity or a NaN gets byte 255.
  *   x LMI_F32 | LMI_F16 | LMI_BF16, k contiguous elements a row, rows row_stride elements apart.
@@ -507,7 +510,7 @@ int lmi_class_logprobs(const lmi_logprob_args *args, void *stream);
  *   w quantised.  The positions m are (batch, pixels).  layout LMI_MX_ROWS (a linear layer, channels-last maps): x
  *   element (b, p, k) at b*x_batch + p*x_stride + k, y contiguous (batch, pixels, n).  LMI_MX_PLANES (NCHW maps): x
  *   element at b*x_batch + k*x_stride + p, y contiguous (batch, n, pixels).
- *   x_dtype LMI_MXFP4: x points at packed rows, x_scales at their scales (rows, batch 1, x_stride unused).
+ *   x_dtype LMI_MXFP4: x points at the packed blocks, x_scales at their scales (rows, batch 1, x_stride unused).
  *   y_dtype LMI_F32 | LMI_F16 | LMI_BF16, the type of x unless that is MXFP4.  bias [device] fp32 (n) or NULL.  workspace [device] of lmi_mx_product_workspace_bytes (0: none).
  *   This is a 1x1 convolution of the network with its folded batch norm (bias) and SiLU.
  */

@@ -3,16 +3,20 @@
 //
 // A block's scale is 2^(floor(log2 max) - 2), so its largest element lands in [4, 8): 6 is the largest magnitude of e2m1, and
 // what rounds beyond it stays at 6.  v_cvt_scalef32_pk_fp4_* divides by the scale and rounds to nearest even with that
-// saturation; x / 2^e is exact, so nothing is rounded twice.  The products run on v_mfma_scale_f32_32x32x64_f8f6f4: 64 elements of k
-// per instruction, every lane brings 32 elements of one row and their scale byte -- one block --, sums in fp32.
+// saturation; x / 2^e is exact, so nothing is rounded twice.  The products run on v_mfma_scale_f32_32x32x64_f8f6f4 (twice the
+// rate of the 16x16x128 form): 64 elements of k per instruction, every lane brings 32 elements of one row and their
+// scale byte -- one block --, sums in fp32.  Quantised tensors are kept in that order (see lmi_hip.h), so an operand of a
+// wave is one contiguous kilobyte, and the scale bytes of four steps are one word of which the instruction picks a byte.
 //
 // Kernels
-//  mx_quantize_kernel     four lanes per block of a row, 8 elements each.
-//  mx_dequantize_kernel   eight elements per thread.
+//  mx_quantize_kernel     a wave takes 8 rows x 256 elements: four lanes per block, 8 elements each, four steps per lane.
+//  mx_dequantize_kernel   the same shape backwards.
 //  mx_product_kernel      64 positions x all of k: activations are read once, quantised in registers (a lane owns whole blocks: 32
 //                         channels of one position) and laid into LDS in the matrix instruction's order; then every wave
 //                         multiplies them with its share of the weight rows.
 #include <hip/hip_fp16.h>
+
+#include <type_traits>
 
 #include "common.h"
 
@@ -20,6 +24,9 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float f16x __attribute__((ext_vector_type(16)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 struct Packed {};   // x is quantised already
 
@@ -43,26 +50,74 @@ __device__ __forceinline__ unsigned pack8(const float *v, float scale) {
   return r;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *x, long long rows, long long k, long long row_stride, unsigned blocks,
-                                                          unsigned char *packed, unsigned char *scales) {
-  const long long quads = rows * blocks * 4;
-  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < quads; q += (long long)gridDim.x * 256) {   // quads % 4 == 0: the four lanes stay together
-    const long long block = q >> 2;
-    const long long row = block / blocks;
-    const long long c0 = (block - row * blocks) * LMI_MX_BLOCK + (q & 3) * 8;
-    const T *p = x + row * row_stride + c0;
-    float v[8];
+// 8 elements from p on, `n` of them in the row; VEC: all 8, 16-byte aligned
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T *p, long long n, float (&v)[8]) {
+  if (VEC && n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = ((const float4 *)p)[0], b = ((const float4 *)p)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      const t8 a = *(const t8 *)p;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = c0 + u < k ? to_float(p[u]) : 0.0f;
-    unsigned m = 0;
+      for (int u = 0; u < 8; ++u) v[u] = to_float(a[u]);
+    }
+  } else {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) m = max(m, __float_as_uint(v[u]) & 0x7fffffffu);
-    m = max(m, __shfl_xor(m, 1));
-    m = max(m, __shfl_xor(m, 2));
-    const unsigned byte = scale_byte(m);
-    ((unsigned *)packed)[q] = pack8(v, scale_value(byte));
-    if ((q & 3) == 0) scales[block] = (unsigned char)byte;
+    for (int u = 0; u < 8; ++u) v[u] = u < n ? to_float(p[u]) : 0.0f;
+  }
+}
+
+// lane = (row of the octet, block of the step, quarter of the block).  The wave reads 8 rows x 128 bytes (16-bit types) per step and writes 8 x 16
+// bytes side by side for either block; the scale bytes of its four steps leave as one word.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *x, long long rows, long long k, long long row_stride, unsigned steps, unsigned quads,
+                                                          long long units, unsigned *packed, unsigned *scales) {
+  const int lane = threadIdx.x & 63, quarter = lane & 3, half = (lane >> 2) & 1, r8 = lane >> 3;
+  for (long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (long long)gridDim.x * 4) {   // row octet x four steps
+    const long long octet = unit / quads;
+    const unsigned quad = (unsigned)(unit - octet * quads);
+    const long long row = octet * 8 + r8, group = octet >> 2;
+    const int rg = (int)(octet & 3) * 8 + r8;
+    const T *p = x + row * row_stride;
+    float v[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long c0 = ((long long)quad * 4 + i) * 64 + half * 32 + quarter * 8;
+      load8<T, VEC>(p + c0, row < rows ? k - c0 : 0, v[i]);
+    }
+    unsigned word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned m = 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) m = max(m, __float_as_uint(v[i][u]) & 0x7fffffffu);
+      m = max(m, __shfl_xor(m, 1));
+      m = max(m, __shfl_xor(m, 2));
+      const unsigned byte = scale_byte(m), step = quad * 4 + i;
+      word |= byte << (8 * i);
+      if (step < steps) packed[(((group * steps + step) * 2 + half) * 32 + rg) * 4 + quarter] = pack8(v[i], scale_value(byte));
+    }
+    if (quarter == 0) scales[((group * quads + quad) * 2 + half) * 32 + rg] = word;
+  }
+}
+
+template <typename T> __device__ __forceinline__ void store8(T *p, long long n, bool vec, const float (&v)[8]) {
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      ((float4 *)p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      ((float4 *)p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      t8 a;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) a[u] = (T)v[u];
+      *(t8 *)p = a;
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (u < n) p[u] = (T)v[u];
   }
 }
 
@@ -74,34 +129,50 @@ __device__ __forceinline__ float code_value(unsigned c) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char *packed, const unsigned char *scales, long long rows,
-                                                            long long k, unsigned blocks, T *out) {
-  const long long quads = rows * blocks * 4;
-  for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < quads; q += (long long)gridDim.x * 256) {
-    const long long block = q >> 2;
-    const long long row = block / blocks;
-    const long long c0 = (block - row * blocks) * LMI_MX_BLOCK + (q & 3) * 8;
-    const unsigned w = ((const unsigned *)packed)[q], byte = scales[block];
-    // 2^(byte - 127); the smallest is subnormal, 255 is NaN
-    const float s = byte == 255u ? NAN : (byte ? __uint_as_float(byte << 23) : 0x1p-127f);
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned *packed, const unsigned *scales, long long rows, long long k, unsigned steps,
+                                                            unsigned quads, long long units, bool vec, T *out) {
+  const int lane = threadIdx.x & 63, quarter = lane & 3, half = (lane >> 2) & 1, r8 = lane >> 3;
+  for (long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (long long)gridDim.x * 4) {
+    const long long octet = unit / quads;
+    const unsigned quad = (unsigned)(unit - octet * quads);
+    const long long row = octet * 8 + r8, group = octet >> 2;
+    if (row >= rows) continue;
+    const int rg = (int)(octet & 3) * 8 + r8;
+    const unsigned word = scales[((group * quads + quad) * 2 + half) * 32 + rg];
+    unsigned w[4];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (c0 + u < k) out[row * k + c0 + u] = (T)(code_value((w >> (4 * u)) & 15u) * s);
+    for (int i = 0; i < 4; ++i) {
+      const unsigned step = quad * 4 + i;
+      w[i] = step < steps ? packed[(((group * steps + step) * 2 + half) * 32 + rg) * 4 + quarter] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long c0 = ((long long)quad * 4 + i) * 64 + half * 32 + quarter * 8;
+      const unsigned byte = (word >> (8 * i)) & 255u;
+      // 2^(byte - 127); the smallest is subnormal, 255 is NaN
+      const float s = byte == 255u ? NAN : (byte ? __uint_as_float(byte << 23) : 0x1p-127f);
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = code_value((w[i] >> (4 * u)) & 15u) * s;
+      store8(out + row * k + c0, k - c0, vec, v);
+    }
   }
 }
 
 struct Product {
   const void *x;
-  const unsigned char *xs;
+  const unsigned *xs;
   long long pixels, k, n, xb, xs1;   // xs1: between positions (rows) or channels (planes)
-  const unsigned char *w, *ws;
+  const uint4 *w;
+  const unsigned *ws;
   const float *bias;
   void *y;
   unsigned blocks;        // blocks of 32 along k
   unsigned tiles_pixels;  // tiles of 64 positions per image
   int tiles_n;            // tiles of 32 weight rows
   int split_n;            // tiles of 32 weight rows per workgroup
-  int steps;              // steps of 64 along k that LDS holds
+  int all_steps;          // steps of 64 along k
+  int steps;              // steps that LDS holds (a multiple of 4, or all)
 };
 
 constexpr int kTile = 64;   // positions per workgroup
@@ -111,125 +182,325 @@ template <int ACT> __device__ __forceinline__ float activate(float v) {
   return v;
 }
 
-// block kb of position p -> 16 bytes and the scale byte
-template <typename T, bool PLANES>
-__device__ __forceinline__ void load_block(const Product &P, const T *x, long long p, unsigned kb, uint4 &frag, unsigned &byte) {
-  float v[LMI_MX_BLOCK];
+// one block from 32 values
+__device__ __forceinline__ uint4 quantize_block(const float (&v)[32], unsigned &byte) {
   unsigned m = 0;
-  const long long c0 = (long long)kb * LMI_MX_BLOCK;
-  const T *q = x + p * (PLANES ? 1 : P.xs1) + c0 * (PLANES ? P.xs1 : 1);
 #pragma unroll
-  for (int u = 0; u < LMI_MX_BLOCK; ++u) {
-    v[u] = c0 + u < P.k ? to_float(q[u * (PLANES ? P.xs1 : 1)]) : 0.0f;
-    m = max(m, __float_as_uint(v[u]) & 0x7fffffffu);
-  }
+  for (int u = 0; u < 32; ++u) m = max(m, __float_as_uint(v[u]) & 0x7fffffffu);
   byte = scale_byte(m);
   const float s = scale_value(byte);
-  frag = make_uint4(pack8(v, s), pack8(v + 8, s), pack8(v + 16, s), pack8(v + 24, s));
-}
-template <bool PLANES>
-__device__ __forceinline__ void load_packed(const Product &P, long long p, unsigned kb, uint4 &frag, unsigned &byte) {
-  const long long block = p * P.blocks + kb;
-  frag = ((const uint4 *)P.x)[block];
-  byte = P.xs[block];
+  return make_uint4(pack8(v, s), pack8(v + 8, s), pack8(v + 16, s), pack8(v + 24, s));
 }
 
-template <typename T, typename Y, bool PLANES, int ACT>
+// two blocks from 32 words that hold one value of either (two neighbouring pixels of 32 channels), 16-bit types: magnitudes are compared as
+// integers, two at a time, and go into the conversion as they are
+template <typename T> __device__ __forceinline__ void quantize_pair16(const unsigned (&w)[32], uint4 (&f)[2], unsigned (&byte)[2]) {
+  us2 m = {0, 0};
+#pragma unroll
+  for (int u = 0; u < 32; ++u) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, w[u] & 0x7fff7fffu));
+#pragma unroll
+  for (int px = 0; px < 2; ++px) {
+    const float mag = to_float(__builtin_bit_cast(T, (unsigned short)m[px]));
+    byte[px] = scale_byte(__float_as_uint(mag));
+    const float s = scale_value(byte[px]);
+    unsigned r[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      unsigned a = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned two = __builtin_amdgcn_perm(w[q * 8 + 2 * j + 1], w[q * 8 + 2 * j], px ? 0x07060302u : 0x05040100u);
+        if constexpr (__is_same(T, _Float16)) {
+          const h2 t = __builtin_bit_cast(h2, two);
+          a = j == 0 ? __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(a, t, s, 0) : j == 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(a, t, s, 1)
+            : j == 2 ? __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(a, t, s, 2) : __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(a, t, s, 3);
+        } else {
+          const b2 t = __builtin_bit_cast(b2, two);
+          a = j == 0 ? __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(a, t, s, 0) : j == 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(a, t, s, 1)
+            : j == 2 ? __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(a, t, s, 2) : __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(a, t, s, 3);
+        }
+      }
+      r[q] = a;
+    }
+    f[px] = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
+
+// Columns of the two 32-column subtiles: position 2j + h of the tile is column j of subtile h, so that a lane's two results are
+// neighbours.  Rows of a weight tile are permuted the same way on both sides of the product: result i of a lane is weight row
+// 16*(lane >> 5) + i of the tile.
+__device__ __forceinline__ int weight_lane(int lane) {
+  const int r = lane & 31;
+  return (lane & 32) + ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3);
+}
+
+// LDS: fragments [step][subtile][64] uint4, then scale words [step / 4][subtile][64]
+template <typename T, bool PLANES, bool VEC>
+__device__ __forceinline__ void fill(const Product &P, long long image, long long p0, int live, int s0, int ns, uint4 *frags, unsigned char *bytes) {
+  const int t = threadIdx.x;
+  auto put = [&](int kl, int px, const uint4 &f, unsigned byte) {
+    const int at = (px & 1) * 64 + (kl & 1) * 32 + (px >> 1), step = kl >> 1;
+    frags[step * 128 + at] = f;
+    bytes[((step >> 2) * 128 + at) * 4 + (step & 3)] = (unsigned char)byte;
+  };
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  if constexpr (__is_same(T, Packed)) {
+    const long long g0 = p0 >> 5;
+    for (int item = t; item < ns * 128; item += 256) {
+      const int step = item >> 7, at = item & 127, px = at & 63, half = at >> 6;   // px: row of the two groups
+      const long long g = g0 + (px >> 5);
+      uint4 f = zero;
+      if (px < live) f = ((const uint4 *)P.x)[((g * P.all_steps + s0 + step) * 2 + half) * 32 + (px & 31)];
+      frags[step * 128 + (px & 1) * 64 + half * 32 + (px >> 1)] = f;
+    }
+    const int quads = (P.all_steps + 3) / 4;
+    for (int item = t; item < (ns + 3) / 4 * 128; item += 256) {   // s0 is a multiple of 4
+      const int q = item >> 7, at = item & 127, px = at & 63, half = at >> 6;
+      const long long g = g0 + (px >> 5);
+      unsigned w = 0;
+      if (px < live) w = P.xs[((g * quads + s0 / 4 + q) * 2 + half) * 32 + (px & 31)];
+      ((unsigned *)bytes)[q * 128 + (px & 1) * 64 + half * 32 + (px >> 1)] = w;
+    }
+    return;
+  } else {
+    const T *x = (const T *)P.x + image * P.xb;
+    if constexpr (PLANES && VEC) {   // two neighbouring pixels per thread
+      for (int item = t; item < ns * 64; item += 256) {
+        const int pair = item & 31, kl = item >> 5;
+        const unsigned kb = 2 * s0 + kl;
+        uint4 f[2] = {zero, zero};
+        unsigned byte[2] = {0, 0};
+        if (2 * pair < live && kb < P.blocks) {
+          const T *q = x + p0 + 2 * pair + (long long)kb * 32 * P.xs1;
+          const int in = (int)(P.k - (long long)kb * 32 < 32 ? P.k - (long long)kb * 32 : 32);
+          if constexpr (sizeof(T) == 4) {
+            float a[32], b[32];
+#pragma unroll
+            for (int u = 0; u < 32; ++u) {
+              const float2 v = u < in ? *(const float2 *)(q + u * P.xs1) : make_float2(0.0f, 0.0f);
+              a[u] = v.x;
+              b[u] = v.y;
+            }
+            f[0] = quantize_block(a, byte[0]);
+            f[1] = quantize_block(b, byte[1]);
+          } else {
+            unsigned w[32];
+            if (in == 32) {
+#pragma unroll
+              for (int u = 0; u < 32; ++u) w[u] = *(const unsigned *)(q + u * P.xs1);
+            } else {
+#pragma unroll
+              for (int u = 0; u < 32; ++u) w[u] = u < in ? *(const unsigned *)(q + u * P.xs1) : 0u;
+            }
+            quantize_pair16<T>(w, f, byte);
+          }
+        }
+        put(kl, 2 * pair, f[0], byte[0]);
+        put(kl, 2 * pair + 1, f[1], byte[1]);
+      }
+    } else {
+      for (int item = t; item < ns * 128; item += 256) {
+        const int px = item & 63, kl = item >> 6;
+        const unsigned kb = 2 * s0 + kl;
+        uint4 f = zero;
+        unsigned byte = 0;
+        if (px < live && kb < P.blocks) {
+          const long long c0 = (long long)kb * 32;
+          float v[32];
+          if constexpr (PLANES) {
+            const T *q = x + p0 + px + c0 * P.xs1;
+#pragma unroll
+            for (int u = 0; u < 32; ++u) v[u] = c0 + u < P.k ? to_float(q[u * P.xs1]) : 0.0f;
+          } else {
+            const T *q = x + (p0 + px) * P.xs1 + c0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              float e[8];
+              load8<T, VEC>(q + 8 * u, P.k - c0 - 8 * u, e);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[8 * u + j] = e[j];
+            }
+          }
+          f = quantize_block(v, byte);
+        }
+        put(kl, px, f, byte);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ v8i operand(const uint4 &a) { return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}; }
+
+template <int BYTE> __device__ __forceinline__ void mfma2(f16x (&acc)[2], const uint4 &a, unsigned sa, const uint4 &b0, const uint4 &b1, unsigned sb0, unsigned sb1) {
+  acc[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b0), acc[0], 4, 4, BYTE, (int)sa, BYTE, (int)sb0);
+  acc[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b1), acc[1], 4, 4, BYTE, (int)sa, BYTE, (int)sb1);
+}
+
+// steps [q0, q1) of four, of the ns in LDS, for weight tile nt
+__device__ __forceinline__ void multiply(const Product &P, int nt, int s0, int ns, int q0, int dq, const uint4 *frags, const unsigned *words, int lane, f16x (&acc)[2]) {
+  const int wl = weight_lane(lane), quads = (P.all_steps + 3) / 4;
+  const uint4 *w = P.w + ((long long)nt * P.all_steps + s0) * 64 + wl;
+  const unsigned *ws = P.ws + ((long long)nt * quads + s0 / 4) * 64 + wl;
+  for (int q = q0; q * 4 < ns; q += dq) {
+    const unsigned sa = ws[q * 64], sb0 = words[q * 128 + lane], sb1 = words[q * 128 + 64 + lane];
+    const uint4 *wq = w + q * 256, *f = frags + q * 512 + lane;
+    if (q * 4 + 4 <= ns) {
+      const uint4 a0 = wq[0], a1 = wq[64], a2 = wq[128], a3 = wq[192];
+      mfma2<0>(acc, a0, sa, f[0], f[64], sb0, sb1);
+      mfma2<1>(acc, a1, sa, f[128], f[192], sb0, sb1);
+      mfma2<2>(acc, a2, sa, f[256], f[320], sb0, sb1);
+      mfma2<3>(acc, a3, sa, f[384], f[448], sb0, sb1);
+    } else {
+      const int left = ns - q * 4;
+      mfma2<0>(acc, wq[0], sa, f[0], f[64], sb0, sb1);
+      if (left > 1) mfma2<1>(acc, wq[64], sa, f[128], f[192], sb0, sb1);
+      if (left > 2) mfma2<2>(acc, wq[128], sa, f[256], f[320], sb0, sb1);
+    }
+  }
+}
+
+template <typename Y, bool PLANES, bool VEC, int ACT>
+__device__ __forceinline__ void store_tile(const Product &P, long long image, long long p0, int live, int nt, int lane, const f16x (&acc)[2]) {
+  Y *y = (Y *)P.y + image * P.pixels * P.n;
+  const int px = 2 * (lane & 31);
+  const long long n0 = (long long)nt * 32 + 16 * (lane >> 5);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const long long n = n0 + i;
+    if (n >= P.n) break;
+    const float b = P.bias ? P.bias[n] : 0.0f;
+    const Y v0 = (Y)activate<ACT>(acc[0][i] + b), v1 = (Y)activate<ACT>(acc[1][i] + b);
+    if constexpr (PLANES) {
+      Y *q = y + n * P.pixels + p0 + px;
+      if (VEC) {
+        typedef Y y2 __attribute__((ext_vector_type(2)));
+        if (px < live) *(y2 *)q = y2{v0, v1};
+      } else {
+        if (px < live) q[0] = v0;
+        if (px + 1 < live) q[1] = v1;
+      }
+    } else {
+      if (px < live) y[(p0 + px) * P.n + n] = v0;
+      if (px + 1 < live) y[(p0 + px + 1) * P.n + n] = v1;
+    }
+  }
+}
+
+// KSPLIT: one weight tile per workgroup, its waves share k (few positions); else the waves share the weight tiles.
+template <typename T, typename Y, bool PLANES, bool VEC, int ACT, bool KSPLIT>
 __global__ __launch_bounds__(256) void mx_product_kernel(const Product P) {
-  extern __shared__ uint4 lds[];   // [step][2][64] fragments, then [step][2][64] scale bytes
+  extern __shared__ uint4 lds[];
   uint4 *frags = lds;
   unsigned char *bytes = (unsigned char *)(lds + (long long)P.steps * 128);
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const unsigned *words = (const unsigned *)bytes;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long image = blockIdx.x / P.tiles_pixels;
   const long long p0 = (long long)(blockIdx.x % P.tiles_pixels) * kTile;
   const int live = (int)(P.pixels - p0 < kTile ? P.pixels - p0 : kTile);
   const int nt0 = blockIdx.y * P.split_n;
   const int nt1 = nt0 + P.split_n < P.tiles_n ? nt0 + P.split_n : P.tiles_n;
-  const int all_steps = (int)(P.blocks + 1) / 2;
-  const bool once = all_steps <= P.steps;
-  Y *y = (Y *)P.y + image * P.pixels * P.n;
-
-  for (int g0 = nt0; g0 < nt1; g0 += 4) {   // every wave takes one tile of a group of four
-    const int nt = g0 + wave;
+  const bool once = P.all_steps <= P.steps;
+  const int group = KSPLIT ? 1 : 4;
+  for (int g0 = nt0; g0 < nt1; g0 += group) {
+    const int nt = KSPLIT ? g0 : g0 + wave;
     f16x acc[2] = {};
-    for (int s0 = 0; s0 < all_steps; s0 += P.steps) {
-      const int ns = all_steps - s0 < P.steps ? all_steps - s0 : P.steps;
+    for (int s0 = 0; s0 < P.all_steps; s0 += P.steps) {
+      const int ns = P.all_steps - s0 < P.steps ? P.all_steps - s0 : P.steps;
       if (!once || g0 == nt0) {
         __syncthreads();   // LDS is free again
-        for (int item = t; item < ns * 2 * kTile; item += 256) {
-          const int px = item % kTile, kl = item / kTile;
-          const unsigned kb = 2 * s0 + kl;
-          uint4 frag = make_uint4(0, 0, 0, 0);
-          unsigned byte = 0;
-          if (px < live && kb < P.blocks) {
-            if constexpr (__is_same(T, Packed)) load_packed<PLANES>(P, p0 + px, kb, frag, byte);
-            else load_block<T, PLANES>(P, (const T *)P.x + image * P.xb, p0 + px, kb, frag, byte);
-          }
-          const int at = ((kl >> 1) * 2 + (px >> 5)) * 64 + (kl & 1) * 32 + (px & 31);
-          frags[at] = frag;
-          bytes[at] = (unsigned char)byte;
-        }
+        fill<T, PLANES, VEC>(P, image, p0, live, s0, ns, frags, bytes);
         __syncthreads();
       }
-      if (nt < nt1) {
-        const long long n = (long long)nt * 32 + (lane & 31);
-        const long long wrow = (n < P.n ? n : P.n - 1) * P.blocks;
-        for (int s = 0; s < ns; ++s) {
-          const unsigned kb = 2 * (s0 + s) + (lane >> 5);
-          uint4 a = make_uint4(0, 0, 0, 0);
-          unsigned sa = 0;
-          if (kb < P.blocks) {
-            a = ((const uint4 *)P.w)[wrow + kb];
-            sa = P.ws[wrow + kb];
-          }
-          const v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 b = frags[(s * 2 + h) * 64 + lane];
-            const v8i bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-            acc[h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[h], 4, 4, 0, (int)sa, 0, (int)bytes[(s * 2 + h) * 64 + lane]);
-          }
-        }
-      }
+      if (nt < nt1) multiply(P, nt, s0, ns, KSPLIT ? wave : 0, KSPLIT ? 4 : 1, frags, words, lane, acc);
     }
-    if (nt < nt1) {
+    if (KSPLIT) {   // sums of the four waves, in their order
+      __syncthreads();
+      float *part = (float *)lds;   // [3][32][64]
+      if (wave) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int px = h * 32 + (lane & 31);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const long long n = (long long)nt * 32 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4;
-          if (px < live && n < P.n) {
-            const float v = activate<ACT>(acc[h][i] + (P.bias ? P.bias[n] : 0.0f));
-            y[PLANES ? n * P.pixels + p0 + px : (p0 + px) * P.n + n] = (Y)v;
-          }
-        }
+          for (int i = 0; i < 16; ++i) part[((wave - 1) * 32 + h * 16 + i) * 64 + lane] = acc[h][i];
       }
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+#pragma unroll
+            for (int w = 0; w < 3; ++w) acc[h][i] += part[(w * 32 + h * 16 + i) * 64 + lane];
+          }
+        store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt, lane, acc);
+      }
+    } else if (nt < nt1) {
+      store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt, lane, acc);
     }
   }
 }
 
-constexpr int kStepBytes = 128 * 17;   // LDS of one step of 64 along k
-constexpr int kMaxSteps = 28;          // 59.5 KB
+constexpr int kMaxSteps = 28;   // 59.5 KB of LDS
+size_t lds_bytes(int steps) { return (size_t)steps * 2048 + (size_t)((steps + 3) / 4) * 512; }
 
-template <typename T, typename Y, bool PLANES, int ACT> int launch_product(Product P, long long batch, hipStream_t st) {
-  const int all_steps = (int)(P.blocks + 1) / 2;
-  P.steps = all_steps < kMaxSteps ? all_steps : kMaxSteps;
+template <typename T, typename Y, bool PLANES, bool VEC, int ACT> int launch_product(Product P, long long batch, hipStream_t st) {
+  P.steps = P.all_steps < kMaxSteps ? P.all_steps : kMaxSteps;
   const long long tiles = batch * P.tiles_pixels;
   // few positions: the weight rows are split over workgroups too, until there are about two per CU
   long long split = 1;
   if (tiles < 512) split = (512 + tiles - 1) / tiles;
   P.split_n = (int)((P.tiles_n + split - 1) / split);
-  const unsigned gy = (unsigned)((P.tiles_n + P.split_n - 1) / P.split_n);
-  mx_product_kernel<T, Y, PLANES, ACT><<<dim3((unsigned)tiles, gy), 256, (size_t)P.steps * kStepBytes, st>>>(P);
+  const dim3 grid((unsigned)tiles, (unsigned)((P.tiles_n + P.split_n - 1) / P.split_n));
+  const size_t lds = lds_bytes(P.steps);
+  if (P.split_n == 1) {
+    const size_t parts = 3 * 32 * 64 * 4;
+    mx_product_kernel<T, Y, PLANES, VEC, ACT, true><<<grid, 256, lds > parts ? lds : parts, st>>>(P);
+  } else {
+    mx_product_kernel<T, Y, PLANES, VEC, ACT, false><<<grid, 256, lds, st>>>(P);
+  }
   return lmi_check_launch("lmi_mx_product");
 }
 
 template <typename T, typename Y, bool PLANES> int launch_act(const Product &P, int act, long long batch, hipStream_t st) {
-  return act == LMI_ACT_SILU ? launch_product<T, Y, PLANES, LMI_ACT_SILU>(P, batch, st) : launch_product<T, Y, PLANES, LMI_ACT_NONE>(P, batch, st);
+  // planes: two pixels of a channel in one load, and of a result in one store; rows: 16-byte loads
+  const uintptr_t align = PLANES ? 2 * sizeof(Y) : 16;
+  bool vec = false;
+  if constexpr (!__is_same(T, Packed)) {
+    vec = (uintptr_t)P.x % align == 0 && P.xb * sizeof(Y) % align == 0 && P.xs1 * sizeof(Y) % align == 0;
+    if (PLANES) vec = vec && P.pixels % 2 == 0 && (uintptr_t)P.y % align == 0;
+    if (vec)
+      return act == LMI_ACT_SILU ? launch_product<T, Y, PLANES, true, LMI_ACT_SILU>(P, batch, st) : launch_product<T, Y, PLANES, true, LMI_ACT_NONE>(P, batch, st);
+  }
+  return act == LMI_ACT_SILU ? launch_product<T, Y, PLANES, false, LMI_ACT_SILU>(P, batch, st) : launch_product<T, Y, PLANES, false, LMI_ACT_NONE>(P, batch, st);
 }
 
 bool float_type(int d) { return d == LMI_F32 || d == LMI_F16 || d == LMI_BF16; }
+
+struct Units {
+  unsigned steps, quads, grid;
+  long long units;
+};
+// sizes of the quantising kernels' work; false: too large
+bool units_of(int64_t rows, int64_t k, Units &u) {
+  if (k >= (1ll << 36) || rows >= (1ll << 36)) return false;
+  const int64_t steps = (k + 63) / 64, quads = (steps + 3) / 4, octets = (rows + 31) / 32 * 4;
+  if (steps >= (1ll << 30) || octets >= (1ll << 40) / quads) return false;
+  u.steps = (unsigned)steps;
+  u.quads = (unsigned)quads;
+  u.units = octets * quads;
+  const int64_t wanted = (u.units + 3) / 4;
+  u.grid = (unsigned)(wanted < (1 << 23) ? wanted : (1 << 23));
+  return true;
+}
+
+template <typename T> void quantize(const void *x, int64_t rows, int64_t k, int64_t stride, const Units &u, void *packed, void *scales, hipStream_t st) {
+  const bool vec = lmi_is_aligned(x, 16) && stride * sizeof(T) % 16 == 0;
+  if (vec) mx_quantize_kernel<T, true><<<u.grid, 256, 0, st>>>((const T *)x, rows, k, stride, u.steps, u.quads, u.units, (unsigned *)packed, (unsigned *)scales);
+  else mx_quantize_kernel<T, false><<<u.grid, 256, 0, st>>>((const T *)x, rows, k, stride, u.steps, u.quads, u.units, (unsigned *)packed, (unsigned *)scales);
+}
+template <typename T> void dequantize(const void *packed, const void *scales, int64_t rows, int64_t k, const Units &u, void *out, hipStream_t st) {
+  const bool vec = lmi_is_aligned(out, 16) && k * sizeof(T) % 16 == 0;
+  mx_dequantize_kernel<<<u.grid, 256, 0, st>>>((const unsigned *)packed, (const unsigned *)scales, rows, k, u.steps, u.quads, u.units, vec, (T *)out);
+}
 
 }  // namespace
 
@@ -240,15 +511,13 @@ int lmi_mx_quantize(const void *x, int dtype, int64_t rows, int64_t k, int64_t r
   LMI_REQUIRE(float_type(dtype), LMI_ERR_BAD_ARG, "lmi_mx_quantize: x must be fp32, fp16 or bf16");
   if (rows == 0) return LMI_OK;
   LMI_REQUIRE(x && packed && scales, LMI_ERR_BAD_ARG, "lmi_mx_quantize: null pointer");
-  LMI_REQUIRE(lmi_is_aligned(packed, 16), LMI_ERR_ALIGNMENT, "lmi_mx_quantize: packed must be 16-byte aligned");
-  const int64_t blocks = (k + LMI_MX_BLOCK - 1) / LMI_MX_BLOCK;
-  LMI_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 40) / blocks, LMI_ERR_LIMIT, "lmi_mx_quantize: too many elements");
-  const int64_t wanted = (rows * blocks * 4 + 255) / 256;
-  const unsigned grid = (unsigned)(wanted < (1 << 23) ? wanted : (1 << 23));
+  LMI_REQUIRE(lmi_is_aligned(packed, 16) && lmi_is_aligned(scales, 4), LMI_ERR_ALIGNMENT, "lmi_mx_quantize: packed must be 16-byte, scales 4-byte aligned");
+  Units u;
+  LMI_REQUIRE(units_of(rows, k, u), LMI_ERR_LIMIT, "lmi_mx_quantize: too many elements");
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == LMI_F32) mx_quantize_kernel<<<grid, 256, 0, st>>>((const float *)x, rows, k, row_stride, (unsigned)blocks, packed, scales);
-  else if (dtype == LMI_F16) mx_quantize_kernel<<<grid, 256, 0, st>>>((const _Float16 *)x, rows, k, row_stride, (unsigned)blocks, packed, scales);
-  else mx_quantize_kernel<<<grid, 256, 0, st>>>((const __bf16 *)x, rows, k, row_stride, (unsigned)blocks, packed, scales);
+  if (dtype == LMI_F32) quantize<float>(x, rows, k, row_stride, u, packed, scales, st);
+  else if (dtype == LMI_F16) quantize<_Float16>(x, rows, k, row_stride, u, packed, scales, st);
+  else quantize<__bf16>(x, rows, k, row_stride, u, packed, scales, st);
   return lmi_check_launch("lmi_mx_quantize");
 }
 
@@ -257,15 +526,13 @@ int lmi_mx_dequantize(const uint8_t *packed, const uint8_t *scales, int64_t rows
   LMI_REQUIRE(float_type(out_dtype), LMI_ERR_BAD_ARG, "lmi_mx_dequantize: out must be fp32, fp16 or bf16");
   if (rows == 0) return LMI_OK;
   LMI_REQUIRE(packed && scales && out, LMI_ERR_BAD_ARG, "lmi_mx_dequantize: null pointer");
-  LMI_REQUIRE(lmi_is_aligned(packed, 16), LMI_ERR_ALIGNMENT, "lmi_mx_dequantize: packed must be 16-byte aligned");
-  const int64_t blocks = (k + LMI_MX_BLOCK - 1) / LMI_MX_BLOCK;
-  LMI_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 40) / blocks, LMI_ERR_LIMIT, "lmi_mx_dequantize: too many elements");
-  const int64_t wanted = (rows * blocks * 4 + 255) / 256;
-  const unsigned grid = (unsigned)(wanted < (1 << 23) ? wanted : (1 << 23));
+  LMI_REQUIRE(lmi_is_aligned(packed, 16) && lmi_is_aligned(scales, 4), LMI_ERR_ALIGNMENT, "lmi_mx_dequantize: packed must be 16-byte, scales 4-byte aligned");
+  Units u;
+  LMI_REQUIRE(units_of(rows, k, u), LMI_ERR_LIMIT, "lmi_mx_dequantize: too many elements");
   hipStream_t st = (hipStream_t)stream;
-  if (out_dtype == LMI_F32) mx_dequantize_kernel<<<grid, 256, 0, st>>>(packed, scales, rows, k, (unsigned)blocks, (float *)out);
-  else if (out_dtype == LMI_F16) mx_dequantize_kernel<<<grid, 256, 0, st>>>(packed, scales, rows, k, (unsigned)blocks, (_Float16 *)out);
-  else mx_dequantize_kernel<<<grid, 256, 0, st>>>(packed, scales, rows, k, (unsigned)blocks, (__bf16 *)out);
+  if (out_dtype == LMI_F32) dequantize<float>(packed, scales, rows, k, u, out, st);
+  else if (out_dtype == LMI_F16) dequantize<_Float16>(packed, scales, rows, k, u, out, st);
+  else dequantize<__bf16>(packed, scales, rows, k, u, out, st);
   return lmi_check_launch("lmi_mx_dequantize");
 }
 
@@ -284,28 +551,30 @@ int lmi_mx_product(const lmi_mx_product_args *a, void *stream) {
   LMI_REQUIRE(a->layout == LMI_MX_ROWS || a->layout == LMI_MX_PLANES, LMI_ERR_BAD_ARG, "lmi_mx_product: unknown layout %d", a->layout);
   const bool rows = a->layout == LMI_MX_ROWS;
   LMI_REQUIRE(a->x_batch >= 0 && a->x_stride >= 0, LMI_ERR_BAD_ARG, "lmi_mx_product: negative stride");
-  LMI_REQUIRE(lmi_is_aligned(a->w_packed, 16), LMI_ERR_ALIGNMENT, "lmi_mx_product: w_packed must be 16-byte aligned");
+  LMI_REQUIRE(lmi_is_aligned(a->w_packed, 16) && lmi_is_aligned(a->w_scales, 4), LMI_ERR_ALIGNMENT,
+              "lmi_mx_product: w_packed must be 16-byte, w_scales 4-byte aligned");
   Product P = {};
   P.x = a->x;
-  P.xs = a->x_scales;
+  P.xs = (const unsigned *)a->x_scales;
   P.pixels = a->pixels;
   P.k = a->k;
   P.n = a->n;
   P.xb = a->x_batch;
   P.xs1 = a->x_stride;
-  P.w = a->w_packed;
-  P.ws = a->w_scales;
+  P.w = (const uint4 *)a->w_packed;
+  P.ws = (const unsigned *)a->w_scales;
   P.bias = a->bias;
   P.y = a->y;
   const int64_t blocks = (a->k + LMI_MX_BLOCK - 1) / LMI_MX_BLOCK, tiles_n = (a->n + 31) / 32, tiles_p = (a->pixels + kTile - 1) / kTile;
   LMI_REQUIRE(blocks < (1 << 24) && tiles_n < (1 << 24) && tiles_p < (1 << 24) && a->batch < (1 << 24) && tiles_p * a->batch < (1 << 24), LMI_ERR_LIMIT,
               "lmi_mx_product: k, n or the number of positions is too large");
   P.blocks = (unsigned)blocks;
+  P.all_steps = (int)((blocks + 1) / 2);
   P.tiles_n = (int)tiles_n;
   P.tiles_pixels = (unsigned)tiles_p;
   hipStream_t st = (hipStream_t)stream;
   if (a->x_dtype == LMI_MXFP4) {
-    LMI_REQUIRE(rows && a->batch == 1 && a->x_scales && lmi_is_aligned(a->x, 16), LMI_ERR_BAD_ARG,
+    LMI_REQUIRE(rows && a->batch == 1 && a->x_scales && lmi_is_aligned(a->x, 16) && lmi_is_aligned(a->x_scales, 4), LMI_ERR_BAD_ARG,
                 "lmi_mx_product: quantised x comes as 16-byte aligned rows with their scales, batch 1");
     if (a->y_dtype == LMI_F32) return launch_act<Packed, float, false>(P, a->act, 1, st);
     if (a->y_dtype == LMI_F16) return launch_act<Packed, _Float16, false>(P, a->act, 1, st);

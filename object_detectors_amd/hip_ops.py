@@ -842,19 +842,29 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
     return out
 
 
+def _mx_sizes(shape):
+    """Shapes of an MxTensor's parts: ((G, S, 1024), (G, Q, 256))."""
+    groups = -(-math.prod(shape[:-1]) // 32)
+    steps = -(-shape[-1] // 64)
+    return (groups, steps, 1024), (groups, -(-steps // 4), 256)
+
+
 class MxTensor:
-    """A tensor (..., k) in MXFP4: blocks of 32 elements along the last dimension share a power-of-two scale.
-    packed uint8 (rows, 16*B): two 4-bit elements per byte, the earlier one in the low half; scales uint8 (rows, B):
-    2^(byte - 127), 255 = NaN; B = ceil(k / 32), the last block filled up with zeros.  4.25 bits per element."""
+    """A tensor (..., k) in MXFP4: blocks of 32 elements along the last dimension share a power-of-two scale; 4.25 bits per
+    element.  The blocks lie in the order the matrix instruction takes them, rows in groups of 32, k in steps of 64 (two
+    blocks): packed uint8 (G, S, 1024), a step's kilobyte as (block, row, 16 bytes), two elements per byte, the earlier one in
+    the low half; scales uint8 (G, Q, 256), the bytes of four steps as (block, row, step): 2^(byte - 127), 255 = NaN.
+    G = ceil(rows / 32), S = ceil(k / 64), Q = ceil(S / 4); what lies beyond the tensor is zero."""
 
     __slots__ = ("packed", "scales", "shape")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, shape):
         self.packed, self.scales, self.shape = packed, scales, torch.Size(shape)
-        rows, blocks = math.prod(self.shape[:-1]), -(-self.shape[-1] // _lib.LMI_MX_BLOCK)
-        for t, s, name in ((packed, (rows, 16 * blocks), "packed"), (scales, (rows, blocks), "scales")):
+        if len(self.shape) < 1 or self.shape[-1] < 1:
+            raise ValueError("MxTensor: shape must end in at least one element")
+        for t, s, name in zip((packed, scales), _mx_sizes(self.shape), ("packed", "scales")):
             if t.dtype != torch.uint8 or tuple(t.shape) != s or not t.is_contiguous() or t.device != packed.device:
-                raise ValueError(f"MxTensor: {name} must be a contiguous uint8 tensor of shape {s}")
+                raise ValueError(f"MxTensor: {name} must be a contiguous uint8 tensor of shape {s} on one device with the other")
 
     @property
     def device(self) -> torch.device:
@@ -887,9 +897,8 @@ def mx_quantize(x: torch.Tensor) -> MxTensor:
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError("mx_quantize: x must hold at least one element in its last dimension")
     shape, k, dev = x.shape, x.shape[-1], x.device
-    blocks, rows = -(-k // _lib.LMI_MX_BLOCK), math.prod(x.shape[:-1])
-    packed = torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=dev)
-    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=dev)
+    rows = math.prod(shape[:-1])
+    packed, scales = (torch.empty(s, dtype=torch.uint8, device=dev) for s in _mx_sizes(shape))
     if rows:
         x, _, stride = _rows_of(x)
         with _on(dev):

@@ -67,7 +67,8 @@ def test_every_layer_of_a_forward(dtype, channels_last):
         xr = a.permute(0, 2, 3, 1).reshape(-1, k).double().cpu().numpy()
         # the weights the layer holds: an fp16 network folds its rounded weights
         m = mods[name]
-        wq = OM.dequantize(OM.unpack(m.packed.cpu().numpy()), m.scales.cpu().numpy(), k)
+        packed, scales, _ = OM.rows_of(m.packed.cpu().numpy(), m.scales.cpu().numpy(), w.shape[0], k)
+        wq = OM.dequantize(OM.unpack(packed), scales, k)
         if dtype == torch.float32:
             assert np.array_equal(wq, OM.values(w.double().cpu().numpy()))
         xq = OM.values(xr)

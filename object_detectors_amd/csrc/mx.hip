@@ -178,7 +178,8 @@ struct Product {
 constexpr int kTile = 64;   // positions per workgroup
 
 template <int ACT> __device__ __forceinline__ float activate(float v) {
-  if (ACT == LMI_ACT_SILU) return v / (1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+  // v_exp_f32 and v_rcp_f32, an ulp each: an IEEE division here made the results' arithmetic, not their bytes, the bound of shallow products
+  if (ACT == LMI_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
   return v;
 }
 
@@ -336,26 +337,57 @@ template <int BYTE> __device__ __forceinline__ void mfma2(f16x (&acc)[2], const 
   acc[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b1), acc[1], 4, 4, BYTE, (int)sa, BYTE, (int)sb1);
 }
 
-// steps [q0, q1) of four, of the ns in LDS, for weight tile nt
-__device__ __forceinline__ void multiply(const Product &P, int nt, int s0, int ns, int q0, int dq, const uint4 *frags, const unsigned *words, int lane, f16x (&acc)[2]) {
+// One quad of steps of G weight tiles: fragments and scale words
+template <int G> struct Quad {
+  uint4 a[G][4];
+  unsigned s[G];
+};
+template <int G> __device__ __forceinline__ void load_quad(Quad<G> &Q, const uint4 *w, const unsigned *ws, long long tile_w, long long tile_s, int q, int last) {
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    Q.s[g] = ws[g * tile_s + q * 64];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) Q.a[g][i] = w[g * tile_w + (q * 4 + i < last ? q * 4 + i : last) * 64];   // beyond the last step: any of the tile's, not used
+  }
+}
+
+// Weight tiles nt .. nt + G - 1 times the ns steps in LDS (steps s0 ..), quads q0, q0 + dq, ...  The next quad's weights are on their way
+// while the matrix instructions run; every fragment read from LDS serves G of them.
+template <int G>
+__device__ __forceinline__ void multiply(const Product &P, int nt, int s0, int ns, int q0, int dq, const uint4 *frags, const unsigned *words, int lane, f16x (&acc)[G][2]) {
   const int wl = weight_lane(lane), quads = (P.all_steps + 3) / 4;
   const uint4 *w = P.w + ((long long)nt * P.all_steps + s0) * 64 + wl;
   const unsigned *ws = P.ws + ((long long)nt * quads + s0 / 4) * 64 + wl;
+  const long long tile_w = (long long)P.all_steps * 64, tile_s = (long long)quads * 64;
+  if (q0 * 4 >= ns) return;
+  Quad<G> cur, next;
+  load_quad<G>(cur, w, ws, tile_w, tile_s, q0, ns - 1);
   for (int q = q0; q * 4 < ns; q += dq) {
-    const unsigned sa = ws[q * 64], sb0 = words[q * 128 + lane], sb1 = words[q * 128 + 64 + lane];
-    const uint4 *wq = w + q * 256, *f = frags + q * 512 + lane;
-    if (q * 4 + 4 <= ns) {
-      const uint4 a0 = wq[0], a1 = wq[64], a2 = wq[128], a3 = wq[192];
-      mfma2<0>(acc, a0, sa, f[0], f[64], sb0, sb1);
-      mfma2<1>(acc, a1, sa, f[128], f[192], sb0, sb1);
-      mfma2<2>(acc, a2, sa, f[256], f[320], sb0, sb1);
-      mfma2<3>(acc, a3, sa, f[384], f[448], sb0, sb1);
-    } else {
-      const int left = ns - q * 4;
-      mfma2<0>(acc, wq[0], sa, f[0], f[64], sb0, sb1);
-      if (left > 1) mfma2<1>(acc, wq[64], sa, f[128], f[192], sb0, sb1);
-      if (left > 2) mfma2<2>(acc, wq[128], sa, f[256], f[320], sb0, sb1);
+    if ((q + dq) * 4 < ns) load_quad<G>(next, w, ws, tile_w, tile_s, q + dq, ns - 1);
+    const unsigned sb0 = words[q * 128 + lane], sb1 = words[q * 128 + 64 + lane];
+    const uint4 *f = frags + q * 512 + lane;
+    const int left = ns - q * 4;
+    {
+      const uint4 b0 = f[0], b1 = f[64];
+#pragma unroll
+      for (int g = 0; g < G; ++g) mfma2<0>(acc[g], cur.a[g][0], cur.s[g], b0, b1, sb0, sb1);
     }
+    if (left > 1) {
+      const uint4 b0 = f[128], b1 = f[192];
+#pragma unroll
+      for (int g = 0; g < G; ++g) mfma2<1>(acc[g], cur.a[g][1], cur.s[g], b0, b1, sb0, sb1);
+    }
+    if (left > 2) {
+      const uint4 b0 = f[256], b1 = f[320];
+#pragma unroll
+      for (int g = 0; g < G; ++g) mfma2<2>(acc[g], cur.a[g][2], cur.s[g], b0, b1, sb0, sb1);
+    }
+    if (left > 3) {
+      const uint4 b0 = f[384], b1 = f[448];
+#pragma unroll
+      for (int g = 0; g < G; ++g) mfma2<3>(acc[g], cur.a[g][3], cur.s[g], b0, b1, sb0, sb1);
+    }
+    cur = next;
   }
 }
 
@@ -386,9 +418,12 @@ __device__ __forceinline__ void store_tile(const Product &P, long long image, lo
   }
 }
 
-// KSPLIT: one weight tile per workgroup, its waves share k (few positions); else the waves share the weight tiles.
+// The weight tiles of a workgroup are dealt to its waves in runs of nearly equal length; which wave gets the longer ones turns with the
+// workgroup, so that no SIMD gets them all.  A wave takes its run two tiles at a time.  k longer than LDS holds: the positions are
+// quantised again for every round of tiles.
+// KSPLIT: one weight tile per workgroup, its waves share k (few positions).
 template <typename T, typename Y, bool PLANES, bool VEC, int ACT, bool KSPLIT>
-__global__ __launch_bounds__(256) void mx_product_kernel(const Product P) {
+__global__ __launch_bounds__(256, KSPLIT ? 1 : 3) void mx_product_kernel(const Product P) {
   extern __shared__ uint4 lds[];
   uint4 *frags = lds;
   unsigned char *bytes = (unsigned char *)(lds + (long long)P.steps * 128);
@@ -400,43 +435,428 @@ __global__ __launch_bounds__(256) void mx_product_kernel(const Product P) {
   const int nt0 = blockIdx.y * P.split_n;
   const int nt1 = nt0 + P.split_n < P.tiles_n ? nt0 + P.split_n : P.tiles_n;
   const bool once = P.all_steps <= P.steps;
-  const int group = KSPLIT ? 1 : 4;
-  for (int g0 = nt0; g0 < nt1; g0 += group) {
-    const int nt = KSPLIT ? g0 : g0 + wave;
-    f16x acc[2] = {};
+  if constexpr (KSPLIT) {
+    f16x acc[1][2] = {};
     for (int s0 = 0; s0 < P.all_steps; s0 += P.steps) {
       const int ns = P.all_steps - s0 < P.steps ? P.all_steps - s0 : P.steps;
-      if (!once || g0 == nt0) {
-        __syncthreads();   // LDS is free again
-        fill<T, PLANES, VEC>(P, image, p0, live, s0, ns, frags, bytes);
-        __syncthreads();
-      }
-      if (nt < nt1) multiply(P, nt, s0, ns, KSPLIT ? wave : 0, KSPLIT ? 4 : 1, frags, words, lane, acc);
+      __syncthreads();   // LDS is free again
+      fill<T, PLANES, VEC>(P, image, p0, live, s0, ns, frags, bytes);
+      __syncthreads();
+      multiply<1>(P, nt0, s0, ns, wave, 4, frags, words, lane, acc);
     }
-    if (KSPLIT) {   // sums of the four waves, in their order
-      __syncthreads();
-      float *part = (float *)lds;   // [3][32][64]
-      if (wave) {
+    __syncthreads();   // sums of the four waves, in their order
+    float *part = (float *)lds;   // [3][32][64]
+    if (wave) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[((wave - 1) * 32 + h * 16 + i) * 64 + lane] = acc[h][i];
+        for (int i = 0; i < 16; ++i) part[((wave - 1) * 32 + h * 16 + i) * 64 + lane] = acc[0][h][i];
+    }
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+#pragma unroll
+          for (int w = 0; w < 3; ++w) acc[0][h][i] += part[(w * 32 + h * 16 + i) * 64 + lane];
+        }
+      store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt0, lane, acc[0]);
+    }
+  } else {
+    const int count = nt1 - nt0, turn = (wave + blockIdx.x) & 3;
+    const int mine = count / 4 + (turn < count % 4), first = nt0 + turn * (count / 4) + (turn < count % 4 ? turn : count % 4);
+    const int rounds = ((count + 3) / 4 + 1) / 2;   // of the longest run
+    for (int r = 0; r < rounds; ++r) {
+      const int nt = first + 2 * r, have = mine - 2 * r;
+      f16x acc[2][2] = {};
+      for (int s0 = 0; s0 < P.all_steps; s0 += P.steps) {
+        const int ns = P.all_steps - s0 < P.steps ? P.all_steps - s0 : P.steps;
+        if (!once || r == 0) {
+          __syncthreads();   // LDS is free again
+          fill<T, PLANES, VEC>(P, image, p0, live, s0, ns, frags, bytes);
+          __syncthreads();
+        }
+        if (have >= 2) {
+          multiply<2>(P, nt, s0, ns, 0, 1, frags, words, lane, acc);
+        } else if (have == 1) {
+          f16x one[1][2] = {{acc[0][0], acc[0][1]}};
+          multiply<1>(P, nt, s0, ns, 0, 1, frags, words, lane, one);
+          acc[0][0] = one[0][0];
+          acc[0][1] = one[0][1];
+        }
       }
-      __syncthreads();
-      if (wave == 0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-#pragma unroll
-            for (int w = 0; w < 3; ++w) acc[h][i] += part[(w * 32 + h * 16 + i) * 64 + lane];
-          }
-        store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt, lane, acc);
-      }
-    } else if (nt < nt1) {
-      store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt, lane, acc);
+      if (have >= 1) store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt, lane, acc[0]);
+      if (have >= 2) store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt + 1, lane, acc[1]);
     }
   }
+}
+
+// One wave, 64 positions, all of k (at most 128) in registers: what a lane quantises is its operand.  No LDS, no barrier: the waves of
+// a CU drift apart, so that some load while others multiply.
+constexpr int kWaveSteps = 2;   // deeper ones stream faster: 64 x 192 -> 192 on 80 x 80: 80 us here, 68 streamed; 128 -> 640: 141 and 172; 48 -> 32 on 160 x 160: 56 and 84
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+template <typename T, bool PLANES> struct Raw;   // one step's values of a lane before they are quantised
+template <> struct Raw<float, true> {
+  float2 v[32];
+};
+template <typename T> struct Raw<T, true> {
+  unsigned v[32];
+};
+template <typename T> struct Raw<T, false> {
+  float v[8][8];
+};
+
+// Addresses are a base that is the same for the wave (scalar registers) plus a 32-bit offset of the lane: the launcher sees to it that
+// 32 channels or rows fit.
+template <typename W> __device__ __forceinline__ const W *at(const void *base, unsigned offset) { return (const W *)((const char *)base + offset); }
+
+// `in` channels (32 or more: all) of two neighbouring pixels from base + offset on; base is uniform
+template <typename T> __device__ __forceinline__ void load_planes(const T *base, unsigned offset, long long stride, bool live, int in, Raw<T, true> &r) {
+  typedef typename std::remove_reference<decltype(r.v[0])>::type W;
+  if (live && in >= 32) {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) r.v[u] = *at<W>(base + u * stride, offset);
+  } else {   // positions beyond the image, the last channels
+#pragma unroll
+    for (int u = 0; u < 32; ++u) r.v[u] = live && u < in ? *at<W>(base + u * stride, offset) : W{};
+  }
+}
+__device__ __forceinline__ void quantize_raw(const Raw<float, true> &r, uint4 (&f)[2], unsigned (&byte)[2]) {
+  float a[32];
+#pragma unroll
+  for (int u = 0; u < 32; ++u) a[u] = r.v[u].x;
+  f[0] = quantize_block(a, byte[0]);
+#pragma unroll
+  for (int u = 0; u < 32; ++u) a[u] = r.v[u].y;
+  f[1] = quantize_block(a, byte[1]);
+}
+template <typename T> __device__ __forceinline__ void quantize_raw(const Raw<T, true> &r, uint4 (&f)[2], unsigned (&byte)[2]) { quantize_pair16<T>(r.v, f, byte); }
+
+// the sums of weight tile nt start at the bias
+__device__ __forceinline__ void start_sums(const Product &P, int nt, int lane, f16x (&acc)[2]) {
+  const long long n0 = (long long)nt * 32 + 16 * (lane >> 5);
+  acc[0] = f16x{};
+  if (P.bias) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[0][i] = n0 + i < P.n ? P.bias[n0 + i] : 0.0f;
+  }
+  acc[1] = acc[0];
+}
+
+// planes: a lane holds 16 weight rows' results of two neighbouring positions.  Results are not read again soon: stored past the caches
+// (the 160 x 160 maps of a batch of 64, 48 -> 32 channels: 75 -> 56 us with the sums starting at the bias).
+template <typename Y>
+__device__ __forceinline__ void store_planes(const Product &P, Y *y, long long p0, int live, int nt, int lane, int act, const f16x (&acc)[2]) {
+  const int px = 2 * (lane & 31), n0 = 16 * (lane >> 5);
+  const long long left = P.n - nt * 32ll - n0;
+  const unsigned offset = (unsigned)(n0 * P.pixels + px) * sizeof(Y);
+  Y *base = y + nt * 32ll * P.pixels + p0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float v0 = acc[0][i], v1 = acc[1][i];
+    if (act) {
+      v0 = activate<LMI_ACT_SILU>(v0);
+      v1 = activate<LMI_ACT_SILU>(v1);
+    }
+    typedef Y y2 __attribute__((ext_vector_type(2)));
+    if (px < live && i < left) __builtin_nontemporal_store(y2{(Y)v0, (Y)v1}, (y2 *)((char *)(base + i * P.pixels) + offset));
+  }
+}
+
+// rows: a lane holds 16 neighbouring results of either of its two positions (32 apart)
+template <typename Y>
+__device__ __forceinline__ void store_rows(const Product &P, Y *y, long long p0, int live, int nt, int lane, int act, int vec, const f16x (&acc)[2]) {
+  const long long n0 = (long long)nt * 32 + 16 * (lane >> 5);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int px = 32 * h + (lane & 31);
+    if (px >= live) continue;
+    Y *q = y + (p0 + px) * P.n + n0;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[i] = acc[h][i];
+      if (act) v[i] = activate<LMI_ACT_SILU>(v[i]);
+    }
+    if (vec && n0 + 16 <= P.n) {
+      constexpr int W = 16 / sizeof(Y);
+      typedef Y yw __attribute__((ext_vector_type(W)));
+#pragma unroll
+      for (int j = 0; j < 16 / W; ++j) {
+        yw o;
+#pragma unroll
+        for (int u = 0; u < W; ++u) o[u] = (Y)v[j * W + u];
+        ((yw *)q)[j] = o;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (n0 + i < P.n) q[i] = (Y)v[i];
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P, int act, long long tiles) {
+  const int lane = threadIdx.x & 63;
+  const unsigned tile = blockIdx.x * 4 + wave_id();
+  if (tile >= tiles) return;
+  const long long image = tile / P.tiles_pixels;
+  const long long p0 = (long long)(tile % P.tiles_pixels) * kTile;
+  const int live = (int)(P.pixels - p0 < kTile ? P.pixels - p0 : kTile);
+  const T *x = (const T *)P.x + image * P.xb + p0;
+  const unsigned offset = (unsigned)((lane >> 5) * 32 * P.xs1 + 2 * (lane & 31)) * sizeof(T);
+  const bool mine = 2 * (lane & 31) < live;
+  const int S = P.all_steps, half = lane >> 5;
+  uint4 f[kWaveSteps][2];
+  unsigned sw[2] = {};
+  Raw<T, true> raw;
+#pragma unroll
+  for (int s = 0; s < kWaveSteps; ++s) {
+    if (s < S) {
+      const int left = (int)(P.k - 64ll * s) - 32 * half;
+      load_planes<T>(x + 64ll * s * P.xs1, offset, P.xs1, mine, left < 0 ? 0 : left, raw);
+      unsigned byte[2];
+      quantize_raw(raw, f[s], byte);
+      sw[0] |= byte[0] << (8 * s);
+      sw[1] |= byte[1] << (8 * s);
+    }
+  }
+  const int wl = weight_lane(lane);
+  const int nt0 = blockIdx.y * P.split_n;
+  const int nt1 = nt0 + P.split_n < P.tiles_n ? nt0 + P.split_n : P.tiles_n;
+  T *y = (T *)P.y + image * P.pixels * P.n;
+  for (int nt = nt0; nt < nt1; ++nt) {
+    f16x acc[2];
+    start_sums(P, nt, lane, acc);
+    const uint4 *w = P.w + (long long)nt * S * 64 + wl;
+    const unsigned sa = P.ws[nt * 64 + wl];
+    uint4 a[kWaveSteps];
+#pragma unroll
+    for (int s = 0; s < kWaveSteps; ++s) a[s] = w[(s < S ? s : S - 1) * 64];
+    mfma2<0>(acc, a[0], sa, f[0][0], f[0][1], sw[0], sw[1]);
+    if (S > 1) mfma2<1>(acc, a[1], sa, f[1][0], f[1][1], sw[0], sw[1]);
+    store_planes<T>(P, y, p0, live, nt, lane, act, acc);
+  }
+}
+
+template <typename T> bool launch_wave_planes(Product P, int act, long long batch, hipStream_t st) {
+  const long long tiles = batch * P.tiles_pixels;
+  if (P.all_steps > kWaveSteps || tiles < 512) return false;
+  const long long split = tiles < 2048 ? (2048 + tiles - 1) / tiles : 1;
+  P.split_n = (int)((P.tiles_n + split - 1) / split);
+  const dim3 grid((unsigned)((tiles + 3) / 4), (unsigned)((P.tiles_n + P.split_n - 1) / P.split_n));
+  mx_wave_planes_kernel<T><<<grid, 256, 0, st>>>(P, act, tiles);
+  return true;
+}
+
+// Streaming product: 128 positions x up to 64 * NT weight rows per workgroup, k in chunks of two steps.  While the matrix instructions run
+// on one chunk, the next chunk's activations are on their way to registers and its weights on their way to LDS; an
+// activation block is quantised by the thread that loaded it.  Waves are dealt 2 (positions) x 2 (weight rows), each 64 positions x 32 * NT
+// rows of sums in registers: a fragment read from LDS serves 2 or NT matrix instructions.
+constexpr int kChunkTile = 128;
+
+template <typename T, bool PLANES> struct Chunk;   // what a thread holds of a chunk
+// planes: two neighbouring pixels x one block
+template <typename T> struct Chunk<T, true> {
+  Raw<T, true> raw;
+  __device__ __forceinline__ void load(const Product &P, const T *x, int live, int chunk) {
+    const int pair = threadIdx.x & 63;
+    const long long c0 = (4ll * chunk + wave_id()) * 32;
+    load_planes<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, 2 * pair < live, c0 < P.k ? (int)(P.k - c0 < 32 ? P.k - c0 : 32) : 0, raw);
+  }
+  __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) const {
+    const int pair = threadIdx.x & 63, kl = wave_id();
+    const int sub = (pair >> 5) * 2, at = (kl & 1) * 32 + (pair & 31);
+    uint4 f[2];
+    unsigned byte[2];
+    quantize_raw(raw, f, byte);
+#pragma unroll
+    for (int px = 0; px < 2; ++px) {
+      xb[kl >> 1][sub + px][at] = f[px];
+      ((unsigned char *)&xs[sub + px][at])[kl >> 1] = (unsigned char)byte[px];
+    }
+  }
+};
+// rows: eight pieces of 8 elements, four lanes per block
+template <typename T> struct Chunk<T, false> {
+  typedef T piece __attribute__((ext_vector_type(8)));
+  piece v[8];
+  __device__ __forceinline__ void load(const Product &P, const T *x, int live, int chunk) {
+    const int t = threadIdx.x;
+    const int row = t >> 4;
+    const unsigned offset = (unsigned)(row * P.xs1 + (t & 15) * 8) * sizeof(T);
+    const T *base = x + chunk * 128ll;
+    const long long n = P.k - chunk * 128ll - (t & 15) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T *q = base + i * 16 * P.xs1;
+      if (row + 16 * i < live && n >= 8) {
+        v[i] = *at<piece>(q, offset);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[i][u] = row + 16 * i < live && u < n ? *at<T>(q, offset + u * sizeof(T)) : (T)0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) const {
+    const int t = threadIdx.x, quarter = t & 3, block = (t >> 2) & 3;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = (t >> 4) + 16 * i, at = (block & 1) * 32 + (row & 31);
+      float e[8];
+      unsigned m = 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        e[u] = to_float(v[i][u]);
+        m = max(m, __float_as_uint(e[u]) & 0x7fffffffu);
+      }
+      m = max(m, __shfl_xor(m, 1));
+      m = max(m, __shfl_xor(m, 2));
+      const unsigned byte = scale_byte(m);
+      ((unsigned *)&xb[block >> 1][row >> 5][at])[quarter] = pack8(e, scale_value(byte));
+      if (quarter == 0) ((unsigned char *)&xs[row >> 5][at])[block >> 1] = (unsigned char)byte;
+    }
+  }
+};
+
+// 64 lanes x SIZE bytes from src (per lane) to dst (the wave's base; lane l lands at l * SIZE).  Complete for the workgroup after a
+// wait for vmcnt(0) and a barrier.
+template <int SIZE> __device__ __forceinline__ void to_lds(const void *src, void *dst) {
+  const auto from = (const __attribute__((address_space(1))) void *)src;
+  const auto to = (__attribute__((address_space(3))) void *)dst;
+  if constexpr (SIZE == 16) __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds(from, to, 4, 0, 0);
+}
+
+template <typename T, typename Y, bool PLANES, int NT>
+__global__ __launch_bounds__(256, NT <= 2 ? 3 : 2) void mx_stream_kernel(const Product P, int act, int splits, long long tiles, int vec_y) {
+  __shared__ uint4 xb[2][2][4][64];
+  __shared__ unsigned xs[2][4][64];
+  __shared__ uint4 wb[2][2][2 * NT][64];
+  __shared__ unsigned wsb[2][2 * NT][64];
+  const int lane = threadIdx.x & 63, wave = wave_id(), wp = wave & 1, wn = wave >> 1;
+  // workgroups go round the eight XCDs: the parts of one tile of positions are eight apart, so that they share an L2
+  const long long tile = (long long)(blockIdx.x / (8 * splits)) * 8 + (blockIdx.x & 7);
+  const int part = (int)(blockIdx.x / 8) % splits;
+  if (tile >= tiles) return;
+  const long long image = tile / P.tiles_pixels;
+  const long long p0 = (tile - image * P.tiles_pixels) * kChunkTile;
+  const int live = (int)(P.pixels - p0 < kChunkTile ? P.pixels - p0 : kChunkTile);
+  const int S = P.all_steps, quads = (S + 3) / 4, chunks = (S + 1) / 2, nt0 = part * 2 * NT;
+
+  auto load_weights = [&](int c, int buf) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {   // 4 * NT fragments over four waves
+      const int id = j * 4 + wave, step = id & 1, t = id >> 1;
+      const int nt = nt0 + t < P.tiles_n ? nt0 + t : P.tiles_n - 1, s = 2 * c + step < S ? 2 * c + step : S - 1;
+      to_lds<16>(P.w + ((long long)nt * S + s) * 64 + lane, &wb[buf][step][t][0]);
+    }
+#pragma unroll
+    for (int j = 0; j < (NT + 1) / 2; ++j) {
+      const int t = j * 4 + wave;
+      if (t < 2 * NT) {
+        const int nt = nt0 + t < P.tiles_n ? nt0 + t : P.tiles_n - 1;
+        to_lds<4>(P.ws + ((long long)nt * quads + c / 2) * 64 + lane, &wsb[buf][t][0]);
+      }
+    }
+  };
+  const long long g0 = p0 >> 5;   // Packed: first group of rows
+  auto load_packed = [&](int c, int buf) {
+    const unsigned char *base = (const unsigned char *)P.x;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int id = j * 4 + wave, step = id & 1, sub = id >> 1;
+      const long long groups = (P.pixels + 31) >> 5, g = g0 + sub < groups ? g0 + sub : groups - 1;
+      const int s = 2 * c + step < S ? 2 * c + step : S - 1;
+      to_lds<16>(base + ((g * S + s) * 64 + lane) * 16, &xb[buf][step][sub][0]);
+    }
+    const long long groups = (P.pixels + 31) >> 5, g = g0 + wave < groups ? g0 + wave : groups - 1;
+    to_lds<4>(P.xs + (g * quads + c / 2) * 64 + lane, &xs[buf][wave][0]);
+  };
+
+  f16x acc[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) start_sums(P, nt0 + wn * NT + t, lane, acc[t]);
+  const int wl = weight_lane(lane);
+  auto multiply_chunk = [&](int c, int buf) {
+    const int shift = 16 * (c & 1);
+    unsigned sb0 = xs[buf][2 * wp][lane], sb1 = xs[buf][2 * wp + 1][lane];
+    if constexpr (__is_same(T, Packed)) sb0 >>= shift, sb1 >>= shift;
+    unsigned sa[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sa[t] = wsb[buf][wn * NT + t][wl] >> shift;
+    {
+      const uint4 b0 = xb[buf][0][2 * wp][lane], b1 = xb[buf][0][2 * wp + 1][lane];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) mfma2<0>(acc[t], wb[buf][0][wn * NT + t][wl], sa[t], b0, b1, sb0, sb1);
+    }
+    if (2 * c + 1 < S) {
+      const uint4 b0 = xb[buf][1][2 * wp][lane], b1 = xb[buf][1][2 * wp + 1][lane];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) mfma2<1>(acc[t], wb[buf][1][wn * NT + t][wl], sa[t], b0, b1, sb0, sb1);
+    }
+  };
+
+  if constexpr (__is_same(T, Packed)) {
+    load_weights(0, 0);
+    load_packed(0, 0);
+    for (int c = 0; c < chunks; ++c) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this chunk's weights and rows are in LDS
+      __syncthreads();
+      if (c + 1 < chunks) {
+        load_weights(c + 1, (c + 1) & 1);
+        load_packed(c + 1, (c + 1) & 1);
+      }
+      multiply_chunk(c, c & 1);
+    }
+  } else {
+    const T *x = (const T *)P.x + image * P.xb + (PLANES ? p0 : p0 * P.xs1);
+    Chunk<T, PLANES> hold;
+    load_weights(0, 0);
+    hold.load(P, x, live, 0);
+    for (int c = 0; c < chunks; ++c) {
+      hold.put(xb[c & 1], xs[c & 1]);                    // chunk c - 2 used this buffer: every wave is past the barrier of c - 1
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this chunk's weights are in LDS
+      __syncthreads();
+      if (c + 1 < chunks) {
+        load_weights(c + 1, (c + 1) & 1);                // chunk c - 1 used this buffer: every wave is past it
+        hold.load(P, x, live, c + 1);
+      }
+      multiply_chunk(c, c & 1);
+    }
+  }
+
+  Y *y = (Y *)P.y + image * P.pixels * P.n;
+  const int live_w = live - 64 * wp;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int nt = nt0 + wn * NT + t;
+    if (nt < P.tiles_n) {
+      if constexpr (PLANES) store_planes<Y>(P, y, p0 + 64 * wp, live_w, nt, lane, act, acc[t]);
+      else store_rows<Y>(P, y, p0 + 64 * wp, live_w, nt, lane, act, vec_y, acc[t]);
+    }
+  }
+}
+
+template <typename T, typename Y, bool PLANES> bool launch_stream(Product P, int act, long long batch, hipStream_t st) {
+  P.tiles_pixels = (unsigned)((P.pixels + kChunkTile - 1) / kChunkTile);
+  const long long tiles = batch * P.tiles_pixels;
+  constexpr int kMaxNT = sizeof(Y) == 4 && !__is_same(T, Packed) ? 4 : 5;
+  int splits = (P.tiles_n + 2 * kMaxNT - 1) / (2 * kMaxNT);
+  while (tiles * splits < 256 && splits * 2 <= P.tiles_n) splits *= 2;
+  int nt = (P.tiles_n + 2 * splits - 1) / (2 * splits);
+  splits = (P.tiles_n + 2 * nt - 1) / (2 * nt);
+  const int vec_y = (uintptr_t)P.y % 16 == 0 && P.n * sizeof(Y) % 16 == 0;
+  const unsigned grid = (unsigned)((tiles + 7) / 8 * 8 * splits);
+  if (nt == 1) mx_stream_kernel<T, Y, PLANES, 1><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  else if (nt == 2) mx_stream_kernel<T, Y, PLANES, 2><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  else if (nt == 3) mx_stream_kernel<T, Y, PLANES, 3><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  else if (nt == 4) mx_stream_kernel<T, Y, PLANES, 4><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  else mx_stream_kernel<T, Y, PLANES, kMaxNT><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  return true;
 }
 
 constexpr int kMaxSteps = 28;   // 59.5 KB of LDS
@@ -461,12 +881,20 @@ template <typename T, typename Y, bool PLANES, bool VEC, int ACT> int launch_pro
 }
 
 template <typename T, typename Y, bool PLANES> int launch_act(const Product &P, int act, long long batch, hipStream_t st) {
+  constexpr long long kStreamFrom = 4096;
+  if constexpr (__is_same(T, Packed)) {
+    if (batch * P.pixels >= kStreamFrom && launch_stream<T, Y, false>(P, act, batch, st)) return lmi_check_launch("lmi_mx_product");
+  }
   // planes: two pixels of a channel in one load, and of a result in one store; rows: 16-byte loads
   const uintptr_t align = PLANES ? 2 * sizeof(Y) : 16;
   bool vec = false;
   if constexpr (!__is_same(T, Packed)) {
-    vec = (uintptr_t)P.x % align == 0 && P.xb * sizeof(Y) % align == 0 && P.xs1 * sizeof(Y) % align == 0;
+    vec = P.xs1 < (1 << 24) && P.pixels < (1 << 24) && (uintptr_t)P.x % align == 0 && P.xb * sizeof(Y) % align == 0 && P.xs1 * sizeof(Y) % align == 0;
     if (PLANES) vec = vec && P.pixels % 2 == 0 && (uintptr_t)P.y % align == 0;
+    if constexpr (PLANES) {
+      if (vec && launch_wave_planes<T>(P, act, batch, st)) return lmi_check_launch("lmi_mx_product");
+    }
+    if (vec && batch * P.pixels >= kStreamFrom && launch_stream<T, Y, PLANES>(P, act, batch, st)) return lmi_check_launch("lmi_mx_product");
     if (vec)
       return act == LMI_ACT_SILU ? launch_product<T, Y, PLANES, true, LMI_ACT_SILU>(P, batch, st) : launch_product<T, Y, PLANES, true, LMI_ACT_NONE>(P, batch, st);
   }

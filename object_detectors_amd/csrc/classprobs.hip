@@ -11,12 +11,15 @@
 // that equal values fall in class order and no two keys are equal (the result does not depend on the order of atomics).
 //
 // Kernels
-//  evidence_rows_kernel    one workgroup of NT threads per row (and per part of a long row): each thread holds J*V values
-//                          in registers, so a row is read once.  The best `top`: the top-th best of the 64 per-lane
-//                          maxima is a lower bound of the answer; what reaches it (a few dozen of thousands) goes to
-//                          LDS and is ranked there by counting.
-//  evidence_join_kernel    joins the parts of long rows.
-//  evidence_planes_kernel  one thread per row, for rows that lie side by side (class planes): a wave reads 64
+//  evidence_team_kernel    16 lanes per row (a DPP row), up to 128 classes in registers: NMS rows (classes an anchor plane apart, so every
+//                          value is a sector of its own: bound by their latency, many rows in flight) and small rows.  The best are
+//                          taken one by one: a maximum over the 16 lanes, a ballot for its lowest class.
+//  evidence_rows_kernel    a wave (four rows per workgroup) or a workgroup per row, or per part of a long row; 128 bytes of the row per
+//                          thread in registers, so that a row is read once and 64 KB of it are in flight.  The top-th best of the 64
+//                          lane maxima is a lower bound of the answer; what reaches it (a few dozen of thousands) goes to LDS and
+//                          is ranked there by counting.
+//  evidence_join_kernel    joins the parts of long rows, the same way.
+//  evidence_planes_kernel  one thread per row (16-bit types: two), for rows that lie side by side (class planes): a wave reads
 //                          neighbouring rows' values of one class at a time; the alternatives sit in registers.
 #include <hip/hip_fp16.h>
 
@@ -62,14 +65,20 @@ typedef unsigned long long u64;
 __device__ __forceinline__ u64 make_key(unsigned o, unsigned c) { return ((u64)o << 32) | (0xffffffffu - c); }
 __device__ __forceinline__ unsigned key_class(u64 k) { return 0xffffffffu - (unsigned)k; }
 
+// log(1 + d) for -1 <= d <= 1: the logarithm of u = 1 + d rounded, and what the rounding took ((d - (u - 1)) / u, where the division by u in
+// [0.5, 2] changes less than half an ulp of the result; below 0.5 nothing was lost)
+__device__ __forceinline__ float log_1_plus(float d) {
+  const float u = 1.0f + d;
+  return fmaf(__builtin_amdgcn_logf(u), 0.6931471805599453f, d - (u - 1.0f));
+}
 // entropy of one yes / no answer
 __device__ __forceinline__ float answer_entropy_sigmoid(float x) {
   const float a = fabsf(x), e = exp_fast(-a);
-  return log1pf(e) + (e > 0.0f ? a * e / (1.0f + e) : e);   // a infinite: e = 0 and both terms are 0; NaN stays
+  return log_1_plus(e) + (e > 0.0f ? a * e * __builtin_amdgcn_rcpf(1.0f + e) : e);   // a infinite: e = 0 and both terms are 0; NaN stays
 }
 __device__ __forceinline__ float answer_entropy_none(float p) {
   const float a = p == 0.0f ? 0.0f : p * logf(p);
-  const float b = p == 1.0f ? 0.0f : (1.0f - p) * log1pf(-p);
+  const float b = p == 1.0f ? 0.0f : (1.0f - p) * log_1_plus(-p);
   return -a - b;
 }
 template <int ACT> __device__ __forceinline__ float answer_entropy(float x) {
@@ -123,16 +132,78 @@ __device__ __forceinline__ long long label_of(const Evidence &E, long long o, lo
   return (f >= 0.0f && f < 9.0e15f) ? (long long)f : -1;   // NaN -> -1
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+// reductions on the data-parallel primitives: within 16 lanes, then across the wave; every lane gets the result
+template <int CTRL> __device__ __forceinline__ unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false); }
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;   // quad_perm [1,0,3,2], [2,3,0,1]; mirror of 8 and of 16 lanes
+template <typename F> __device__ __forceinline__ unsigned reduce16(unsigned v, F f) {
+  v = f(v, dpp<kXor1>(v));
+  v = f(v, dpp<kXor2>(v));
+  v = f(v, dpp<kHalfMirror>(v));
+  return f(v, dpp<kMirror>(v));
 }
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+struct MaxF {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+};
+struct MinF {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b))); }
+};
+struct SumF {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }
+};
+struct MaxU {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; }
+};
+template <typename F> __device__ __forceinline__ float reduce64(float x, F f) {
+  unsigned v = reduce16(__float_as_uint(x), f);
+  const unsigned a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16), c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+  return __uint_as_float(f(f(a, b), f(c, d)));
 }
+
+// NT threads share a row: one wave (several of them per workgroup, each on its own) or the workgroup
+template <int NT> __device__ __forceinline__ void team_sync() {
+  if (NT == 64) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+
+constexpr int kCand = 256;
+template <int NT> struct TeamShared {
+  float lane_max[NT / 64][64];
+  float red[NT / 64][2];
+  u64 best[NT / 64];
+  u64 cand[kCand + kMaxTop];
+  u64 list[kMaxTop];   // the best so far, descending
+  float threshold;
+  int n;
+};
+
+// the top-th largest of the wave's 64 values (rank by counting; equal values share a rank)
+__device__ __forceinline__ float kth_of_lanes(float v, int top) {
+  int above = 0;
+#pragma unroll 16
+  for (int j = 0; j < 64; ++j) above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), j)) > v;
+  return reduce64(above < top ? v : INFINITY, MinF());
+}
+
+// the `top` best of the table's n keys and the list -> list
+template <int NT> __device__ __forceinline__ void rank_candidates(TeamShared<NT> &L, int n, int t, int top) {
+  if (t < top) L.cand[n + t] = L.list[t];
+  team_sync<NT>();
+  n += top;
+  if (t < top) L.list[t] = 0;
+  team_sync<NT>();
+  for (int i = t; i < n; i += NT) {
+    const u64 k = L.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += L.cand[j] > k;
+    if (rank < top && k) L.list[rank] = k;   // keys are distinct unless 0
+  }
+  team_sync<NT>();
+}
+
 __device__ __forceinline__ u64 wave_max_key(u64 v) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
@@ -142,93 +213,38 @@ __device__ __forceinline__ u64 wave_max_key(u64 v) {
   return v;
 }
 
-// the best `top` keys of the workgroup's registers and of the list kept so far -> list (LDS, descending)
-constexpr int kCand = 256;
-template <int NT> struct TopShared {
-  u64 lane_best[NT / 64][64];
-  u64 cand[kCand + kMaxTop];
-  u64 list[kMaxTop];
-  u64 threshold;
-  int n;
-};
-template <int NT, int N, typename Key>
-__device__ __forceinline__ void merge_top(TopShared<NT> &L, Key key, int top) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  u64 best = 0;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const u64 k = key(e);
-    best = k > best ? k : best;
-  }
-  L.lane_best[wave][lane] = best;
-  if (t == 0) L.n = 0;
-  __syncthreads();
-  if (wave == 0) {   // the top-th best of 64 lane maxima bounds the top-th best of all values from below
-    u64 k = best;
-    for (int w = 1; w < NT / 64; ++w) k = L.lane_best[w][lane] > k ? L.lane_best[w][lane] : k;
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) rank += __shfl(k, j) > k;
-    if (rank == top - 1 && k) L.threshold = k;   // keys are distinct unless 0: at most one lane
-    if (lane == 0) {
-      const u64 any = __ballot(rank == top - 1 && k != 0);
-      if (!any) L.threshold = 1;                 // fewer than `top` lanes hold a value: everything is a candidate
-    }
-  }
-  __syncthreads();
-  u64 thr = L.threshold;
-  const u64 kept = L.list[top - 1];
-  thr = kept > thr ? kept : thr;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const u64 k = key(e);
-    if (k >= thr) {
-      const int at = atomicAdd(&L.n, 1);
-      if (at < kCand) L.cand[at] = k;
-    }
-  }
-  __syncthreads();
-  int n = L.n;
-  if (n <= kCand) {
-    if (t < top) L.cand[n + t] = L.list[t];
-    __syncthreads();
-    n += top;
-    if (t < top) L.list[t] = 0;
-    __syncthreads();
-    for (int i = t; i < n; i += NT) {
-      const u64 k = L.cand[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += L.cand[j] > k;
-      if (rank < top && k) L.list[rank] = k;
-    }
-    __syncthreads();
-    return;
-  }
-  // more candidates than the table holds (values arranged so that few lanes own nearly all of the best): `top` rounds, each
-  // taking the best key below the last one
+// More candidates than the table holds (equal values, or values arranged so that few lanes own nearly all of the best): `top` rounds,
+// each taking the best key below the last one from key(0) .. key(n - 1), read again.
+template <int NT, typename Key> __device__ __forceinline__ void top_by_rounds(TeamShared<NT> &L, Key key, int n, int t, int top) {
+  const int lane = t & 63, wave = t >> 6;
   if (t < top) L.cand[t] = L.list[t];
-  __syncthreads();
+  team_sync<NT>();
   u64 last = ~0ull;
   for (int r = 0; r < top; ++r) {
     u64 b = (t < top && L.cand[t] < last) ? L.cand[t] : 0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
+    for (int e = t; e < n; e += NT) {
       const u64 k = key(e);
       if (k < last && k > b) b = k;
     }
     b = wave_max_key(b);
-    if (lane == 0) L.lane_best[wave][0] = b;
-    __syncthreads();
-    for (int w = 0; w < NT / 64; ++w) b = L.lane_best[w][0] > b ? L.lane_best[w][0] : b;
+    if (lane == 0) L.best[wave] = b;
+    team_sync<NT>();
+    for (int w = 0; w < NT / 64; ++w) b = L.best[w] > b ? L.best[w] : b;
     if (t == 0) L.list[r] = b;
-    __syncthreads();
+    team_sync<NT>();
     last = b;
   }
 }
 
+// The values in `p` as if just loaded: what was computed from them is not kept in registers beside them.
+template <typename P, int J> __device__ __forceinline__ void forget(P (&p)[J]) {
+#pragma unroll
+  for (int j = 0; j < J; ++j) asm volatile("" : "+v"(p[j]));
+}
+
 template <int ACT>
-__device__ void store_row(const Evidence &E, long long row, float ref, float log_s, float h, bool has_label, float label_x,
-                          const u64 *list, int lane) {
+__device__ __forceinline__ void store_row(const Evidence &E, long long row, float ref, float log_s, float h, bool has_label, float label_x,
+                                          const u64 *list, int lane) {
   if (lane == 0) {
     if (E.entropy) E.entropy[row] = h;
     if (E.logprob) E.logprob[row] = has_label ? log_prob<ACT>(label_x, ref, log_s) : NAN;
@@ -240,108 +256,232 @@ __device__ void store_row(const Evidence &E, long long row, float ref, float log
   }
 }
 
+__device__ __forceinline__ void store_nan(const Evidence &E, long long row, int t) {
+  if (t == 0 && E.entropy) E.entropy[row] = NAN;
+  if (t == 0 && E.logprob) E.logprob[row] = NAN;
+  for (int k = t; k < E.top; k += 16) {
+    if (E.top_logprob) E.top_logprob[row * E.top + k] = NAN;
+    if (E.top_index) E.top_index[row * E.top + k] = -1;
+  }
+}
+
+// 16 lanes per row, class j * 16 + l in value j of lane l
+template <typename T, int J, int ACT>
+__global__ __launch_bounds__(256) void evidence_team_kernel(const Evidence E, long long rows) {
+  const int l = threadIdx.x & 15, group = (threadIdx.x & 63) >> 4;
+  const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  bool on = row < rows;
+  const long long o = on ? row / E.n1 : 0, m = on ? row - o * E.n1 : 0;
+  if (on && E.count && m >= E.count[o]) on = false;
+  long long i = m;
+  if (on && E.index) {
+    i = E.index[row];
+    if (i < 0 || i >= E.index_range) {
+      store_nan(E, row, l);
+      on = false;
+    }
+  }
+  const T *x = (const T *)E.x + o * E.s0 + i * E.s1;
+  const int C = (int)E.classes;
+  float v[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = j * 16 + l;
+    v[j] = on && c < C ? to_float(x[c * E.cs]) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
+  }
+  long long label = -1;
+  float lx = 0.0f;
+  if (on && E.labels && l == 0) {
+    label = label_of(E, o, m);
+    if (label >= C) label = -1;
+    if (label >= 0) lx = to_float(x[label * E.cs]);
+  }
+  float ref = 0.0f, log_s = 0.0f, h = 0.0f;
+  if (ACT == LMI_PROB_SOFTMAX) {
+    float mx = v[0];
+#pragma unroll
+    for (int j = 1; j < J; ++j) mx = fmaxf(mx, v[j]);
+    Sums S = {__uint_as_float(reduce16(__float_as_uint(mx), MaxF())), 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < J; ++j) add_value(S, finite_ref(S.m), v[j]);
+    S.s = __uint_as_float(reduce16(__float_as_uint(S.s), SumF()));
+    S.t = __uint_as_float(reduce16(__float_as_uint(S.t), SumF()));
+    softmax_result(S, ref, log_s, h);
+  } else {
+#pragma unroll
+    for (int j = 0; j < J; ++j) h += answer_entropy<ACT>(v[j]);
+    h = __uint_as_float(reduce16(__float_as_uint(h), SumF()));
+  }
+  if (on && l == 0) {
+    if (E.entropy) E.entropy[row] = h;
+    if (E.logprob) E.logprob[row] = label >= 0 ? log_prob<ACT>(lx, ref, log_s) : NAN;
+  }
+  unsigned ord[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) ord[j] = j * 16 + l < C ? order_bits(v[j]) : 0u;
+  for (int r = 0; r < E.top; ++r) {
+    unsigned b = ord[0];
+#pragma unroll
+    for (int j = 1; j < J; ++j) b = ord[j] > b ? ord[j] : b;
+    b = reduce16(b, MaxU());
+    int c = -1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {   // the lowest class that has it
+      const unsigned hit = (unsigned)(__ballot(ord[j] == b) >> (16 * group)) & 0xffffu;
+      if (c < 0 && hit) {
+        const int at = __builtin_ctz(hit);
+        c = j * 16 + at;
+        if (l == at) ord[j] = 0;
+      }
+    }
+    if (on && l == 0) {
+      if (E.top_logprob) E.top_logprob[row * E.top + r] = log_prob<ACT>(order_value(b), ref, log_s);
+      if (E.top_index) E.top_index[row * E.top + r] = c;
+    }
+  }
+}
+
 struct alignas(16) PartHead {
   float m, s, t, pad;
 };
 
-template <typename T, int V> struct Pack {
-  typedef T type __attribute__((ext_vector_type(V)));
-};
-template <typename T> struct Pack<T, 1> {
-  typedef T type;
-};
-
 // V > 1: classes lie side by side and are read in aligned 16-byte groups (the row may start anywhere; the groups at its two ends
 // are read value by value).  V == 1: any class stride.
+template <typename T, int V> struct Group {
+  typedef T type __attribute__((ext_vector_type(V)));
+  __device__ static __forceinline__ float get(const type &p, int u) { return to_float(p[u]); }
+  __device__ static __forceinline__ void set(type &p, int u, T x) { p[u] = x; }
+};
+template <typename T> struct Group<T, 1> {
+  typedef T type;
+  __device__ static __forceinline__ float get(const type &p, int) { return to_float(p); }
+  __device__ static __forceinline__ void set(type &p, int, T x) { p = x; }
+};
+
 template <typename T, int NT, int J, int V, int ACT>
-__device__ __forceinline__ void evidence_row(const Evidence &E, long long row, TopShared<NT> &L, float (&red)[NT / 64][4]) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+__device__ __forceinline__ void evidence_row(const Evidence &E, long long row, int part, int t, TeamShared<NT> &L) {
+  typedef Group<T, V> G;
+  const int lane = t & 63, wave = t >> 6;
   const long long o = row / E.n1, m = row - o * E.n1;
   if (E.count && m >= E.count[o]) return;
   long long i = m;
   if (E.index) {
     i = E.index[row];
     if (i < 0 || i >= E.index_range) {
-      if (t == 0 && E.entropy) E.entropy[row] = NAN;
-      if (t == 0 && E.logprob) E.logprob[row] = NAN;
-      if (t < E.top && E.top_logprob) E.top_logprob[row * E.top + t] = NAN;
-      if (t < E.top && E.top_index) E.top_index[row * E.top + t] = -1;
+      if (t < 16) store_nan(E, row, t);
       return;
     }
   }
   const T *x = (const T *)E.x + o * E.s0 + i * E.s1;
-  const long long c0 = (long long)blockIdx.y * E.part_len;
-  const long long c1 = c0 + E.part_len < E.classes ? c0 + E.part_len : E.classes;
-  long long start = c0;
-  if (V > 1) start -= (long long)(((uintptr_t)(x + c0) & 15) / sizeof(T));
+  // this part's classes [c0, c0 + len); a tile starts up to 15 bytes before them, so that groups are aligned
+  const long long c0 = (long long)part * E.part_len;
+  const int len = (int)(E.classes - c0 < E.part_len ? E.classes - c0 : E.part_len);
+  const T *xp = x + c0 * (V > 1 ? 1 : E.cs);
+  const int start = V > 1 ? -(int)(((uintptr_t)xp & 15) / sizeof(T)) : 0;
 
   if (t < kMaxTop) L.list[t] = 0;
-  Sums S = {-INFINITY, 0.0f, 0.0f};   // softmax: sums with respect to the workgroup's m; else t = the entropy
+  Sums S = {-INFINITY, 0.0f, 0.0f};   // softmax: sums with respect to the team's m; else t = the entropy
   constexpr int N = J * V;
-  for (long long tile = start; tile < c1; tile += (long long)NT * N) {
-    float v[N];
+  const T absent = (T)(ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);   // adds nothing to the sums
+  for (long long tile = start; tile < len; tile += NT * N) {
+    typename G::type p[J];
+    const long long first = tile + t * V;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const long long e0 = tile + ((long long)j * NT + t) * V;
-      if (V > 1 && e0 >= c0 && e0 + V <= c1) {
-        typedef typename Pack<T, V>::type P;
-        const P p = *(const P *)(x + e0);
-#pragma unroll
-        for (int u = 0; u < V; ++u) v[j * V + u] = to_float(((const T *)&p)[u]);
+      const long long e0 = first + j * NT * V;
+      if (V > 1 && e0 >= 0 && e0 + V <= len) {
+        p[j] = *(const typename G::type *)(xp + e0);
       } else {
 #pragma unroll
         for (int u = 0; u < V; ++u) {
           const long long c = e0 + u;
-          v[j * V + u] = c >= c0 && c < c1 ? to_float(x[c * (V > 1 ? 1 : E.cs)]) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
+          G::set(p[j], u, c >= 0 && c < len ? xp[c * (V > 1 ? 1 : E.cs)] : absent);
         }
       }
     }
-    if (ACT == LMI_PROB_SOFTMAX) {
-      float mx = -INFINITY;
+    float mx = -INFINITY, team_mx = -INFINITY;
+    if (ACT == LMI_PROB_SOFTMAX || E.top) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) mx = fmaxf(mx, v[e]);
-      mx = wave_max(mx);
+      for (int e = 0; e < N; ++e) mx = fmaxf(mx, G::get(p[e / V], e % V));   // drops NaN
       if (NT > 64) {
-        if (lane == 0) red[wave][0] = mx;
+        L.lane_max[wave][lane] = mx;
+        if (t == 0) L.n = 0;
         __syncthreads();
-        for (int w = 0; w < NT / 64; ++w) mx = fmaxf(mx, red[w][0]);
+        float q = mx;
+        for (int w = 0; w < NT / 64; ++w) q = fmaxf(q, L.lane_max[w][lane]);
+        mx = q;   // of this lane in every wave
+      } else if (t == 0) {
+        L.n = 0;
       }
-      rebase(S, fmaxf(S.m, mx));
+      team_mx = reduce64(mx, MaxF());
+      if (E.top && wave == 0) {   // the top-th best of 64 lane maxima bounds the top-th best of all values from below
+        const float k = kth_of_lanes(mx, E.top);
+        if (lane == 0) L.threshold = k;
+      }
+    }
+    forget(p);
+    if (ACT == LMI_PROB_SOFTMAX) {
+      rebase(S, fmaxf(S.m, team_mx));
       const float ref = finite_ref(S.m);
 #pragma unroll
-      for (int e = 0; e < N; ++e) add_value(S, ref, v[e]);
+      for (int e = 0; e < N; ++e) add_value(S, ref, G::get(p[e / V], e % V));
     } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) S.t += answer_entropy<ACT>(v[e]);
+      for (int e = 0; e < N; ++e) S.t += answer_entropy<ACT>(G::get(p[e / V], e % V));
     }
     if (E.top) {
-      const long long first = tile + (long long)t * V;
-      merge_top<NT, N>(L, [&](int e) -> u64 {
-        const long long c = first + (e / V) * (NT * V) + e % V;
-        return c >= c0 && c < c1 ? make_key(order_bits(v[e]), (unsigned)c) : 0;
-      }, E.top);
-    } else if (NT > 64 && ACT == LMI_PROB_SOFTMAX) {
-      __syncthreads();   // red[][0] is written again by the next tile
+      team_sync<NT>();
+      float thr = L.threshold;
+      const u64 kept = L.list[E.top - 1];
+      if (kept) {
+        const float k = order_value((unsigned)(kept >> 32));   // a NaN there: only NaNs can still be better
+        thr = k != k ? INFINITY : fmaxf(thr, k);
+      }
+      forget(p);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v = G::get(p[e / V], e % V);
+        if (!(v < thr)) {   // NaN too
+          const long long c = first + (e / V) * (NT * V) + e % V;
+          if (c >= 0 && c < len) {
+            const int at = atomicAdd(&L.n, 1);
+            if (at < kCand) L.cand[at] = make_key(order_bits(v), (unsigned)(c0 + c));
+          }
+        }
+      }
+      team_sync<NT>();
+      const int n = L.n;
+      if (n <= kCand) {
+        rank_candidates<NT>(L, n, t, E.top);
+      } else {
+        const long long lo = tile > 0 ? tile : 0, hi = tile + NT * N < len ? tile + NT * N : len;
+        top_by_rounds<NT>(L, [&](int e) -> u64 {
+          const long long c = lo + e;
+          return make_key(order_bits(to_float(xp[c * (V > 1 ? 1 : E.cs)])), (unsigned)(c0 + c));
+        }, (int)(hi - lo), t, E.top);
+      }
+    } else if (NT > 64) {
+      __syncthreads();   // lane_max is written again by the next tile
     }
   }
-  // sums over the workgroup
-  S.s = wave_sum(S.s);
-  S.t = wave_sum(S.t);
+  // sums over the team
+  S.s = reduce64(S.s, SumF());
+  S.t = reduce64(S.t, SumF());
   if (NT > 64) {
     if (lane == 0) {
-      red[wave][1] = S.s;
-      red[wave][2] = S.t;
+      L.red[wave][0] = S.s;
+      L.red[wave][1] = S.t;
     }
     __syncthreads();
     S.s = S.t = 0.0f;
     for (int w = 0; w < NT / 64; ++w) {
-      S.s += red[w][1];
-      S.t += red[w][2];
+      S.s += L.red[w][0];
+      S.t += L.red[w][1];
     }
   }
   if (wave) return;
   if (E.parts > 1) {
-    unsigned char *out = E.ws + (row * E.parts + blockIdx.y) * (sizeof(PartHead) + (long long)kMaxTop * 8);
+    unsigned char *out = E.ws + (row * E.parts + part) * (sizeof(PartHead) + (long long)kMaxTop * 8);
     if (lane == 0) *(PartHead *)out = PartHead{S.m, S.s, S.t, 0.0f};
     if (lane < E.top) ((u64 *)(out + sizeof(PartHead)))[lane] = L.list[lane];
     return;
@@ -359,53 +499,75 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, T
 }
 
 template <typename T, int NT, int J, int V, int ACT>
-__global__ __launch_bounds__(NT) void evidence_rows_kernel(const Evidence E) {
-  __shared__ TopShared<NT> L;
-  __shared__ float red[NT / 64][4];
-  for (long long row = blockIdx.x; row < E.n0 * E.n1; row += gridDim.x) {   // more rows than a grid holds: several each
-    evidence_row<T, NT, J, V, ACT>(E, row, L, red);
-    __syncthreads();
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, 4) void evidence_rows_kernel(const Evidence E) {
+  constexpr int kTeams = NT == 64 ? 4 : 1;
+  __shared__ TeamShared<NT> L[kTeams];
+  const int team = NT == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int t = threadIdx.x - team * NT;
+  const long long rows = E.n0 * E.n1;
+  for (long long row = (long long)blockIdx.x * kTeams + team; row < rows; row += (long long)gridDim.x * kTeams) {   // more rows than a grid holds: several each
+    evidence_row<T, NT, J, V, ACT>(E, row, blockIdx.y, t, L[team]);
+    team_sync<NT>();
   }
 }
 
-// one wave per row: lane p holds part p (at most 64), whose list is sorted
+// a workgroup per row; lane p of the first wave holds the sums of part p (at most 64); a part's list is sorted
 template <typename T, int ACT>
-__global__ __launch_bounds__(64) void evidence_join_kernel(const Evidence E) {
-  __shared__ u64 list[kMaxTop];
-  const int lane = threadIdx.x;
+__global__ __launch_bounds__(256) void evidence_join_kernel(const Evidence E) {
+  __shared__ TeamShared<256> L;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const long long row = blockIdx.x;   // fewer than 128 of them
   const long long o = row / E.n1, m = row - o * E.n1;
   if (E.count && m >= E.count[o]) return;
   const long long i = E.index ? E.index[row] : m;
   if (E.index && (i < 0 || i >= E.index_range)) return;   // written by the parts
-  const unsigned char *in = E.ws + (row * E.parts + lane) * (sizeof(PartHead) + (long long)kMaxTop * 8);
-  const bool live = lane < E.parts;
-  Sums S = {-INFINITY, 0.0f, 0.0f};
-  if (live) {
-    const PartHead p = *(const PartHead *)in;
-    S = Sums{p.m, p.s, p.t};
+  constexpr long long kPart = sizeof(PartHead) + (long long)kMaxTop * 8;
+  const unsigned char *base = E.ws + row * E.parts * kPart;
+  // thread t: part t / 4, every fourth of its keys from t % 4 on; all loads at once
+  u64 keys[kMaxTop / 4];
+#pragma unroll
+  for (int j = 0; j < kMaxTop / 4; ++j) {
+    const int k = j * 4 + (t & 3);
+    keys[j] = (t >> 2) < E.parts && k < E.top ? ((const u64 *)(base + (t >> 2) * kPart + sizeof(PartHead)))[k] : 0;
   }
+  PartHead head = {-INFINITY, 0.0f, 0.0f, 0.0f};
+  u64 best = 0;
+  if (lane < E.parts) {
+    head = *(const PartHead *)(base + lane * kPart);
+    if (E.top) best = *(const u64 *)(base + lane * kPart + sizeof(PartHead));
+  }
+  Sums S = {head.m, head.s, head.t};
   float ref = 0.0f, log_s = 0.0f, h;
   if (ACT == LMI_PROB_SOFTMAX) {
-    rebase(S, wave_max(S.m));
-    S.s = wave_sum(S.s);
-    S.t = wave_sum(S.t);
+    rebase(S, reduce64(S.m, MaxF()));
+    S.s = reduce64(S.s, SumF());
+    S.t = reduce64(S.t, SumF());
     softmax_result(S, ref, log_s, h);
   } else {
-    h = wave_sum(S.t);
+    h = reduce64(S.t, SumF());
   }
-  const u64 *keys = (const u64 *)(in + sizeof(PartHead));
-  int at = 0;
-  u64 head = live && E.top ? keys[0] : 0;
-  for (int r = 0; r < E.top; ++r) {
-    const u64 b = wave_max_key(head);
-    if (lane == 0) list[r] = b;
-    if (live && head == b) {
-      ++at;
-      head = at < E.top ? keys[at] : 0;
-    }
+  if (E.top) {   // the top-th best of the parts' best bounds the answer from below; keys are distinct, so are ranks
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) above += (u64)__shfl(best, j) > best;
+    const u64 sel = __ballot(above == E.top - 1 && best != 0);
+    const u64 thr = sel ? (u64)__shfl(best, __builtin_ctzll(sel)) : 1;
+    if (t == 0) L.n = 0;
+    if (t < kMaxTop) L.list[t] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kMaxTop / 4; ++j)
+      if (keys[j] >= thr) {
+        const int at = atomicAdd(&L.n, 1);
+        if (at < kCand) L.cand[at] = keys[j];
+      }
+    __syncthreads();
+    const int n = L.n;
+    if (n <= kCand) rank_candidates<256>(L, n, t, E.top);
+    else top_by_rounds<256>(L, [&](int e) -> u64 { return e % kMaxTop < E.top ? ((const u64 *)(base + e / kMaxTop * kPart + sizeof(PartHead)))[e % kMaxTop] : 0; },
+                            E.parts * kMaxTop, t, E.top);
   }
-  __syncthreads();
+  if (wave) return;
   bool has = false;
   float lx = 0.0f;
   if (E.labels && lane == 0) {
@@ -413,78 +575,120 @@ __global__ __launch_bounds__(64) void evidence_join_kernel(const Evidence E) {
     has = l >= 0 && l < E.classes;
     if (has) lx = to_float(((const T *)E.x)[o * E.s0 + i * E.s1 + l * E.cs]);
   }
-  store_row<ACT>(E, row, ref, log_s, h, has, lx, list, lane);
+  store_row<ACT>(E, row, ref, log_s, h, has, lx, L.list, lane);
 }
 
-template <typename T, int ACT, int KT>
-__global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) {
-  const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (row >= E.n0 * E.n1) return;
-  const long long o = row / E.n1, i = row - o * E.n1;
-  if (E.count && i >= E.count[o]) return;
-  const T *x = (const T *)E.x + o * E.s0 + i * E.s1;
-  Sums S = {-INFINITY, 0.0f, 0.0f};
-  unsigned ord[KT ? KT : 1];
-  int cls[KT ? KT : 1];
+// insertion into a descending list; equal values stay in class order
+template <int KT> __device__ __forceinline__ void insert(float (&val)[KT], int (&cls)[KT], float v, int c) {
+  bool up = false;   // from its place on, everything moves down by one
 #pragma unroll
-  for (int k = 0; k < KT; ++k) ord[k] = 0, cls[k] = -1;
+  for (int k = 0; k < KT; ++k) {
+    up = up || !(v <= val[k]);   // an empty place is NaN
+    const float a = val[k];
+    const int b = cls[k];
+    val[k] = up ? v : a;
+    cls[k] = up ? c : b;
+    v = up ? a : v;
+    c = up ? b : c;
+  }
+}
+
+// R rows side by side per thread, read as one word.  The lists are kept by float comparisons; a row that holds a NaN (or an
+// infinity that made one) is gone through again in the order that puts NaN first.
+template <typename T, int ACT, int KT, int R>
+__global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) {
+  const long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * R;
+  if (first >= E.n0 * E.n1) return;
+  const long long o = first / E.n1, i0 = first - o * E.n1;   // R divides n1: the rows share o
+  const T *x = (const T *)E.x + o * E.s0 + i0 * E.s1;
+  typedef typename Group<T, R>::type W;
+  Sums S[R];
+  constexpr int KL = KT ? KT : 1;
+  float val[R][KL];
+  int cls[R][KL];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    S[r] = Sums{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < KT; ++k) val[r][k] = NAN, cls[r][k] = -1;
+  }
   constexpr int U = 8;
   const int C = (int)E.classes;
   for (int c = 0; c < C; c += U) {
-    float v[U];
+    W w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      v[u] = c + u < C ? to_float(x[(long long)(c + u) * E.cs]) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
-    if (ACT == LMI_PROB_SOFTMAX) {
-      float mx = S.m;
+      if (c + u < C) w[u] = *(const W *)(x + (long long)(c + u) * E.cs);
 #pragma unroll
-      for (int u = 0; u < U; ++u) mx = fmaxf(mx, v[u]);
-      rebase(S, mx);
-      const float ref = finite_ref(mx);
+    for (int r = 0; r < R; ++r) {
+      float v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) add_value(S, ref, v[u]);
-    } else {
+      for (int u = 0; u < U; ++u) v[u] = c + u < C ? Group<T, R>::get(w[u], r) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
+      if (ACT == LMI_PROB_SOFTMAX) {
+        float mx = S[r].m;
 #pragma unroll
-      for (int u = 0; u < U; ++u) S.t += answer_entropy<ACT>(v[u]);
-    }
-    if (KT) {
+        for (int u = 0; u < U; ++u) mx = fmaxf(mx, v[u]);
+        rebase(S[r], mx);
+        const float ref = finite_ref(mx);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        unsigned q = c + u < C ? order_bits(v[u]) : 0u;
-        int qc = c + u;
-        if (q > ord[KT ? KT - 1 : 0]) {   // strictly better than the last kept one: equal values stay in class order
-          bool up = false;                // from its place on, everything moves down by one
+        for (int u = 0; u < U; ++u) add_value(S[r], ref, v[u]);
+      } else {
 #pragma unroll
-          for (int k = 0; k < KT; ++k) {
-            up = up || q > ord[k];
-            const unsigned a = ord[k];
-            const int b = cls[k];
-            ord[k] = up ? q : a;
-            cls[k] = up ? qc : b;
-            q = up ? a : q;
-            qc = up ? b : qc;
-          }
-        }
+        for (int u = 0; u < U; ++u) S[r].t += answer_entropy<ACT>(v[u]);
+      }
+      if (KT) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c + u < C && !(v[u] <= val[r][KL - 1])) insert<KL>(val[r], cls[r], v[u], c + u);
       }
     }
   }
-  float ref = 0.0f, log_s = 0.0f, h = S.t;
-  if (ACT == LMI_PROB_SOFTMAX) softmax_result(S, ref, log_s, h);
-  if (E.entropy) E.entropy[row] = h;
-  if (E.logprob) {
-    float lp = NAN;
-    if (E.labels) {
-      const long long l = label_of(E, o, i);
-      if (l >= 0 && l < C) lp = log_prob<ACT>(to_float(x[l * E.cs]), ref, log_s);
-    }
-    E.logprob[row] = lp;
-  }
 #pragma unroll
-  for (int k = 0; k < KT; ++k)
-    if (k < E.top) {
-      if (E.top_logprob) E.top_logprob[row * E.top + k] = log_prob<ACT>(order_value(ord[k]), ref, log_s);
-      if (E.top_index) E.top_index[row * E.top + k] = cls[k];
+  for (int r = 0; r < R; ++r) {
+    const long long row = first + r, i = i0 + r;
+    if (E.count && i >= E.count[o]) continue;
+    float ref = 0.0f, log_s = 0.0f, h = S[r].t;
+    if (ACT == LMI_PROB_SOFTMAX) softmax_result(S[r], ref, log_s, h);
+    if (E.entropy) E.entropy[row] = h;
+    if (E.logprob) {
+      float lp = NAN;
+      if (E.labels) {
+        const long long l = label_of(E, o, i);
+        if (l >= 0 && l < C) lp = log_prob<ACT>(to_float(x[r * E.s1 + l * E.cs]), ref, log_s);
+      }
+      E.logprob[row] = lp;
     }
+    if (KT && h != h) {   // first the NaNs by class, then the others
+      int n = 0;
+      for (int c = 0; c < C && n < E.top; ++c) {
+        const float v = to_float(x[r * E.s1 + (long long)c * E.cs]);
+        if (v != v) {
+          if (E.top_logprob) E.top_logprob[row * E.top + n] = NAN;
+          if (E.top_index) E.top_index[row * E.top + n] = c;
+          ++n;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < KT; ++k) val[r][k] = NAN, cls[r][k] = -1;
+      for (int c = 0; c < C; ++c) {
+        const float v = to_float(x[r * E.s1 + (long long)c * E.cs]);
+        if (v == v && !(v <= val[r][KL - 1])) insert<KL>(val[r], cls[r], v, c);
+      }
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+        if (n + k < E.top) {
+          if (E.top_logprob) E.top_logprob[row * E.top + n + k] = log_prob<ACT>(val[r][k], ref, log_s);
+          if (E.top_index) E.top_index[row * E.top + n + k] = cls[r][k];
+        }
+      continue;
+    }
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+      if (k < E.top) {
+        if (E.top_logprob) E.top_logprob[row * E.top + k] = log_prob<ACT>(val[r][k], ref, log_s);
+        if (E.top_index) E.top_index[row * E.top + k] = cls[r][k];
+      }
+  }
 }
 
 // parts per row: long rows of a batch too small to fill the chip are cut into parts of at least 4096 values, at most 64 (one
@@ -495,32 +699,49 @@ int split_parts(long long rows, long long classes) {
   return (int)(p < 64 ? p : 64);
 }
 
+template <typename T, int ACT, int KT> void launch_planes(const Evidence &E, hipStream_t st) {
+  const long long rows = E.n0 * E.n1;
+  if constexpr (sizeof(T) == 2 && KT <= 8) {   // two rows of a 16-bit type in one word
+    if (E.s1 == 1 && E.n1 % 2 == 0 && E.cs % 2 == 0 && E.s0 % 2 == 0 && lmi_is_aligned(E.x, 4)) {
+      evidence_planes_kernel<T, ACT, KT, 2><<<(unsigned)((rows / 2 + 255) / 256), 256, 0, st>>>(E);
+      return;
+    }
+  }
+  evidence_planes_kernel<T, ACT, KT, 1><<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(E);
+}
+
 template <typename T, int ACT> int launch(const Evidence &E0, hipStream_t st) {
   Evidence E = E0;
   const long long rows = E.n0 * E.n1;
   // rows side by side and few classes each, or many rows: a thread per row
   const bool planes = !E.index && E.classes <= 65536 && ((E.cs != 1 && E.s1 < E.cs && (rows >= 4096 || E.classes <= 64)) || E.classes <= 8);
   if (planes) {
-    const dim3 g((unsigned)((rows + 255) / 256));
-    if (E.top == 0) evidence_planes_kernel<T, ACT, 0><<<g, 256, 0, st>>>(E);
-    else if (E.top <= 2) evidence_planes_kernel<T, ACT, 2><<<g, 256, 0, st>>>(E);
-    else if (E.top <= 8) evidence_planes_kernel<T, ACT, 8><<<g, 256, 0, st>>>(E);
-    else evidence_planes_kernel<T, ACT, 32><<<g, 256, 0, st>>>(E);
+    if (E.top == 0) launch_planes<T, ACT, 0>(E, st);
+    else if (E.top <= 2) launch_planes<T, ACT, 2>(E, st);
+    else if (E.top <= 8) launch_planes<T, ACT, 8>(E, st);
+    else launch_planes<T, ACT, 32>(E, st);
+    return lmi_check_launch("lmi_class_logprobs");
+  }
+  if (E.classes <= 128) {
+    const unsigned g = (unsigned)((rows + 15) / 16);
+    if (E.classes <= 32) evidence_team_kernel<T, 2, ACT><<<g, 256, 0, st>>>(E, rows);
+    else evidence_team_kernel<T, 8, ACT><<<g, 256, 0, st>>>(E, rows);
     return lmi_check_launch("lmi_class_logprobs");
   }
   E.parts = split_parts(rows, E.classes);
   E.part_len = (E.classes + E.parts - 1) / E.parts;
-  const dim3 g((unsigned)(rows < (1 << 22) ? rows : (1 << 22)), (unsigned)E.parts);   // grid x workgroup size stays below 2^32
-  constexpr int V = 16 / sizeof(T);
+  const long long cap = 1 << 22;   // grid x workgroup size stays below 2^32
+  const dim3 g((unsigned)(rows < cap ? rows : cap), (unsigned)E.parts), g4((unsigned)((rows + 3) / 4 < cap ? (rows + 3) / 4 : cap), (unsigned)E.parts);
+  constexpr int V = 16 / sizeof(T);   // 128 bytes of a row per thread
   if (E.cs == 1) {
-    if (E.part_len <= 1024 - V) evidence_rows_kernel<T, 64, 16 / V, V, ACT><<<g, 64, 0, st>>>(E);
-    else if (E.part_len <= 8192 || E.parts > 1) evidence_rows_kernel<T, 256, 16 / V, V, ACT><<<g, 256, 0, st>>>(E);
-    else evidence_rows_kernel<T, 512, 32 / V, V, ACT><<<g, 512, 0, st>>>(E);
+    if (E.part_len <= 63 * 8 * V) evidence_rows_kernel<T, 64, 8, V, ACT><<<g4, 256, 0, st>>>(E);
+    else if (E.parts > 1) evidence_rows_kernel<T, 256, 8, V, ACT><<<g, 256, 0, st>>>(E);
+    else evidence_rows_kernel<T, 512, 8, V, ACT><<<g, 512, 0, st>>>(E);
   } else {
-    if (E.part_len <= 128) evidence_rows_kernel<T, 64, 2, 1, ACT><<<g, 64, 0, st>>>(E);
+    if (E.part_len <= 512) evidence_rows_kernel<T, 64, 8, 1, ACT><<<g4, 256, 0, st>>>(E);
     else evidence_rows_kernel<T, 256, 8, 1, ACT><<<g, 256, 0, st>>>(E);
   }
-  if (E.parts > 1) evidence_join_kernel<T, ACT><<<(unsigned)rows, 64, 0, st>>>(E);
+  if (E.parts > 1) evidence_join_kernel<T, ACT><<<(unsigned)rows, 256, 0, st>>>(E);
   return lmi_check_launch("lmi_class_logprobs");
 }
 

@@ -473,8 +473,10 @@ int64_t lmi_trace_contours_host(const uint64_t *words, int64_t m, const int32_t 
  * [0, classes) gives NaN.
  * Outputs [device], any of them NULL if not wanted, contiguous: logprob (n0,n1), entropy (n0,n1) fp32; top_logprob fp32 and
  * top_index int32 (n0,n1,top), best first, equal values in the order of their classes, NaN before everything else.
- * 0 <= top <= min(classes, LMI_MAX_TOP).  `workspace` [device] of lmi_class_logprobs_workspace_bytes (0: none needed).
+ * 0 <= top <= min(classes, LMI_MAX_TOP).  `workspace` [device] of lmi_class_logprobs_workspace_bytes; none is needed below
+ * LMI_LOGPROB_SPLIT_FROM classes or from 128 rows on.
  */
+#define LMI_LOGPROB_SPLIT_FROM 8193
 enum lmi_prob_activation { LMI_PROB_SOFTMAX = 0, LMI_PROB_SIGMOID = 1, LMI_PROB_NONE = 2 };
 typedef struct lmi_logprob_args {
   const void *x;
@@ -509,7 +511,8 @@ int lmi_class_logprobs(const lmi_logprob_args *args, void *stream);
  * lmi_mx_product: y[m][n] = act(sum_k Q(x)[m][k] * w[n][k] + bias[n]) with fp32 sums, Q = lmi_mx_quantize along k,
  *   w quantised.  The positions m are (batch, pixels).  layout LMI_MX_ROWS (a linear layer, channels-last maps): x
  *   element (b, p, k) at b*x_batch + p*x_stride + k, y contiguous (batch, pixels, n).  LMI_MX_PLANES (NCHW maps): x
- *   element at b*x_batch + k*x_stride + p, y contiguous (batch, n, pixels).
+ *   element at b*x_batch + k*x_stride + p, y contiguous (batch, n, pixels).  x_stride, and the pixels of a plane, stay
+ *   below 2^24.
  *   x_dtype LMI_MXFP4: x points at the packed blocks, x_scales at their scales (rows, batch 1, x_stride unused).
  *   y_dtype LMI_F32 | LMI_F16 | LMI_BF16, the type of x unless that is MXFP4.  bias [device] fp32 (n) or NULL.  workspace [device] of lmi_mx_product_workspace_bytes (0: none).
  *   This is a 1x1 convolution of the network with its folded batch norm (bias) and SiLU.

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch  # noqa: F401  -- must come first: the library has to bind to the HIP runtime torch ships and uses
 
@@ -51,6 +52,7 @@ class lmi_point_op(C.Structure):
 
 LMI_PROB_SOFTMAX, LMI_PROB_SIGMOID, LMI_PROB_NONE = 0, 1, 2
 LMI_MAX_TOP = 32
+LMI_LOGPROB_SPLIT_FROM = 8193
 
 
 class lmi_logprob_args(C.Structure):
@@ -61,6 +63,9 @@ class lmi_logprob_args(C.Structure):
                 ("entropy", C.c_void_p), ("top_logprob", C.c_void_p), ("top_index", C.c_void_p), ("workspace", C.c_void_p),
                 ("workspace_bytes", C.c_int64)]
 
+
+LOGPROB_ARGS = struct.Struct("<QiiqqqqqqQqQQqqiiQQQQQq")   # lmi_logprob_args, packed in one go (a ctypes structure costs a call several us)
+assert LOGPROB_ARGS.size == C.sizeof(lmi_logprob_args)
 
 LMI_MX_BLOCK = 32
 LMI_ACT_NONE, LMI_ACT_SILU = 0, 1
@@ -73,6 +78,9 @@ class lmi_mx_product_args(C.Structure):
                 ("w_packed", C.c_void_p), ("w_scales", C.c_void_p), ("bias", C.c_void_p), ("y", C.c_void_p), ("y_dtype", C.c_int32),
                 ("layout", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
+
+MX_PRODUCT_ARGS = struct.Struct("<QQiiqqqqqqQQQQiiQq")   # lmi_mx_product_args
+assert MX_PRODUCT_ARGS.size == C.sizeof(lmi_mx_product_args)
 
 LMI_POINT_DIV, LMI_POINT_SUB, LMI_POINT_FLIP_X, LMI_POINT_FLIP_Y, LMI_POINT_FLIP_XY = 1, 2, 3, 4, 5
 LMI_MAX_POINT_OPS = 16
@@ -140,11 +148,11 @@ SIGNATURES = {
     "lmi_trace_contours_host": (C.c_int64, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int64,
                                             C.c_void_p]),
     "lmi_class_logprobs_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int]),
-    "lmi_class_logprobs": (C.c_int, [C.POINTER(lmi_logprob_args), C.c_void_p]),
+    "lmi_class_logprobs": (C.c_int, [C.c_void_p, C.c_void_p]),
     "lmi_mx_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
     "lmi_mx_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_void_p]),
-    "lmi_mx_product_workspace_bytes": (C.c_int64, [C.POINTER(lmi_mx_product_args)]),
-    "lmi_mx_product": (C.c_int, [C.POINTER(lmi_mx_product_args), C.c_void_p]),
+    "lmi_mx_product_workspace_bytes": (C.c_int64, [C.c_void_p]),
+    "lmi_mx_product": (C.c_int, [C.c_void_p, C.c_void_p]),
     "lmi_revert_points_f32": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
     "lmi_revert_masks_stage": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),

@@ -694,7 +694,7 @@ __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) 
 // parts per row: long rows of a batch too small to fill the chip are cut into parts of at least 4096 values, at most 64 (one
 // per lane of the joining wave)
 int split_parts(long long rows, long long classes) {
-  if (rows >= 128 || classes <= 8192) return 1;
+  if (rows >= 128 || classes < LMI_LOGPROB_SPLIT_FROM) return 1;
   const long long p = (classes + 4095) / 4096;
   return (int)(p < 64 ? p : 64);
 }

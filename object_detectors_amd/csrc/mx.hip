@@ -11,9 +11,9 @@
 // Kernels
 //  mx_quantize_kernel     a wave takes 8 rows x 256 elements: four lanes per block, 8 elements each, four steps per lane.
 //  mx_dequantize_kernel   the same shape backwards.
-//  mx_product_kernel      64 positions x all of k: activations are read once, quantised in registers (a lane owns whole blocks: 32
-//                         channels of one position) and laid into LDS in the matrix instruction's order; then every wave
-//                         multiplies them with its share of the weight rows.
+//  mx_stream_kernel       the product of many positions: 128 of them x up to 320 weight rows per workgroup, streamed along k.
+//  mx_wave_planes_kernel  shallow 1x1 convolutions (k <= 128): a wave per 64 positions, everything in registers.
+//  mx_few_kernel          few positions (a single row, one image's deepest maps): the waves of a workgroup share k.
 #include <hip/hip_fp16.h>
 
 #include <type_traits>
@@ -167,15 +167,14 @@ struct Product {
   const unsigned *ws;
   const float *bias;
   void *y;
-  unsigned blocks;        // blocks of 32 along k
-  unsigned tiles_pixels;  // tiles of 64 positions per image
+  unsigned tiles_pixels;  // tiles of positions per image
   int tiles_n;            // tiles of 32 weight rows
-  int split_n;            // tiles of 32 weight rows per workgroup
+  int split_n;            // tiles of 32 weight rows per wave (mx_wave_planes_kernel)
   int all_steps;          // steps of 64 along k
-  int steps;              // steps that LDS holds (a multiple of 4, or all)
+  int vec;                // x allows wide loads: planes, two pixels; rows, 16 bytes
 };
 
-constexpr int kTile = 64;   // positions per workgroup
+constexpr int kTile = 64;   // positions of a wave
 
 template <int ACT> __device__ __forceinline__ float activate(float v) {
   // v_exp_f32 and v_rcp_f32, an ulp each: an IEEE division here made the results' arithmetic, not their bytes, the bound of shallow products
@@ -235,261 +234,11 @@ __device__ __forceinline__ int weight_lane(int lane) {
   return (lane & 32) + ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3);
 }
 
-// LDS: fragments [step][subtile][64] uint4, then scale words [step / 4][subtile][64]
-template <typename T, bool PLANES, bool VEC>
-__device__ __forceinline__ void fill(const Product &P, long long image, long long p0, int live, int s0, int ns, uint4 *frags, unsigned char *bytes) {
-  const int t = threadIdx.x;
-  auto put = [&](int kl, int px, const uint4 &f, unsigned byte) {
-    const int at = (px & 1) * 64 + (kl & 1) * 32 + (px >> 1), step = kl >> 1;
-    frags[step * 128 + at] = f;
-    bytes[((step >> 2) * 128 + at) * 4 + (step & 3)] = (unsigned char)byte;
-  };
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  if constexpr (__is_same(T, Packed)) {
-    const long long g0 = p0 >> 5;
-    for (int item = t; item < ns * 128; item += 256) {
-      const int step = item >> 7, at = item & 127, px = at & 63, half = at >> 6;   // px: row of the two groups
-      const long long g = g0 + (px >> 5);
-      uint4 f = zero;
-      if (px < live) f = ((const uint4 *)P.x)[((g * P.all_steps + s0 + step) * 2 + half) * 32 + (px & 31)];
-      frags[step * 128 + (px & 1) * 64 + half * 32 + (px >> 1)] = f;
-    }
-    const int quads = (P.all_steps + 3) / 4;
-    for (int item = t; item < (ns + 3) / 4 * 128; item += 256) {   // s0 is a multiple of 4
-      const int q = item >> 7, at = item & 127, px = at & 63, half = at >> 6;
-      const long long g = g0 + (px >> 5);
-      unsigned w = 0;
-      if (px < live) w = P.xs[((g * quads + s0 / 4 + q) * 2 + half) * 32 + (px & 31)];
-      ((unsigned *)bytes)[q * 128 + (px & 1) * 64 + half * 32 + (px >> 1)] = w;
-    }
-    return;
-  } else {
-    const T *x = (const T *)P.x + image * P.xb;
-    if constexpr (PLANES && VEC) {   // two neighbouring pixels per thread
-      for (int item = t; item < ns * 64; item += 256) {
-        const int pair = item & 31, kl = item >> 5;
-        const unsigned kb = 2 * s0 + kl;
-        uint4 f[2] = {zero, zero};
-        unsigned byte[2] = {0, 0};
-        if (2 * pair < live && kb < P.blocks) {
-          const T *q = x + p0 + 2 * pair + (long long)kb * 32 * P.xs1;
-          const int in = (int)(P.k - (long long)kb * 32 < 32 ? P.k - (long long)kb * 32 : 32);
-          if constexpr (sizeof(T) == 4) {
-            float a[32], b[32];
-#pragma unroll
-            for (int u = 0; u < 32; ++u) {
-              const float2 v = u < in ? *(const float2 *)(q + u * P.xs1) : make_float2(0.0f, 0.0f);
-              a[u] = v.x;
-              b[u] = v.y;
-            }
-            f[0] = quantize_block(a, byte[0]);
-            f[1] = quantize_block(b, byte[1]);
-          } else {
-            unsigned w[32];
-            if (in == 32) {
-#pragma unroll
-              for (int u = 0; u < 32; ++u) w[u] = *(const unsigned *)(q + u * P.xs1);
-            } else {
-#pragma unroll
-              for (int u = 0; u < 32; ++u) w[u] = u < in ? *(const unsigned *)(q + u * P.xs1) : 0u;
-            }
-            quantize_pair16<T>(w, f, byte);
-          }
-        }
-        put(kl, 2 * pair, f[0], byte[0]);
-        put(kl, 2 * pair + 1, f[1], byte[1]);
-      }
-    } else {
-      for (int item = t; item < ns * 128; item += 256) {
-        const int px = item & 63, kl = item >> 6;
-        const unsigned kb = 2 * s0 + kl;
-        uint4 f = zero;
-        unsigned byte = 0;
-        if (px < live && kb < P.blocks) {
-          const long long c0 = (long long)kb * 32;
-          float v[32];
-          if constexpr (PLANES) {
-            const T *q = x + p0 + px + c0 * P.xs1;
-#pragma unroll
-            for (int u = 0; u < 32; ++u) v[u] = c0 + u < P.k ? to_float(q[u * P.xs1]) : 0.0f;
-          } else {
-            const T *q = x + (p0 + px) * P.xs1 + c0;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              float e[8];
-              load8<T, VEC>(q + 8 * u, P.k - c0 - 8 * u, e);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[8 * u + j] = e[j];
-            }
-          }
-          f = quantize_block(v, byte);
-        }
-        put(kl, px, f, byte);
-      }
-    }
-  }
-}
-
 __device__ __forceinline__ v8i operand(const uint4 &a) { return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}; }
 
 template <int BYTE> __device__ __forceinline__ void mfma2(f16x (&acc)[2], const uint4 &a, unsigned sa, const uint4 &b0, const uint4 &b1, unsigned sb0, unsigned sb1) {
   acc[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b0), acc[0], 4, 4, BYTE, (int)sa, BYTE, (int)sb0);
   acc[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b1), acc[1], 4, 4, BYTE, (int)sa, BYTE, (int)sb1);
-}
-
-// One quad of steps of G weight tiles: fragments and scale words
-template <int G> struct Quad {
-  uint4 a[G][4];
-  unsigned s[G];
-};
-template <int G> __device__ __forceinline__ void load_quad(Quad<G> &Q, const uint4 *w, const unsigned *ws, long long tile_w, long long tile_s, int q, int last) {
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    Q.s[g] = ws[g * tile_s + q * 64];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) Q.a[g][i] = w[g * tile_w + (q * 4 + i < last ? q * 4 + i : last) * 64];   // beyond the last step: any of the tile's, not used
-  }
-}
-
-// Weight tiles nt .. nt + G - 1 times the ns steps in LDS (steps s0 ..), quads q0, q0 + dq, ...  The next quad's weights are on their way
-// while the matrix instructions run; every fragment read from LDS serves G of them.
-template <int G>
-__device__ __forceinline__ void multiply(const Product &P, int nt, int s0, int ns, int q0, int dq, const uint4 *frags, const unsigned *words, int lane, f16x (&acc)[G][2]) {
-  const int wl = weight_lane(lane), quads = (P.all_steps + 3) / 4;
-  const uint4 *w = P.w + ((long long)nt * P.all_steps + s0) * 64 + wl;
-  const unsigned *ws = P.ws + ((long long)nt * quads + s0 / 4) * 64 + wl;
-  const long long tile_w = (long long)P.all_steps * 64, tile_s = (long long)quads * 64;
-  if (q0 * 4 >= ns) return;
-  Quad<G> cur, next;
-  load_quad<G>(cur, w, ws, tile_w, tile_s, q0, ns - 1);
-  for (int q = q0; q * 4 < ns; q += dq) {
-    if ((q + dq) * 4 < ns) load_quad<G>(next, w, ws, tile_w, tile_s, q + dq, ns - 1);
-    const unsigned sb0 = words[q * 128 + lane], sb1 = words[q * 128 + 64 + lane];
-    const uint4 *f = frags + q * 512 + lane;
-    const int left = ns - q * 4;
-    {
-      const uint4 b0 = f[0], b1 = f[64];
-#pragma unroll
-      for (int g = 0; g < G; ++g) mfma2<0>(acc[g], cur.a[g][0], cur.s[g], b0, b1, sb0, sb1);
-    }
-    if (left > 1) {
-      const uint4 b0 = f[128], b1 = f[192];
-#pragma unroll
-      for (int g = 0; g < G; ++g) mfma2<1>(acc[g], cur.a[g][1], cur.s[g], b0, b1, sb0, sb1);
-    }
-    if (left > 2) {
-      const uint4 b0 = f[256], b1 = f[320];
-#pragma unroll
-      for (int g = 0; g < G; ++g) mfma2<2>(acc[g], cur.a[g][2], cur.s[g], b0, b1, sb0, sb1);
-    }
-    if (left > 3) {
-      const uint4 b0 = f[384], b1 = f[448];
-#pragma unroll
-      for (int g = 0; g < G; ++g) mfma2<3>(acc[g], cur.a[g][3], cur.s[g], b0, b1, sb0, sb1);
-    }
-    cur = next;
-  }
-}
-
-template <typename Y, bool PLANES, bool VEC, int ACT>
-__device__ __forceinline__ void store_tile(const Product &P, long long image, long long p0, int live, int nt, int lane, const f16x (&acc)[2]) {
-  Y *y = (Y *)P.y + image * P.pixels * P.n;
-  const int px = 2 * (lane & 31);
-  const long long n0 = (long long)nt * 32 + 16 * (lane >> 5);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const long long n = n0 + i;
-    if (n >= P.n) break;
-    const float b = P.bias ? P.bias[n] : 0.0f;
-    const Y v0 = (Y)activate<ACT>(acc[0][i] + b), v1 = (Y)activate<ACT>(acc[1][i] + b);
-    if constexpr (PLANES) {
-      Y *q = y + n * P.pixels + p0 + px;
-      if (VEC) {
-        typedef Y y2 __attribute__((ext_vector_type(2)));
-        if (px < live) *(y2 *)q = y2{v0, v1};
-      } else {
-        if (px < live) q[0] = v0;
-        if (px + 1 < live) q[1] = v1;
-      }
-    } else {
-      if (px < live) y[(p0 + px) * P.n + n] = v0;
-      if (px + 1 < live) y[(p0 + px + 1) * P.n + n] = v1;
-    }
-  }
-}
-
-// The weight tiles of a workgroup are dealt to its waves in runs of nearly equal length; which wave gets the longer ones turns with the
-// workgroup, so that no SIMD gets them all.  A wave takes its run two tiles at a time.  k longer than LDS holds: the positions are
-// quantised again for every round of tiles.
-// KSPLIT: one weight tile per workgroup, its waves share k (few positions).
-template <typename T, typename Y, bool PLANES, bool VEC, int ACT, bool KSPLIT>
-__global__ __launch_bounds__(256, KSPLIT ? 1 : 3) void mx_product_kernel(const Product P) {
-  extern __shared__ uint4 lds[];
-  uint4 *frags = lds;
-  unsigned char *bytes = (unsigned char *)(lds + (long long)P.steps * 128);
-  const unsigned *words = (const unsigned *)bytes;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long image = blockIdx.x / P.tiles_pixels;
-  const long long p0 = (long long)(blockIdx.x % P.tiles_pixels) * kTile;
-  const int live = (int)(P.pixels - p0 < kTile ? P.pixels - p0 : kTile);
-  const int nt0 = blockIdx.y * P.split_n;
-  const int nt1 = nt0 + P.split_n < P.tiles_n ? nt0 + P.split_n : P.tiles_n;
-  const bool once = P.all_steps <= P.steps;
-  if constexpr (KSPLIT) {
-    f16x acc[1][2] = {};
-    for (int s0 = 0; s0 < P.all_steps; s0 += P.steps) {
-      const int ns = P.all_steps - s0 < P.steps ? P.all_steps - s0 : P.steps;
-      __syncthreads();   // LDS is free again
-      fill<T, PLANES, VEC>(P, image, p0, live, s0, ns, frags, bytes);
-      __syncthreads();
-      multiply<1>(P, nt0, s0, ns, wave, 4, frags, words, lane, acc);
-    }
-    __syncthreads();   // sums of the four waves, in their order
-    float *part = (float *)lds;   // [3][32][64]
-    if (wave) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[((wave - 1) * 32 + h * 16 + i) * 64 + lane] = acc[0][h][i];
-    }
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-#pragma unroll
-          for (int w = 0; w < 3; ++w) acc[0][h][i] += part[(w * 32 + h * 16 + i) * 64 + lane];
-        }
-      store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt0, lane, acc[0]);
-    }
-  } else {
-    const int count = nt1 - nt0, turn = (wave + blockIdx.x) & 3;
-    const int mine = count / 4 + (turn < count % 4), first = nt0 + turn * (count / 4) + (turn < count % 4 ? turn : count % 4);
-    const int rounds = ((count + 3) / 4 + 1) / 2;   // of the longest run
-    for (int r = 0; r < rounds; ++r) {
-      const int nt = first + 2 * r, have = mine - 2 * r;
-      f16x acc[2][2] = {};
-      for (int s0 = 0; s0 < P.all_steps; s0 += P.steps) {
-        const int ns = P.all_steps - s0 < P.steps ? P.all_steps - s0 : P.steps;
-        if (!once || r == 0) {
-          __syncthreads();   // LDS is free again
-          fill<T, PLANES, VEC>(P, image, p0, live, s0, ns, frags, bytes);
-          __syncthreads();
-        }
-        if (have >= 2) {
-          multiply<2>(P, nt, s0, ns, 0, 1, frags, words, lane, acc);
-        } else if (have == 1) {
-          f16x one[1][2] = {{acc[0][0], acc[0][1]}};
-          multiply<1>(P, nt, s0, ns, 0, 1, frags, words, lane, one);
-          acc[0][0] = one[0][0];
-          acc[0][1] = one[0][1];
-        }
-      }
-      if (have >= 1) store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt, lane, acc[0]);
-      if (have >= 2) store_tile<Y, PLANES, VEC, ACT>(P, image, p0, live, nt + 1, lane, acc[1]);
-    }
-  }
 }
 
 // One wave, 64 positions, all of k (at most 128) in registers: what a lane quantises is its operand.  No LDS, no barrier: the waves of
@@ -518,9 +267,44 @@ template <typename T> __device__ __forceinline__ void load_planes(const T *base,
   if (live && in >= 32) {
 #pragma unroll
     for (int u = 0; u < 32; ++u) r.v[u] = *at<W>(base + u * stride, offset);
-  } else {   // positions beyond the image, the last channels
+  } else if (live && in > 0) {   // the last channels: all loads at once, those beyond read the first again
 #pragma unroll
-    for (int u = 0; u < 32; ++u) r.v[u] = live && u < in ? *at<W>(base + u * stride, offset) : W{};
+    for (int u = 0; u < 32; ++u) r.v[u] = *at<W>(base + (u < in ? u * stride : 0), offset);
+#pragma unroll
+    for (int u = 0; u < 32; ++u) r.v[u] = u < in ? r.v[u] : W{};
+  } else {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) r.v[u] = W{};
+  }
+}
+// the same value by value; `live` of the two pixels are there
+template <typename T> __device__ __forceinline__ void load_planes_single(const T *base, unsigned offset, long long stride, int live, int in, Raw<T, true> &r) {
+  auto put = [&](int u, T a, T b) {
+    if constexpr (sizeof(T) == 4) r.v[u] = make_float2(a, b);
+    else r.v[u] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
+  };
+  const unsigned next = offset + (live > 1 ? sizeof(T) : 0);   // what is not there reads a neighbour that is
+  if (live > 0 && in >= 32) {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) put(u, *at<T>(base + u * stride, offset), *at<T>(base + u * stride, next));
+    if (live == 1) {
+#pragma unroll
+      for (int u = 0; u < 32; ++u) {
+        if constexpr (sizeof(T) == 4) r.v[u].y = 0.0f;
+        else r.v[u] &= 0xffffu;
+      }
+    }
+  } else if (live > 0 && in > 0) {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) put(u, *at<T>(base + (u < in ? u * stride : 0), offset), *at<T>(base + (u < in ? u * stride : 0), next));
+#pragma unroll
+    for (int u = 0; u < 32; ++u) {
+      if constexpr (sizeof(T) == 4) r.v[u] = make_float2(u < in ? r.v[u].x : 0.0f, u < in && live > 1 ? r.v[u].y : 0.0f);
+      else r.v[u] = u < in ? (live > 1 ? r.v[u] : r.v[u] & 0xffffu) : 0u;
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 32; ++u) put(u, (T)0.0f, (T)0.0f);
   }
 }
 __device__ __forceinline__ void quantize_raw(const Raw<float, true> &r, uint4 (&f)[2], unsigned (&byte)[2]) {
@@ -548,7 +332,7 @@ __device__ __forceinline__ void start_sums(const Product &P, int nt, int lane, f
 // planes: a lane holds 16 weight rows' results of two neighbouring positions.  Results are not read again soon: stored past the caches
 // (the 160 x 160 maps of a batch of 64, 48 -> 32 channels: 75 -> 56 us with the sums starting at the bias).
 template <typename Y>
-__device__ __forceinline__ void store_planes(const Product &P, Y *y, long long p0, int live, int nt, int lane, int act, const f16x (&acc)[2]) {
+__device__ __forceinline__ void store_planes(const Product &P, Y *y, long long p0, int live, int nt, int lane, int act, bool vec, const f16x (&acc)[2]) {
   const int px = 2 * (lane & 31), n0 = 16 * (lane >> 5);
   const long long left = P.n - nt * 32ll - n0;
   const unsigned offset = (unsigned)(n0 * P.pixels + px) * sizeof(Y);
@@ -561,7 +345,13 @@ __device__ __forceinline__ void store_planes(const Product &P, Y *y, long long p
       v1 = activate<LMI_ACT_SILU>(v1);
     }
     typedef Y y2 __attribute__((ext_vector_type(2)));
-    if (px < live && i < left) __builtin_nontemporal_store(y2{(Y)v0, (Y)v1}, (y2 *)((char *)(base + i * P.pixels) + offset));
+    if (vec) {
+      if (px < live && i < left) __builtin_nontemporal_store(y2{(Y)v0, (Y)v1}, (y2 *)((char *)(base + i * P.pixels) + offset));
+    } else if (i < left) {
+      Y *q = base + (n0 + i) * P.pixels + px;
+      if (px < live) q[0] = (Y)v0;
+      if (px + 1 < live) q[1] = (Y)v1;
+    }
   }
 }
 
@@ -638,18 +428,17 @@ __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P,
     for (int s = 0; s < kWaveSteps; ++s) a[s] = w[(s < S ? s : S - 1) * 64];
     mfma2<0>(acc, a[0], sa, f[0][0], f[0][1], sw[0], sw[1]);
     if (S > 1) mfma2<1>(acc, a[1], sa, f[1][0], f[1][1], sw[0], sw[1]);
-    store_planes<T>(P, y, p0, live, nt, lane, act, acc);
+    store_planes<T>(P, y, p0, live, nt, lane, act, true, acc);
   }
 }
 
-template <typename T> bool launch_wave_planes(Product P, int act, long long batch, hipStream_t st) {
+template <typename T> void launch_wave_planes(Product P, int act, long long batch, hipStream_t st) {
+  P.tiles_pixels = (unsigned)((P.pixels + kTile - 1) / kTile);
   const long long tiles = batch * P.tiles_pixels;
-  if (P.all_steps > kWaveSteps || tiles < 512) return false;
   const long long split = tiles < 2048 ? (2048 + tiles - 1) / tiles : 1;
   P.split_n = (int)((P.tiles_n + split - 1) / split);
   const dim3 grid((unsigned)((tiles + 3) / 4), (unsigned)((P.tiles_n + P.split_n - 1) / P.split_n));
   mx_wave_planes_kernel<T><<<grid, 256, 0, st>>>(P, act, tiles);
-  return true;
 }
 
 // Streaming product: 128 positions x up to 64 * NT weight rows per workgroup, k in chunks of two steps.  While the matrix instructions run
@@ -664,8 +453,10 @@ template <typename T> struct Chunk<T, true> {
   Raw<T, true> raw;
   __device__ __forceinline__ void load(const Product &P, const T *x, int live, int chunk) {
     const int pair = threadIdx.x & 63;
-    const long long c0 = (4ll * chunk + wave_id()) * 32;
-    load_planes<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, 2 * pair < live, c0 < P.k ? (int)(P.k - c0 < 32 ? P.k - c0 : 32) : 0, raw);
+    const long long c0 = (4ll * chunk + wave_id()) * 32;   // beyond k: in = 0
+    const int in = c0 < P.k ? (int)(P.k - c0 < 32 ? P.k - c0 : 32) : 0;
+    if (P.vec) load_planes<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, 2 * pair < live, in, raw);
+    else load_planes_single<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, live - 2 * pair, in, raw);
   }
   __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) const {
     const int pair = threadIdx.x & 63, kl = wave_id();
@@ -693,11 +484,16 @@ template <typename T> struct Chunk<T, false> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const T *q = base + i * 16 * P.xs1;
-      if (row + 16 * i < live && n >= 8) {
+      if (P.vec && row + 16 * i < live && n >= 8) {
         v[i] = *at<piece>(q, offset);
-      } else {
+      } else if (row + 16 * i < live && n > 0) {   // value by value: those beyond the row read its last again
+        const T *single = x + (row + 16 * i) * P.xs1 + chunk * 128ll + (t & 15) * 8;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[i][u] = row + 16 * i < live && u < n ? *at<T>(q, offset + u * sizeof(T)) : (T)0.0f;
+        for (int u = 0; u < 8; ++u) v[i][u] = single[u < n ? u : n - 1];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[i][u] = u < n ? v[i][u] : (T)0.0f;
+      } else {
+        v[i] = piece{};
       }
     }
   }
@@ -732,7 +528,7 @@ template <int SIZE> __device__ __forceinline__ void to_lds(const void *src, void
 }
 
 template <typename T, typename Y, bool PLANES, int NT>
-__global__ __launch_bounds__(256, NT <= 2 ? 3 : 2) void mx_stream_kernel(const Product P, int act, int splits, long long tiles, int vec_y) {
+__global__ __launch_bounds__(256, NT <= 2 && (PLANES || sizeof(Y) == 2) ? 3 : 2) void mx_stream_kernel(const Product P, int act, int splits, long long tiles, int vec_y) {
   __shared__ uint4 xb[2][2][4][64];
   __shared__ unsigned xs[2][4][64];
   __shared__ uint4 wb[2][2][2 * NT][64];
@@ -835,13 +631,13 @@ __global__ __launch_bounds__(256, NT <= 2 ? 3 : 2) void mx_stream_kernel(const P
   for (int t = 0; t < NT; ++t) {
     const int nt = nt0 + wn * NT + t;
     if (nt < P.tiles_n) {
-      if constexpr (PLANES) store_planes<Y>(P, y, p0 + 64 * wp, live_w, nt, lane, act, acc[t]);
+      if constexpr (PLANES) store_planes<Y>(P, y, p0 + 64 * wp, live_w, nt, lane, act, P.vec, acc[t]);
       else store_rows<Y>(P, y, p0 + 64 * wp, live_w, nt, lane, act, vec_y, acc[t]);
     }
   }
 }
 
-template <typename T, typename Y, bool PLANES> bool launch_stream(Product P, int act, long long batch, hipStream_t st) {
+template <typename T, typename Y, bool PLANES> void launch_stream(Product P, int act, long long batch, hipStream_t st) {
   P.tiles_pixels = (unsigned)((P.pixels + kChunkTile - 1) / kChunkTile);
   const long long tiles = batch * P.tiles_pixels;
   constexpr int kMaxNT = sizeof(Y) == 4 && !__is_same(T, Packed) ? 4 : 5;
@@ -856,49 +652,134 @@ template <typename T, typename Y, bool PLANES> bool launch_stream(Product P, int
   else if (nt == 3) mx_stream_kernel<T, Y, PLANES, 3><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
   else if (nt == 4) mx_stream_kernel<T, Y, PLANES, 4><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
   else mx_stream_kernel<T, Y, PLANES, kMaxNT><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
-  return true;
 }
 
-constexpr int kMaxSteps = 28;   // 59.5 KB of LDS
-size_t lds_bytes(int steps) { return (size_t)steps * 2048 + (size_t)((steps + 3) / 4) * 512; }
+// Few positions: 64 of them x 32 weight rows per workgroup, its eight waves share k.  A wave loads its steps' blocks straight into the
+// operands -- no LDS, no barrier before the sums meet; a workgroup's time is the latency of a load or two.
+constexpr int kFewWaves = 8;
+// up to this many pairs of tiles (about a thousand: 4 x 320 -> 320 on 40 x 40, 100 x 10 of them, 11.3 us here and 11.7 streamed; 16 x 640 -> 640
+// on 20 x 20, 112 x 20, 31 and 21); quantised rows stream sooner (1024 x 1280 x 1280, 16 x 40: 10.7 and 7.6)
+constexpr long long kFewTiles = 1024, kFewTilesPacked = 320;
 
-template <typename T, typename Y, bool PLANES, bool VEC, int ACT> int launch_product(Product P, long long batch, hipStream_t st) {
-  P.steps = P.all_steps < kMaxSteps ? P.all_steps : kMaxSteps;
-  const long long tiles = batch * P.tiles_pixels;
-  // few positions: the weight rows are split over workgroups too, until there are about two per CU
-  long long split = 1;
-  if (tiles < 512) split = (512 + tiles - 1) / tiles;
-  P.split_n = (int)((P.tiles_n + split - 1) / split);
-  const dim3 grid((unsigned)tiles, (unsigned)((P.tiles_n + P.split_n - 1) / P.split_n));
-  const size_t lds = lds_bytes(P.steps);
-  if (P.split_n == 1) {
-    const size_t parts = 3 * 32 * 64 * 4;
-    mx_product_kernel<T, Y, PLANES, VEC, ACT, true><<<grid, 256, lds > parts ? lds : parts, st>>>(P);
-  } else {
-    mx_product_kernel<T, Y, PLANES, VEC, ACT, false><<<grid, 256, lds, st>>>(P);
-  }
-  return lmi_check_launch("lmi_mx_product");
-}
-
-template <typename T, typename Y, bool PLANES> int launch_act(const Product &P, int act, long long batch, hipStream_t st) {
-  constexpr long long kStreamFrom = 4096;
+// blocks kb = 2 * step + (lane >> 5) of the lane's two positions
+template <typename T, bool PLANES>
+__device__ __forceinline__ void load_few(const Product &P, const T *x, long long p0, int live, int step, int lane, uint4 (&f)[2], unsigned (&byte)[2]) {
+  const int j = lane & 31;
   if constexpr (__is_same(T, Packed)) {
-    if (batch * P.pixels >= kStreamFrom && launch_stream<T, Y, false>(P, act, batch, st)) return lmi_check_launch("lmi_mx_product");
-  }
-  // planes: two pixels of a channel in one load, and of a result in one store; rows: 16-byte loads
-  const uintptr_t align = PLANES ? 2 * sizeof(Y) : 16;
-  bool vec = false;
-  if constexpr (!__is_same(T, Packed)) {
-    vec = P.xs1 < (1 << 24) && P.pixels < (1 << 24) && (uintptr_t)P.x % align == 0 && P.xb * sizeof(Y) % align == 0 && P.xs1 * sizeof(Y) % align == 0;
-    if (PLANES) vec = vec && P.pixels % 2 == 0 && (uintptr_t)P.y % align == 0;
-    if constexpr (PLANES) {
-      if (vec && launch_wave_planes<T>(P, act, batch, st)) return lmi_check_launch("lmi_mx_product");
+    const int quads = (P.all_steps + 3) / 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long group = (p0 >> 5) + h;
+      const bool in = 32 * h < live;   // rows of the last group that lie beyond are zeros
+      f[h] = in ? ((const uint4 *)P.x)[(group * P.all_steps + step) * 64 + lane] : make_uint4(0, 0, 0, 0);
+      byte[h] = in ? (P.xs[(group * quads + step / 4) * 64 + lane] >> (8 * (step & 3))) & 255u : 0u;
     }
-    if (vec && batch * P.pixels >= kStreamFrom && launch_stream<T, Y, PLANES>(P, act, batch, st)) return lmi_check_launch("lmi_mx_product");
-    if (vec)
-      return act == LMI_ACT_SILU ? launch_product<T, Y, PLANES, true, LMI_ACT_SILU>(P, batch, st) : launch_product<T, Y, PLANES, true, LMI_ACT_NONE>(P, batch, st);
+  } else {
+    const long long c0 = step * 64ll + (lane >> 5) * 32;
+    const int in = (int)(P.k - c0 < 0 ? 0 : P.k - c0 < 32 ? P.k - c0 : 32);
+    if constexpr (PLANES) {
+      if (P.vec) {
+        Raw<T, true> raw;
+        load_planes<T>(x + step * 64ll * P.xs1, (unsigned)((lane >> 5) * 32 * P.xs1 + 2 * j) * sizeof(T), P.xs1, 2 * j < live, in, raw);
+        quantize_raw(raw, f, byte);
+        return;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int px = 32 * h + j;
+      const long long stride = PLANES ? P.xs1 : 1;
+      const T *base = x + step * 64ll * stride;
+      const unsigned offset = (unsigned)((lane >> 5) * 32 * stride + px * (PLANES ? 1 : P.xs1)) * sizeof(T);
+      const T *q = at<T>(base, offset);
+      float v[32];
+      if (!PLANES && P.vec && px < live && in == 32) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float e[8];
+          load8<T, true>(q + 8 * u, 8, e);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[8 * u + i] = e[i];
+        }
+      } else if (px < live && in == 32) {
+#pragma unroll
+        for (int u = 0; u < 32; ++u) v[u] = to_float(*at<T>(base + u * stride, offset));
+      } else if (px < live && in > 0) {   // all loads at once: channels beyond the last read the first again
+#pragma unroll
+        for (int u = 0; u < 32; ++u) v[u] = to_float(*at<T>(base + (u < in ? u * stride : 0), offset));
+#pragma unroll
+        for (int u = 0; u < 32; ++u) v[u] = u < in ? v[u] : 0.0f;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 32; ++u) v[u] = 0.0f;
+      }
+      f[h] = quantize_block(v, byte[h]);
+    }
   }
-  return act == LMI_ACT_SILU ? launch_product<T, Y, PLANES, false, LMI_ACT_SILU>(P, batch, st) : launch_product<T, Y, PLANES, false, LMI_ACT_NONE>(P, batch, st);
+}
+
+template <typename T, typename Y, bool PLANES>
+__global__ __launch_bounds__(64 * kFewWaves, 4) void mx_few_kernel(const Product P, int act) {
+  __shared__ float part[kFewWaves][32][64];
+  const int lane = threadIdx.x & 63, wave = wave_id(), S = P.all_steps, quads = (S + 3) / 4;
+  const long long image = blockIdx.x / P.tiles_pixels;
+  const long long p0 = (long long)(blockIdx.x % P.tiles_pixels) * kTile;
+  const int live = (int)(P.pixels - p0 < kTile ? P.pixels - p0 : kTile);
+  const int nt = blockIdx.y, wl = weight_lane(lane);
+  const uint4 *w = P.w + (long long)nt * S * 64 + wl;
+  const unsigned *ws = P.ws + (long long)nt * quads * 64 + wl;
+  f16x acc[2] = {};
+  for (int s = wave; s < S; s += kFewWaves) {
+    const uint4 a = w[s * 64ll];
+    const unsigned sa = ws[(s >> 2) * 64ll] >> (8 * (s & 3));
+    uint4 f[2];
+    unsigned byte[2];
+    if constexpr (__is_same(T, Packed)) load_few<T, PLANES>(P, nullptr, p0, live, s, lane, f, byte);
+    else load_few<T, PLANES>(P, (const T *)P.x + image * P.xb + (PLANES ? p0 : p0 * P.xs1), p0, live, s, lane, f, byte);
+    mfma2<0>(acc, a, sa, f[0], f[1], byte[0], byte[1]);
+  }
+  const int waves = S < kFewWaves ? S : kFewWaves;
+  if (wave < waves) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) part[wave][i][lane] = acc[i >> 4][i & 15];
+  }
+  __syncthreads();
+  Y *y = (Y *)P.y + image * P.pixels * P.n;
+#pragma unroll
+  for (int r = 0; r < 2048 / (64 * kFewWaves); ++r) {   // sums of the waves, in their order
+    const int i = r * kFewWaves + wave;
+    const int px = PLANES && P.vec ? 2 * (lane & 31) + (i >> 4) : 32 * (i >> 4) + (lane & 31);
+    const long long n = nt * 32ll + 16 * (lane >> 5) + (i & 15);
+    float v = 0.0f;
+    for (int q = 0; q < waves; ++q) v += part[q][i][lane];
+    if (px < live && n < P.n) {
+      v += P.bias ? P.bias[n] : 0.0f;
+      if (act) v = activate<LMI_ACT_SILU>(v);
+      y[PLANES ? n * P.pixels + p0 + px : (p0 + px) * P.n + n] = (Y)v;
+    }
+  }
+}
+
+template <typename T, typename Y, bool PLANES> int launch_product(Product P, int act, long long batch, hipStream_t st) {
+  if constexpr (!__is_same(T, Packed)) {
+    const uintptr_t align = PLANES ? 2 * sizeof(T) : 16;
+    P.vec = (uintptr_t)P.x % align == 0 && P.xb * sizeof(T) % align == 0 && P.xs1 * sizeof(T) % align == 0;
+    if (PLANES) P.vec = P.vec && P.pixels % 2 == 0 && (uintptr_t)P.y % align == 0;
+  }
+  P.tiles_pixels = (unsigned)((P.pixels + kTile - 1) / kTile);
+  const long long tiles = batch * P.tiles_pixels;
+  if (tiles * P.tiles_n <= (__is_same(T, Packed) ? kFewTilesPacked : kFewTiles)) {
+    mx_few_kernel<T, Y, PLANES><<<dim3((unsigned)tiles, (unsigned)P.tiles_n), 64 * kFewWaves, 0, st>>>(P, act);
+    return lmi_check_launch("lmi_mx_product");
+  }
+  if constexpr (PLANES) {
+    if (P.vec && P.all_steps <= kWaveSteps && tiles >= 512) {
+      launch_wave_planes<T>(P, act, batch, st);
+      return lmi_check_launch("lmi_mx_product");
+    }
+  }
+  launch_stream<T, Y, PLANES>(P, act, batch, st);
+  return lmi_check_launch("lmi_mx_product");
 }
 
 bool float_type(int d) { return d == LMI_F32 || d == LMI_F16 || d == LMI_BF16; }
@@ -979,6 +860,8 @@ int lmi_mx_product(const lmi_mx_product_args *a, void *stream) {
   LMI_REQUIRE(a->layout == LMI_MX_ROWS || a->layout == LMI_MX_PLANES, LMI_ERR_BAD_ARG, "lmi_mx_product: unknown layout %d", a->layout);
   const bool rows = a->layout == LMI_MX_ROWS;
   LMI_REQUIRE(a->x_batch >= 0 && a->x_stride >= 0, LMI_ERR_BAD_ARG, "lmi_mx_product: negative stride");
+  LMI_REQUIRE(a->x_stride < (1 << 24) && (rows || a->pixels < (1 << 24)), LMI_ERR_LIMIT,
+              "lmi_mx_product: rows or channels must lie less than 2^24 elements apart, and a plane hold fewer");
   LMI_REQUIRE(lmi_is_aligned(a->w_packed, 16) && lmi_is_aligned(a->w_scales, 4), LMI_ERR_ALIGNMENT,
               "lmi_mx_product: w_packed must be 16-byte, w_scales 4-byte aligned");
   Product P = {};
@@ -996,26 +879,24 @@ int lmi_mx_product(const lmi_mx_product_args *a, void *stream) {
   const int64_t blocks = (a->k + LMI_MX_BLOCK - 1) / LMI_MX_BLOCK, tiles_n = (a->n + 31) / 32, tiles_p = (a->pixels + kTile - 1) / kTile;
   LMI_REQUIRE(blocks < (1 << 24) && tiles_n < (1 << 24) && tiles_p < (1 << 24) && a->batch < (1 << 24) && tiles_p * a->batch < (1 << 24), LMI_ERR_LIMIT,
               "lmi_mx_product: k, n or the number of positions is too large");
-  P.blocks = (unsigned)blocks;
   P.all_steps = (int)((blocks + 1) / 2);
   P.tiles_n = (int)tiles_n;
-  P.tiles_pixels = (unsigned)tiles_p;
   hipStream_t st = (hipStream_t)stream;
   if (a->x_dtype == LMI_MXFP4) {
     LMI_REQUIRE(rows && a->batch == 1 && a->x_scales && lmi_is_aligned(a->x, 16) && lmi_is_aligned(a->x_scales, 4), LMI_ERR_BAD_ARG,
                 "lmi_mx_product: quantised x comes as 16-byte aligned rows with their scales, batch 1");
-    if (a->y_dtype == LMI_F32) return launch_act<Packed, float, false>(P, a->act, 1, st);
-    if (a->y_dtype == LMI_F16) return launch_act<Packed, _Float16, false>(P, a->act, 1, st);
-    return launch_act<Packed, __bf16, false>(P, a->act, 1, st);
+    if (a->y_dtype == LMI_F32) return launch_product<Packed, float, false>(P, a->act, 1, st);
+    if (a->y_dtype == LMI_F16) return launch_product<Packed, _Float16, false>(P, a->act, 1, st);
+    return launch_product<Packed, __bf16, false>(P, a->act, 1, st);
   }
   if (rows) {
-    if (a->x_dtype == LMI_F32) return launch_act<float, float, false>(P, a->act, a->batch, st);
-    if (a->x_dtype == LMI_F16) return launch_act<_Float16, _Float16, false>(P, a->act, a->batch, st);
-    return launch_act<__bf16, __bf16, false>(P, a->act, a->batch, st);
+    if (a->x_dtype == LMI_F32) return launch_product<float, float, false>(P, a->act, a->batch, st);
+    if (a->x_dtype == LMI_F16) return launch_product<_Float16, _Float16, false>(P, a->act, a->batch, st);
+    return launch_product<__bf16, __bf16, false>(P, a->act, a->batch, st);
   }
-  if (a->x_dtype == LMI_F32) return launch_act<float, float, true>(P, a->act, a->batch, st);
-  if (a->x_dtype == LMI_F16) return launch_act<_Float16, _Float16, true>(P, a->act, a->batch, st);
-  return launch_act<__bf16, __bf16, true>(P, a->act, a->batch, st);
+  if (a->x_dtype == LMI_F32) return launch_product<float, float, true>(P, a->act, a->batch, st);
+  if (a->x_dtype == LMI_F16) return launch_product<_Float16, _Float16, true>(P, a->act, a->batch, st);
+  return launch_product<__bf16, __bf16, true>(P, a->act, a->batch, st);
 }
 
 }  // extern "C"

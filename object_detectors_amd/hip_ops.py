@@ -6,7 +6,6 @@ unless they say so.  There is no CPU fallback: tensors must live on a HIP device
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import functools
 import math
@@ -709,12 +708,18 @@ def paste_masks(masks: torch.Tensor, boxes: torch.Tensor, image_shape: Tuple[int
 
 
 _FLOAT_DTYPES = {torch.float32: LMI_F32, torch.float16: LMI_F16, torch.bfloat16: _lib.LMI_BF16}
-_NO_GUARD = contextlib.nullcontext()
 
 
-def _on(device: torch.device):
-    """Makes `device` the current one for a launch (nothing to do in the usual case)."""
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _launch(entry, args, device: torch.device, *more) -> None:
+    """entry(args, *more, stream) on the current stream of `device`, which is made the current device for it if it is not."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = entry(args, *more, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(args, *more, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status)
 
 
 def _no_gradient(what: str, *tensors) -> None:
@@ -827,18 +832,17 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
             if not labels.is_contiguous():
                 labels = labels.contiguous()
             l0, l1 = n1, 1
-    a = _lib.lmi_logprob_args(
-        x.data_ptr(), _FLOAT_DTYPES[x.dtype], act, c, cs, n0, n1, s0, s1, None if index is None else index.data_ptr(),
-        0 if index is None else x.shape[1], None if count is None else count.data_ptr(), None if labels is None else labels.data_ptr(), l0, l1,
-        0 if labels is None else _LABEL_DTYPES[labels.dtype], top, out["logprob"].data_ptr() if labels is not None else None,
-        out["entropy"].data_ptr(), out["top_logprob"].data_ptr() if top else None, out["top_index"].data_ptr() if top else None, None, 0)
-    need = int(_L.lmi_class_logprobs_workspace_bytes(n0 * n1, c, cs, top))
-    ws = None
-    if need:   # not from the shared cache: two captured graphs that run side by side must not share it
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    with _on(dev):
-        check(_L.lmi_class_logprobs(C.byref(a), _stream(dev)))
+    workspace, need = None, 0
+    if c >= _lib.LMI_LOGPROB_SPLIT_FROM:
+        need = int(_L.lmi_class_logprobs_workspace_bytes(n0 * n1, c, cs, top))
+        if need:   # not from the shared cache: two captured graphs that run side by side must not share it
+            workspace = torch.empty((need,), dtype=torch.uint8, device=dev)
+    args = _lib.LOGPROB_ARGS.pack(
+        x.data_ptr(), _FLOAT_DTYPES[x.dtype], act, c, cs, n0, n1, s0, s1, 0 if index is None else index.data_ptr(),
+        0 if index is None else x.shape[1], 0 if count is None else count.data_ptr(), 0 if labels is None else labels.data_ptr(), l0, l1,
+        0 if labels is None else _LABEL_DTYPES[labels.dtype], top, 0 if labels is None else out["logprob"].data_ptr(), out["entropy"].data_ptr(),
+        out["top_logprob"].data_ptr() if top else 0, out["top_index"].data_ptr() if top else 0, workspace.data_ptr() if need else 0, need)
+    _launch(_L.lmi_class_logprobs, args, dev)
     return out
 
 
@@ -901,8 +905,7 @@ def mx_quantize(x: torch.Tensor) -> MxTensor:
     packed, scales = (torch.empty(s, dtype=torch.uint8, device=dev) for s in _mx_sizes(shape))
     if rows:
         x, _, stride = _rows_of(x)
-        with _on(dev):
-            check(_L.lmi_mx_quantize(x.data_ptr(), _FLOAT_DTYPES[x.dtype], rows, k, stride, packed.data_ptr(), scales.data_ptr(), _stream(dev)))
+        _launch(_L.lmi_mx_quantize, x.data_ptr(), dev, _FLOAT_DTYPES[x.dtype], rows, k, stride, packed.data_ptr(), scales.data_ptr())
     return MxTensor(packed, scales, shape)
 
 
@@ -919,9 +922,8 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
         raise TypeError("mx_dequantize: dtype must be float32, float16 or bfloat16")
     y = torch.empty(q.shape, dtype=dtype, device=q.device)
     if y.numel():
-        with _on(q.device):
-            check(_L.lmi_mx_dequantize(q.packed.data_ptr(), q.scales.data_ptr(), math.prod(q.shape[:-1]), q.shape[-1], y.data_ptr(),
-                                       _FLOAT_DTYPES[dtype], _stream(q.device)))
+        _launch(_L.lmi_mx_dequantize, q.packed.data_ptr(), q.device, q.scales.data_ptr(), math.prod(q.shape[:-1]), q.shape[-1], y.data_ptr(),
+                _FLOAT_DTYPES[dtype])
     return y
 
 
@@ -935,16 +937,15 @@ def _mx_product(what, x_ptr, x_scales, x_dtype, batch, pixels, k, x_batch, x_str
         raise ValueError(f"{what}: bias must be a contiguous float32 tensor ({weight.shape[0]},) on x's device")
     if y.numel() == 0:
         return y
-    a = _lib.lmi_mx_product_args(x_ptr, x_scales, x_dtype, _MX_ACTS[act], batch, pixels, k, weight.shape[0], x_batch, x_stride,
-                                 weight.packed.data_ptr(), weight.scales.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
-                                 _FLOAT_DTYPES[y.dtype], layout, None, 0)
-    need = int(_L.lmi_mx_product_workspace_bytes(C.byref(a)))
-    ws = None
+    fields = [x_ptr, x_scales or 0, x_dtype, _MX_ACTS[act], batch, pixels, k, weight.shape[0], x_batch, x_stride, weight.packed.data_ptr(),
+              weight.scales.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(), _FLOAT_DTYPES[y.dtype], layout, 0, 0]
+    args = _lib.MX_PRODUCT_ARGS.pack(*fields)
+    need = int(_L.lmi_mx_product_workspace_bytes(args))
     if need:   # not from the shared cache: two captured graphs that run side by side must not share it
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    with _on(dev):
-        check(_L.lmi_mx_product(C.byref(a), _stream(dev)))
+        workspace = torch.empty((need,), dtype=torch.uint8, device=dev)
+        fields[-2:] = workspace.data_ptr(), need
+        args = _lib.MX_PRODUCT_ARGS.pack(*fields)
+    _launch(_L.lmi_mx_product, args, dev)
     return y
 
 
@@ -985,7 +986,7 @@ def mx_linear(x: Union[torch.Tensor, MxTensor], weight: MxTensor, bias: Optional
         if dtype not in (None, x.dtype):
             raise ValueError("mx_linear: the result has x's dtype unless x is an MxTensor")
         dtype = x.dtype
-    if len(x.shape) < 1:
+    if not len(x.shape):
         raise ValueError("mx_linear: x must be (..., k)")
     k = x.shape[-1]
     _mx_common("mx_linear", x.packed if quantised else x, weight, act, k)
@@ -996,6 +997,9 @@ def mx_linear(x: Union[torch.Tensor, MxTensor], weight: MxTensor, bias: Optional
     stride = k
     if m:
         x, _, stride = _rows_of(x)
+        if stride >= 1 << 24:
+            x = x.contiguous()
+            stride = k
     return _mx_product("mx_linear", x.data_ptr(), None, _FLOAT_DTYPES[dtype], 1, m, k, 0, stride, weight, bias, act, y, _lib.LMI_MX_ROWS)
 
 
@@ -1017,10 +1021,10 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
     if planes and w == 1 and h > 1:
         planes = sh == 1
     rows = (k == 1 or sk == 1) and not planes and (h == 1 or w == 1 or sh == w * sw)
-    if not planes and not rows:
+    if (not planes and not rows) or (sk if planes else sw) >= 1 << 24:
         x = x.contiguous()
         sb, sk, sh, sw = x.stride()
-        planes, rows = h * w > 1, h * w <= 1
+        planes = h * w > 1
     if planes:
         y = _mx_out("mx_pointwise", out, (b, n, h, w), x.dtype, x.device)
         return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], b, h * w, k, sb, sk, weight, bias, act, y, _lib.LMI_MX_PLANES)

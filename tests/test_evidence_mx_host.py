@@ -91,6 +91,7 @@ def test_mx_arguments(L):
                 dict(x_dtype=6, x_scales=4096, layout=1)):
         assert _product(L, **bad) == -1, bad
     assert _product(L, w_packed=4104) == -2
+    assert _product(L, x_stride=1 << 24) == -4 and _product(L, layout=1, pixels=1 << 24) == -4 and _product(L, pixels=1 << 40) == -4
 
 
 def test_oracle_mx_by_hand():

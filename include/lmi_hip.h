@@ -501,8 +501,8 @@ int lmi_class_logprobs(const lmi_logprob_args *args, void *stream);
  * 2^(byte - 127), byte 255 = NaN; elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two per byte, the
  * earlier one in the low half.  Blocks are kept in the order the matrix instruction takes them, rows in groups of 32, k in
  * steps of 64 = two blocks:
- *   packed uint8 [G][S][2][32][16]  group of rows, step, which block of the step, row of the group, 16 bytes = 32 elements
- *   scales uint8 [G][Q][2][32][4]   group, four steps, block, row, step of the four
+ *   packed uint8 [S][G][2][32][16]  step, group of rows, which block of the step, row of the group, 16 bytes = 32 elements
+ *   scales uint8 [Q][G][2][32][4]   four steps, group, block, row, step of the four
  * with G = ceil(rows / 32), S = ceil(ceil(k / 32) / 2), Q = ceil(S / 4); rows and blocks beyond the tensor are zeros (scale byte 0).
  * lmi_mx_quantize: scale exponent floor(log2(max |x|)) - 2 of each block, at least -127 (also for a block of zeros);
  *   elements rounded to nearest, ties to even, beyond 6 to 6.  A block that holds an infinity or a NaN gets byte 255.

@@ -6,7 +6,8 @@
 // saturation; x / 2^e is exact, so nothing is rounded twice.  The products run on v_mfma_scale_f32_32x32x64_f8f6f4 (twice the
 // rate of the 16x16x128 form): 64 elements of k per instruction, every lane brings 32 elements of one row and their
 // scale byte -- one block --, sums in fp32.  Quantised tensors are kept in that order (see lmi_hip.h), so an operand of a
-// wave is one contiguous kilobyte, and the scale bytes of four steps are one word of which the instruction picks a byte.
+// wave is one contiguous kilobyte, and the scale bytes of four steps are one word of which the instruction picks a byte; a step of all rows lies together, so
+// that what neighbouring workgroups read at a time does, too.
 //
 // Kernels
 //  mx_quantize_kernel     a wave takes 8 rows x 256 elements: four lanes per block, 8 elements each, four steps per lane.
@@ -27,6 +28,7 @@ typedef float f16x __attribute__((ext_vector_type(16)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 struct Packed {};   // x is quantised already
 
@@ -74,6 +76,7 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *x, long long rows, long long k, long long row_stride, unsigned steps, unsigned quads,
                                                           long long units, unsigned *packed, unsigned *scales) {
   const int lane = threadIdx.x & 63, quarter = lane & 3, half = (lane >> 2) & 1, r8 = lane >> 3;
+  const long long groups = (rows + 31) >> 5;
   for (long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (long long)gridDim.x * 4) {   // row octet x four steps
     const long long octet = unit / quads;
     const unsigned quad = (unsigned)(unit - octet * quads);
@@ -96,9 +99,9 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *x, long long 
       m = max(m, __shfl_xor(m, 2));
       const unsigned byte = scale_byte(m), step = quad * 4 + i;
       word |= byte << (8 * i);
-      if (step < steps) packed[(((group * steps + step) * 2 + half) * 32 + rg) * 4 + quarter] = pack8(v[i], scale_value(byte));
+      if (step < steps) packed[(((step * groups + group) * 2 + half) * 32 + rg) * 4 + quarter] = pack8(v[i], scale_value(byte));
     }
-    if (quarter == 0) scales[((group * quads + quad) * 2 + half) * 32 + rg] = word;
+    if (quarter == 0) scales[((quad * groups + group) * 2 + half) * 32 + rg] = word;
   }
 }
 
@@ -132,18 +135,19 @@ template <typename T>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned *packed, const unsigned *scales, long long rows, long long k, unsigned steps,
                                                             unsigned quads, long long units, bool vec, T *out) {
   const int lane = threadIdx.x & 63, quarter = lane & 3, half = (lane >> 2) & 1, r8 = lane >> 3;
+  const long long groups = (rows + 31) >> 5;
   for (long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (long long)gridDim.x * 4) {
     const long long octet = unit / quads;
     const unsigned quad = (unsigned)(unit - octet * quads);
     const long long row = octet * 8 + r8, group = octet >> 2;
     if (row >= rows) continue;
     const int rg = (int)(octet & 3) * 8 + r8;
-    const unsigned word = scales[((group * quads + quad) * 2 + half) * 32 + rg];
+    const unsigned word = scales[((quad * groups + group) * 2 + half) * 32 + rg];
     unsigned w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const unsigned step = quad * 4 + i;
-      w[i] = step < steps ? packed[(((group * steps + step) * 2 + half) * 32 + rg) * 4 + quarter] : 0;
+      w[i] = step < steps ? packed[(((step * groups + group) * 2 + half) * 32 + rg) * 4 + quarter] : 0;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -247,8 +251,9 @@ constexpr int kWaveSteps = 2;   // deeper ones stream faster: 64 x 192 -> 192 on
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 template <typename T, bool PLANES> struct Raw;   // one step's values of a lane before they are quantised
+typedef float f2 __attribute__((ext_vector_type(2)));
 template <> struct Raw<float, true> {
-  float2 v[32];
+  f2 v[32];
 };
 template <typename T> struct Raw<T, true> {
   unsigned v[32];
@@ -259,17 +264,24 @@ template <typename T> struct Raw<T, false> {
 
 // Addresses are a base that is the same for the wave (scalar registers) plus a 32-bit offset of the lane: the launcher sees to it that
 // 32 channels or rows fit.
-template <typename W> __device__ __forceinline__ const W *at(const void *base, unsigned offset) { return (const W *)((const char *)base + offset); }
+template <typename W> __device__ __forceinline__ W at(const void *base, unsigned offset) {
+  typedef const __attribute__((address_space(1))) char *global;
+  global b = (global)base;
+  asm("" : "+s"(b));   // kept in scalar registers: without this the sum goes to a pair of vector registers per load
+  return *(const __attribute__((address_space(1))) W *)(b + offset);
+}
+template <typename W> __device__ __forceinline__ const W *at_any(const void *base, unsigned offset) { return (const W *)((const char *)base + offset); }   // a base of the lane's own
 
 // `in` channels (32 or more: all) of two neighbouring pixels from base + offset on; base is uniform
-template <typename T> __device__ __forceinline__ void load_planes(const T *base, unsigned offset, long long stride, bool live, int in, Raw<T, true> &r) {
+template <typename T, bool SCALAR = true>
+__device__ __forceinline__ void load_planes(const T *base, unsigned offset, long long stride, bool live, int in, Raw<T, true> &r) {
   typedef typename std::remove_reference<decltype(r.v[0])>::type W;
   if (live && in >= 32) {
 #pragma unroll
-    for (int u = 0; u < 32; ++u) r.v[u] = *at<W>(base + u * stride, offset);
+    for (int u = 0; u < 32; ++u) r.v[u] = SCALAR ? at<W>(base + u * stride, offset) : *at_any<W>(base + u * stride, offset);
   } else if (live && in > 0) {   // the last channels: all loads at once, those beyond read the first again
 #pragma unroll
-    for (int u = 0; u < 32; ++u) r.v[u] = *at<W>(base + (u < in ? u * stride : 0), offset);
+    for (int u = 0; u < 32; ++u) r.v[u] = *at_any<W>(base + (u < in ? u * stride : 0), offset);
 #pragma unroll
     for (int u = 0; u < 32; ++u) r.v[u] = u < in ? r.v[u] : W{};
   } else {
@@ -280,13 +292,13 @@ template <typename T> __device__ __forceinline__ void load_planes(const T *base,
 // the same value by value; `live` of the two pixels are there
 template <typename T> __device__ __forceinline__ void load_planes_single(const T *base, unsigned offset, long long stride, int live, int in, Raw<T, true> &r) {
   auto put = [&](int u, T a, T b) {
-    if constexpr (sizeof(T) == 4) r.v[u] = make_float2(a, b);
+    if constexpr (sizeof(T) == 4) r.v[u] = f2{a, b};
     else r.v[u] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
   };
   const unsigned next = offset + (live > 1 ? sizeof(T) : 0);   // what is not there reads a neighbour that is
   if (live > 0 && in >= 32) {
 #pragma unroll
-    for (int u = 0; u < 32; ++u) put(u, *at<T>(base + u * stride, offset), *at<T>(base + u * stride, next));
+    for (int u = 0; u < 32; ++u) put(u, at<T>(base + u * stride, offset), at<T>(base + u * stride, next));
     if (live == 1) {
 #pragma unroll
       for (int u = 0; u < 32; ++u) {
@@ -296,10 +308,10 @@ template <typename T> __device__ __forceinline__ void load_planes_single(const T
     }
   } else if (live > 0 && in > 0) {
 #pragma unroll
-    for (int u = 0; u < 32; ++u) put(u, *at<T>(base + (u < in ? u * stride : 0), offset), *at<T>(base + (u < in ? u * stride : 0), next));
+    for (int u = 0; u < 32; ++u) put(u, *at_any<T>(base + (u < in ? u * stride : 0), offset), *at_any<T>(base + (u < in ? u * stride : 0), next));
 #pragma unroll
     for (int u = 0; u < 32; ++u) {
-      if constexpr (sizeof(T) == 4) r.v[u] = make_float2(u < in ? r.v[u].x : 0.0f, u < in && live > 1 ? r.v[u].y : 0.0f);
+      if constexpr (sizeof(T) == 4) r.v[u] = f2{u < in ? r.v[u].x : 0.0f, u < in && live > 1 ? r.v[u].y : 0.0f};
       else r.v[u] = u < in ? (live > 1 ? r.v[u] : r.v[u] & 0xffffu) : 0u;
     }
   } else {
@@ -324,7 +336,7 @@ __device__ __forceinline__ void start_sums(const Product &P, int nt, int lane, f
   acc[0] = f16x{};
   if (P.bias) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[0][i] = n0 + i < P.n ? P.bias[n0 + i] : 0.0f;
+    for (int i = 0; i < 16; ++i) acc[0][i] = P.bias[n0 + i < P.n ? n0 + i : P.n - 1];   // rows beyond the last are not stored
   }
   acc[1] = acc[0];
 }
@@ -421,11 +433,11 @@ __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P,
   for (int nt = nt0; nt < nt1; ++nt) {
     f16x acc[2];
     start_sums(P, nt, lane, acc);
-    const uint4 *w = P.w + (long long)nt * S * 64 + wl;
+    const uint4 *w = P.w + nt * 64ll + wl;
     const unsigned sa = P.ws[nt * 64 + wl];
     uint4 a[kWaveSteps];
 #pragma unroll
-    for (int s = 0; s < kWaveSteps; ++s) a[s] = w[(s < S ? s : S - 1) * 64];
+    for (int s = 0; s < kWaveSteps; ++s) a[s] = w[(s < S ? s : S - 1) * (long long)P.tiles_n * 64];
     mfma2<0>(acc, a[0], sa, f[0][0], f[0][1], sw[0], sw[1]);
     if (S > 1) mfma2<1>(acc, a[1], sa, f[1][0], f[1][1], sw[0], sw[1]);
     store_planes<T>(P, y, p0, live, nt, lane, act, true, acc);
@@ -442,23 +454,23 @@ template <typename T> void launch_wave_planes(Product P, int act, long long batc
 }
 
 // Streaming product: 128 positions x up to 64 * NT weight rows per workgroup, k in chunks of two steps.  While the matrix instructions run
-// on one chunk, the next chunk's activations are on their way to registers and its weights on their way to LDS; an
-// activation block is quantised by the thread that loaded it.  Waves are dealt 2 (positions) x 2 (weight rows), each 64 positions x 32 * NT
+// on one chunk, the next chunk's activations and weights are on their way to registers (loads straight to LDS would be waited for
+// before the next read of any LDS); an activation block is quantised by the thread that loaded it.  Waves are dealt 2 (positions) x 2 (weight rows), each 64 positions x 32 * NT
 // rows of sums in registers: a fragment read from LDS serves 2 or NT matrix instructions.
 constexpr int kChunkTile = 128;
 
-template <typename T, bool PLANES> struct Chunk;   // what a thread holds of a chunk
+template <typename T, bool PLANES, bool VEC> struct Chunk;   // what a thread holds of a chunk
 // planes: two neighbouring pixels x one block
-template <typename T> struct Chunk<T, true> {
+template <typename T, bool VEC> struct Chunk<T, true, VEC> {
   Raw<T, true> raw;
   __device__ __forceinline__ void load(const Product &P, const T *x, int live, int chunk) {
     const int pair = threadIdx.x & 63;
     const long long c0 = (4ll * chunk + wave_id()) * 32;   // beyond k: in = 0
     const int in = c0 < P.k ? (int)(P.k - c0 < 32 ? P.k - c0 : 32) : 0;
-    if (P.vec) load_planes<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, 2 * pair < live, in, raw);
+    if constexpr (VEC) load_planes<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, 2 * pair < live, in, raw);
     else load_planes_single<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, live - 2 * pair, in, raw);
   }
-  __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) const {
+  template <int P> __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) const {
     const int pair = threadIdx.x & 63, kl = wave_id();
     const int sub = (pair >> 5) * 2, at = (kl & 1) * 32 + (pair & 31);
     uint4 f[2];
@@ -467,12 +479,12 @@ template <typename T> struct Chunk<T, true> {
 #pragma unroll
     for (int px = 0; px < 2; ++px) {
       xb[kl >> 1][sub + px][at] = f[px];
-      ((unsigned char *)&xs[sub + px][at])[kl >> 1] = (unsigned char)byte[px];
+      ((unsigned char *)&xs[sub + px][at])[2 * P + (kl >> 1)] = (unsigned char)byte[px];
     }
   }
 };
 // rows: eight pieces of 8 elements, four lanes per block
-template <typename T> struct Chunk<T, false> {
+template <typename T, bool VEC> struct Chunk<T, false, VEC> {
   typedef T piece __attribute__((ext_vector_type(8)));
   piece v[8];
   __device__ __forceinline__ void load(const Product &P, const T *x, int live, int chunk) {
@@ -484,8 +496,8 @@ template <typename T> struct Chunk<T, false> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const T *q = base + i * 16 * P.xs1;
-      if (P.vec && row + 16 * i < live && n >= 8) {
-        v[i] = *at<piece>(q, offset);
+      if (VEC && row + 16 * i < live && n >= 8) {
+        v[i] = at<piece>(q, offset);
       } else if (row + 16 * i < live && n > 0) {   // value by value: those beyond the row read its last again
         const T *single = x + (row + 16 * i) * P.xs1 + chunk * 128ll + (t & 15) * 8;
 #pragma unroll
@@ -497,7 +509,7 @@ template <typename T> struct Chunk<T, false> {
       }
     }
   }
-  __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) const {
+  template <int P> __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) const {
     const int t = threadIdx.x, quarter = t & 3, block = (t >> 2) & 3;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -513,26 +525,17 @@ template <typename T> struct Chunk<T, false> {
       m = max(m, __shfl_xor(m, 2));
       const unsigned byte = scale_byte(m);
       ((unsigned *)&xb[block >> 1][row >> 5][at])[quarter] = pack8(e, scale_value(byte));
-      if (quarter == 0) ((unsigned char *)&xs[row >> 5][at])[block >> 1] = (unsigned char)byte;
+      if (quarter == 0) ((unsigned char *)&xs[row >> 5][at])[2 * P + (block >> 1)] = (unsigned char)byte;
     }
   }
 };
 
-// 64 lanes x SIZE bytes from src (per lane) to dst (the wave's base; lane l lands at l * SIZE).  Complete for the workgroup after a
-// wait for vmcnt(0) and a barrier.
-template <int SIZE> __device__ __forceinline__ void to_lds(const void *src, void *dst) {
-  const auto from = (const __attribute__((address_space(1))) void *)src;
-  const auto to = (__attribute__((address_space(3))) void *)dst;
-  if constexpr (SIZE == 16) __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
-  else __builtin_amdgcn_global_load_lds(from, to, 4, 0, 0);
-}
-
-template <typename T, typename Y, bool PLANES, int NT>
-__global__ __launch_bounds__(256, NT <= 2 && (PLANES || sizeof(Y) == 2) ? 3 : 2) void mx_stream_kernel(const Product P, int act, int splits, long long tiles, int vec_y) {
+template <typename T, typename Y, bool PLANES, bool VEC, int NT>
+__global__ __launch_bounds__(256, sizeof(Y) == 2 && NT <= (PLANES ? 2 : 1) ? 3 : 2) void mx_stream_kernel(const Product P, int act, int splits, long long tiles, int vec_y) {
   __shared__ uint4 xb[2][2][4][64];
   __shared__ unsigned xs[2][4][64];
   __shared__ uint4 wb[2][2][2 * NT][64];
-  __shared__ unsigned wsb[2][2 * NT][64];
+  __shared__ unsigned wsb[2][(NT + 1) / 2 * 4][64];   // a multiple of the waves
   const int lane = threadIdx.x & 63, wave = wave_id(), wp = wave & 1, wn = wave >> 1;
   // workgroups go round the eight XCDs: the parts of one tile of positions are eight apart, so that they share an L2
   const long long tile = (long long)(blockIdx.x / (8 * splits)) * 8 + (blockIdx.x & 7);
@@ -541,88 +544,109 @@ __global__ __launch_bounds__(256, NT <= 2 && (PLANES || sizeof(Y) == 2) ? 3 : 2)
   const long long image = tile / P.tiles_pixels;
   const long long p0 = (tile - image * P.tiles_pixels) * kChunkTile;
   const int live = (int)(P.pixels - p0 < kChunkTile ? P.pixels - p0 : kChunkTile);
-  const int S = P.all_steps, quads = (S + 3) / 4, chunks = (S + 1) / 2, nt0 = part * 2 * NT;
+  const int S = P.all_steps, chunks = (S + 1) / 2, nt0 = part * 2 * NT;
 
-  auto load_weights = [&](int c, int buf) {
+  // What a wave brings of a chunk: of one of its two steps NT weight fragments, and of four steps their words of scale bytes;
+  // Packed: two of the rows' eight fragments and the words of group `wave`.  Pointers move on from chunk to chunk.
+  constexpr bool kPacked = __is_same(T, Packed);
+  constexpr int NW = (NT + 1) / 2;
+  const int step = wave & 1, wl = weight_lane(lane);   // the weights are put in the order of use: reads of LDS stay linear
+  const uint4 *wp_src[NT], *xp_src[2];
+  const unsigned *ws_src[NW], *xs_src = nullptr;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {   // 4 * NT fragments over four waves
-      const int id = j * 4 + wave, step = id & 1, t = id >> 1;
-      const int nt = nt0 + t < P.tiles_n ? nt0 + t : P.tiles_n - 1, s = 2 * c + step < S ? 2 * c + step : S - 1;
-      to_lds<16>(P.w + ((long long)nt * S + s) * 64 + lane, &wb[buf][step][t][0]);
-    }
+  for (int j = 0; j < NT; ++j) {
+    const int nt = nt0 + 2 * j + (wave >> 1);
+    wp_src[j] = P.w + ((long long)step * P.tiles_n + (nt < P.tiles_n ? nt : P.tiles_n - 1)) * 64;
+  }
 #pragma unroll
-    for (int j = 0; j < (NT + 1) / 2; ++j) {
-      const int t = j * 4 + wave;
-      if (t < 2 * NT) {
-        const int nt = nt0 + t < P.tiles_n ? nt0 + t : P.tiles_n - 1;
-        to_lds<4>(P.ws + ((long long)nt * quads + c / 2) * 64 + lane, &wsb[buf][t][0]);
-      }
-    }
-  };
-  const long long g0 = p0 >> 5;   // Packed: first group of rows
-  auto load_packed = [&](int c, int buf) {
-    const unsigned char *base = (const unsigned char *)P.x;
+  for (int j = 0; j < NW; ++j) {
+    const int nt = nt0 + 4 * j + wave;
+    ws_src[j] = P.ws + (nt < P.tiles_n ? nt : P.tiles_n - 1) * 64ll;
+  }
+  const long long groups = (P.pixels + 31) >> 5;
+  if constexpr (kPacked) {
+    const long long g0 = p0 >> 5;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int id = j * 4 + wave, step = id & 1, sub = id >> 1;
-      const long long groups = (P.pixels + 31) >> 5, g = g0 + sub < groups ? g0 + sub : groups - 1;
-      const int s = 2 * c + step < S ? 2 * c + step : S - 1;
-      to_lds<16>(base + ((g * S + s) * 64 + lane) * 16, &xb[buf][step][sub][0]);
+      const long long g = g0 + 2 * j + (wave >> 1);
+      xp_src[j] = (const uint4 *)P.x + (step * groups + (g < groups ? g : groups - 1)) * 64;
     }
-    const long long groups = (P.pixels + 31) >> 5, g = g0 + wave < groups ? g0 + wave : groups - 1;
-    to_lds<4>(P.xs + (g * quads + c / 2) * 64 + lane, &xs[buf][wave][0]);
+    xs_src = P.xs + (g0 + wave < groups ? g0 + wave : groups - 1) * 64;
+  }
+  u4 w_reg[NT], x_reg[2];
+  unsigned ws_reg[NW], xs_reg = 0;
+  auto load_part = [&](int c, auto parity) {
+    if (2 * c + step < S) {   // the second step of the last chunk may be missing: not used then
+#pragma unroll
+      for (int j = 0; j < NT; ++j) w_reg[j] = at<u4>(wp_src[j], wl * 16);
+      if constexpr (kPacked) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) x_reg[j] = at<u4>(xp_src[j], lane * 16);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) wp_src[j] += 128ll * P.tiles_n;
+    if constexpr (kPacked) xp_src[0] += 128 * groups, xp_src[1] += 128 * groups;
+    if constexpr (decltype(parity)::value == 0) {   // a word of scale bytes serves two chunks
+#pragma unroll
+      for (int j = 0; j < NW; ++j) {
+        ws_reg[j] = at<unsigned>(ws_src[j], wl * 4);
+        ws_src[j] += 64ll * P.tiles_n;
+      }
+      if constexpr (kPacked) {
+        xs_reg = at<unsigned>(xs_src, lane * 4);
+        xs_src += 64 * groups;
+      }
+    }
   };
 
   f16x acc[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) start_sums(P, nt0 + wn * NT + t, lane, acc[t]);
-  const int wl = weight_lane(lane);
-  auto multiply_chunk = [&](int c, int buf) {
-    const int shift = 16 * (c & 1);
-    unsigned sb0 = xs[buf][2 * wp][lane], sb1 = xs[buf][2 * wp + 1][lane];
-    if constexpr (__is_same(T, Packed)) sb0 >>= shift, sb1 >>= shift;
+
+  const T *x = nullptr;
+  typename std::conditional<kPacked, int, Chunk<T, PLANES, VEC>>::type hold;
+  if constexpr (!kPacked) x = (const T *)P.x + image * P.xb + (PLANES ? p0 : p0 * P.xs1);
+  load_part(0, std::integral_constant<int, 0>());
+  if constexpr (!kPacked) hold.load(P, x, live, 0);
+
+  // Chunk c goes through buffer c & 1, which was read for c - 2 last: every wave is past the barrier of c - 1 by now.
+  auto chunk = [&](int c, auto parity) {
+    constexpr int B = decltype(parity)::value;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *(u4 *)&wb[B][step][2 * j + (wave >> 1)][lane] = w_reg[j];
+#pragma unroll
+    for (int j = 0; j < NW; ++j) wsb[B][4 * j + wave][lane] = ws_reg[j];
+    if constexpr (kPacked) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) *(u4 *)&xb[B][step][2 * j + (wave >> 1)][lane] = x_reg[j];
+      xs[B][wave][lane] = xs_reg;
+    } else {
+      hold.template put<B>(xb[B], xs[B]);
+    }
+    __syncthreads();
+    if (c + 1 < chunks) {
+      load_part(c + 1, std::integral_constant<int, 1 - B>());
+      if constexpr (!kPacked) hold.load(P, x, live, c + 1);
+    }
+    const unsigned sb0 = xs[B][2 * wp][lane], sb1 = xs[B][2 * wp + 1][lane];
     unsigned sa[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) sa[t] = wsb[buf][wn * NT + t][wl] >> shift;
+    for (int t = 0; t < NT; ++t) sa[t] = wsb[B][wn * NT + t][lane];
     {
-      const uint4 b0 = xb[buf][0][2 * wp][lane], b1 = xb[buf][0][2 * wp + 1][lane];
+      const uint4 b0 = xb[B][0][2 * wp][lane], b1 = xb[B][0][2 * wp + 1][lane];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) mfma2<0>(acc[t], wb[buf][0][wn * NT + t][wl], sa[t], b0, b1, sb0, sb1);
+      for (int t = 0; t < NT; ++t) mfma2<2 * B>(acc[t], wb[B][0][wn * NT + t][lane], sa[t], b0, b1, sb0, sb1);
     }
     if (2 * c + 1 < S) {
-      const uint4 b0 = xb[buf][1][2 * wp][lane], b1 = xb[buf][1][2 * wp + 1][lane];
+      const uint4 b0 = xb[B][1][2 * wp][lane], b1 = xb[B][1][2 * wp + 1][lane];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) mfma2<1>(acc[t], wb[buf][1][wn * NT + t][wl], sa[t], b0, b1, sb0, sb1);
+      for (int t = 0; t < NT; ++t) mfma2<2 * B + 1>(acc[t], wb[B][1][wn * NT + t][lane], sa[t], b0, b1, sb0, sb1);
     }
   };
-
-  if constexpr (__is_same(T, Packed)) {
-    load_weights(0, 0);
-    load_packed(0, 0);
-    for (int c = 0; c < chunks; ++c) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this chunk's weights and rows are in LDS
-      __syncthreads();
-      if (c + 1 < chunks) {
-        load_weights(c + 1, (c + 1) & 1);
-        load_packed(c + 1, (c + 1) & 1);
-      }
-      multiply_chunk(c, c & 1);
-    }
-  } else {
-    const T *x = (const T *)P.x + image * P.xb + (PLANES ? p0 : p0 * P.xs1);
-    Chunk<T, PLANES> hold;
-    load_weights(0, 0);
-    hold.load(P, x, live, 0);
-    for (int c = 0; c < chunks; ++c) {
-      hold.put(xb[c & 1], xs[c & 1]);                    // chunk c - 2 used this buffer: every wave is past the barrier of c - 1
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this chunk's weights are in LDS
-      __syncthreads();
-      if (c + 1 < chunks) {
-        load_weights(c + 1, (c + 1) & 1);                // chunk c - 1 used this buffer: every wave is past it
-        hold.load(P, x, live, c + 1);
-      }
-      multiply_chunk(c, c & 1);
-    }
+  for (int c = 0; c < chunks; c += 2) {
+    chunk(c, std::integral_constant<int, 0>());
+    if (c + 1 < chunks) chunk(c + 1, std::integral_constant<int, 1>());
   }
 
   Y *y = (Y *)P.y + image * P.pixels * P.n;
@@ -631,27 +655,31 @@ __global__ __launch_bounds__(256, NT <= 2 && (PLANES || sizeof(Y) == 2) ? 3 : 2)
   for (int t = 0; t < NT; ++t) {
     const int nt = nt0 + wn * NT + t;
     if (nt < P.tiles_n) {
-      if constexpr (PLANES) store_planes<Y>(P, y, p0 + 64 * wp, live_w, nt, lane, act, P.vec, acc[t]);
+      if constexpr (PLANES) store_planes<Y>(P, y, p0 + 64 * wp, live_w, nt, lane, act, VEC, acc[t]);
       else store_rows<Y>(P, y, p0 + 64 * wp, live_w, nt, lane, act, vec_y, acc[t]);
     }
   }
 }
 
-template <typename T, typename Y, bool PLANES> void launch_stream(Product P, int act, long long batch, hipStream_t st) {
+template <typename T, typename Y, bool PLANES, bool VEC> void launch_stream(Product P, int act, long long batch, hipStream_t st) {
   P.tiles_pixels = (unsigned)((P.pixels + kChunkTile - 1) / kChunkTile);
   const long long tiles = batch * P.tiles_pixels;
-  constexpr int kMaxNT = sizeof(Y) == 4 && !__is_same(T, Packed) ? 4 : 5;
+  // as many weight rows per workgroup as the registers hold beside a chunk (fp32 and single loads hold more): 1280 -> 320 on 64 maps of 80 x 80
+  // with 5 tiles per wave 302 us, with 3 or 4 and the activations read twice through the L2 415
+  constexpr int kMaxNT = !VEC ? 3 : __is_same(T, Packed) ? 5 : PLANES && sizeof(Y) == 2 ? 5 : 4;
   int splits = (P.tiles_n + 2 * kMaxNT - 1) / (2 * kMaxNT);
   while (tiles * splits < 256 && splits * 2 <= P.tiles_n) splits *= 2;
   int nt = (P.tiles_n + 2 * splits - 1) / (2 * splits);
   splits = (P.tiles_n + 2 * nt - 1) / (2 * nt);
   const int vec_y = (uintptr_t)P.y % 16 == 0 && P.n * sizeof(Y) % 16 == 0;
   const unsigned grid = (unsigned)((tiles + 7) / 8 * 8 * splits);
-  if (nt == 1) mx_stream_kernel<T, Y, PLANES, 1><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
-  else if (nt == 2) mx_stream_kernel<T, Y, PLANES, 2><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
-  else if (nt == 3) mx_stream_kernel<T, Y, PLANES, 3><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
-  else if (nt == 4) mx_stream_kernel<T, Y, PLANES, 4><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
-  else mx_stream_kernel<T, Y, PLANES, kMaxNT><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  if (nt == 1) mx_stream_kernel<T, Y, PLANES, VEC, 1><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  else if (nt == 2) mx_stream_kernel<T, Y, PLANES, VEC, 2><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  else if (nt == 3) mx_stream_kernel<T, Y, PLANES, VEC, 3><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  else if constexpr (kMaxNT > 3) {
+    if (nt == 4) mx_stream_kernel<T, Y, PLANES, VEC, 4><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+    else mx_stream_kernel<T, Y, PLANES, VEC, kMaxNT><<<grid, 256, 0, st>>>(P, act, splits, tiles, vec_y);
+  }
 }
 
 // Few positions: 64 of them x 32 weight rows per workgroup, its eight waves share k.  A wave loads its steps' blocks straight into the
@@ -666,13 +694,13 @@ template <typename T, bool PLANES>
 __device__ __forceinline__ void load_few(const Product &P, const T *x, long long p0, int live, int step, int lane, uint4 (&f)[2], unsigned (&byte)[2]) {
   const int j = lane & 31;
   if constexpr (__is_same(T, Packed)) {
-    const int quads = (P.all_steps + 3) / 4;
+    const long long groups = (P.pixels + 31) >> 5;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const long long group = (p0 >> 5) + h;
       const bool in = 32 * h < live;   // rows of the last group that lie beyond are zeros
-      f[h] = in ? ((const uint4 *)P.x)[(group * P.all_steps + step) * 64 + lane] : make_uint4(0, 0, 0, 0);
-      byte[h] = in ? (P.xs[(group * quads + step / 4) * 64 + lane] >> (8 * (step & 3))) & 255u : 0u;
+      f[h] = in ? ((const uint4 *)P.x)[(step * groups + group) * 64 + lane] : make_uint4(0, 0, 0, 0);
+      byte[h] = in ? (P.xs[(step / 4 * groups + group) * 64 + lane] >> (8 * (step & 3))) & 255u : 0u;
     }
   } else {
     const long long c0 = step * 64ll + (lane >> 5) * 32;
@@ -680,7 +708,7 @@ __device__ __forceinline__ void load_few(const Product &P, const T *x, long long
     if constexpr (PLANES) {
       if (P.vec) {
         Raw<T, true> raw;
-        load_planes<T>(x + step * 64ll * P.xs1, (unsigned)((lane >> 5) * 32 * P.xs1 + 2 * j) * sizeof(T), P.xs1, 2 * j < live, in, raw);
+        load_planes<T, false>(x + step * 64ll * P.xs1, (unsigned)((lane >> 5) * 32 * P.xs1 + 2 * j) * sizeof(T), P.xs1, 2 * j < live, in, raw);
         quantize_raw(raw, f, byte);
         return;
       }
@@ -691,7 +719,7 @@ __device__ __forceinline__ void load_few(const Product &P, const T *x, long long
       const long long stride = PLANES ? P.xs1 : 1;
       const T *base = x + step * 64ll * stride;
       const unsigned offset = (unsigned)((lane >> 5) * 32 * stride + px * (PLANES ? 1 : P.xs1)) * sizeof(T);
-      const T *q = at<T>(base, offset);
+      const T *q = at_any<T>(base, offset);
       float v[32];
       if (!PLANES && P.vec && px < live && in == 32) {
 #pragma unroll
@@ -703,10 +731,10 @@ __device__ __forceinline__ void load_few(const Product &P, const T *x, long long
         }
       } else if (px < live && in == 32) {
 #pragma unroll
-        for (int u = 0; u < 32; ++u) v[u] = to_float(*at<T>(base + u * stride, offset));
+        for (int u = 0; u < 32; ++u) v[u] = to_float(*at_any<T>(base + u * stride, offset));
       } else if (px < live && in > 0) {   // all loads at once: channels beyond the last read the first again
 #pragma unroll
-        for (int u = 0; u < 32; ++u) v[u] = to_float(*at<T>(base + (u < in ? u * stride : 0), offset));
+        for (int u = 0; u < 32; ++u) v[u] = to_float(*at_any<T>(base + (u < in ? u * stride : 0), offset));
 #pragma unroll
         for (int u = 0; u < 32; ++u) v[u] = u < in ? v[u] : 0.0f;
       } else {
@@ -721,17 +749,17 @@ __device__ __forceinline__ void load_few(const Product &P, const T *x, long long
 template <typename T, typename Y, bool PLANES>
 __global__ __launch_bounds__(64 * kFewWaves, 4) void mx_few_kernel(const Product P, int act) {
   __shared__ float part[kFewWaves][32][64];
-  const int lane = threadIdx.x & 63, wave = wave_id(), S = P.all_steps, quads = (S + 3) / 4;
+  const int lane = threadIdx.x & 63, wave = wave_id(), S = P.all_steps;
   const long long image = blockIdx.x / P.tiles_pixels;
   const long long p0 = (long long)(blockIdx.x % P.tiles_pixels) * kTile;
   const int live = (int)(P.pixels - p0 < kTile ? P.pixels - p0 : kTile);
   const int nt = blockIdx.y, wl = weight_lane(lane);
-  const uint4 *w = P.w + (long long)nt * S * 64 + wl;
-  const unsigned *ws = P.ws + (long long)nt * quads * 64 + wl;
+  const uint4 *w = P.w + nt * 64ll + wl;
+  const unsigned *ws = P.ws + nt * 64ll + wl;
   f16x acc[2] = {};
   for (int s = wave; s < S; s += kFewWaves) {
-    const uint4 a = w[s * 64ll];
-    const unsigned sa = ws[(s >> 2) * 64ll] >> (8 * (s & 3));
+    const uint4 a = w[s * 64ll * P.tiles_n];
+    const unsigned sa = ws[(s >> 2) * 64ll * P.tiles_n] >> (8 * (s & 3));
     uint4 f[2];
     unsigned byte[2];
     if constexpr (__is_same(T, Packed)) load_few<T, PLANES>(P, nullptr, p0, live, s, lane, f, byte);
@@ -778,7 +806,12 @@ template <typename T, typename Y, bool PLANES> int launch_product(Product P, int
       return lmi_check_launch("lmi_mx_product");
     }
   }
-  launch_stream<T, Y, PLANES>(P, act, batch, st);
+  if constexpr (__is_same(T, Packed)) {
+    launch_stream<T, Y, false, true>(P, act, batch, st);
+  } else {
+    if (P.vec) launch_stream<T, Y, PLANES, true>(P, act, batch, st);
+    else launch_stream<T, Y, PLANES, false>(P, act, batch, st);
+  }
   return lmi_check_launch("lmi_mx_product");
 }
 

@@ -847,17 +847,17 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
 
 
 def _mx_sizes(shape):
-    """Shapes of an MxTensor's parts: ((G, S, 1024), (G, Q, 256))."""
+    """Shapes of an MxTensor's parts: ((S, G, 1024), (Q, G, 256))."""
     groups = -(-math.prod(shape[:-1]) // 32)
     steps = -(-shape[-1] // 64)
-    return (groups, steps, 1024), (groups, -(-steps // 4), 256)
+    return (steps, groups, 1024), (-(-steps // 4), groups, 256)
 
 
 class MxTensor:
     """A tensor (..., k) in MXFP4: blocks of 32 elements along the last dimension share a power-of-two scale; 4.25 bits per
-    element.  The blocks lie in the order the matrix instruction takes them, rows in groups of 32, k in steps of 64 (two
-    blocks): packed uint8 (G, S, 1024), a step's kilobyte as (block, row, 16 bytes), two elements per byte, the earlier one in
-    the low half; scales uint8 (G, Q, 256), the bytes of four steps as (block, row, step): 2^(byte - 127), 255 = NaN.
+    element.  The blocks lie in the order the matrix instruction takes them, k in steps of 64 (two blocks), rows in groups of
+    32: packed uint8 (S, G, 1024), a group's kilobyte as (block, row, 16 bytes), two elements per byte, the earlier one in
+    the low half; scales uint8 (Q, G, 256), the bytes of four steps as (block, row, step): 2^(byte - 127), 255 = NaN.
     G = ceil(rows / 32), S = ceil(k / 64), Q = ceil(S / 4); what lies beyond the tensor is zero."""
 
     __slots__ = ("packed", "scales", "shape")

@@ -41,13 +41,13 @@ def unpack(packed):
 
 
 def rows_of(packed, scales, rows, k):
-    """The kernels' order -- packed (G, S, [2][32][16]), scales (G, Q, [2][32][4]): group of 32 rows, step of 64 along k (scales: four steps),
+    """The kernels' order -- packed (S, G, [2][32][16]), scales (Q, G, [2][32][4]): step of 64 along k (scales: four steps), group of 32 rows,
     block of the step, row, bytes (steps) -- as (bytes (rows, 16*B), scales (rows, B)); and whether all that lies beyond is zero."""
     packed, scales = np.asarray(packed), np.asarray(scales)
     packed, scales = packed.reshape(*packed.shape[:2], 2, 32, 16), scales.reshape(*scales.shape[:2], 2, 32, 4)
     b = -(-k // BLOCK)
-    p = packed.transpose(0, 3, 1, 2, 4).reshape(packed.shape[0] * 32, -1)
-    s = scales.transpose(0, 3, 1, 4, 2).reshape(scales.shape[0] * 32, -1)
+    p = packed.transpose(1, 3, 0, 2, 4).reshape(packed.shape[1] * 32, -1)
+    s = scales.transpose(1, 3, 0, 4, 2).reshape(scales.shape[1] * 32, -1)
     clean = not (p[rows:].any() or p[:, 16 * b:].any() or s[rows:].any() or s[:, b:].any())
     return p[:rows, :16 * b], s[:rows, :b], clean
 

@@ -35,8 +35,8 @@ def test_cpu_tensors_are_refused():
 
 
 @pytest.mark.parametrize("packed,scales,shape", [((2, 32), (2, 2), (2, 33)), ((1, 1, 1024), (1, 1, 256), (33, 33)),
-                                                 ((1, 1, 1024), (1, 1, 256), (2, 65)), ((1, 2, 1024), (1, 2, 256), (2, 65)),
-                                                 ((1, 5, 1024), (1, 1, 256), (2, 300))])
+                                                 ((1, 1, 1024), (1, 1, 256), (2, 65)), ((2, 1, 1024), (2, 1, 256), (2, 65)),
+                                                 ((5, 1, 1024), (1, 1, 256), (2, 300))])
 def test_mx_tensor_checks_its_parts(packed, scales, shape):
     from object_detectors_amd import hip_ops as ops
     with pytest.raises(ValueError, match="MxTensor"):
@@ -109,12 +109,12 @@ def test_oracle_mx_by_hand():
 
 def test_oracle_order_by_hand():
     """Row 33, block 5 of k = 200: group 1, row 1 of it, step 2, second block; its scale in the first four steps, third of them."""
-    packed, scales = np.zeros((2, 4, 2, 32, 16), np.uint8), np.zeros((2, 1, 2, 32, 4), np.uint8)
-    packed[1, 2, 1, 1, 3], scales[1, 0, 1, 1, 2] = 7, 9
+    packed, scales = np.zeros((4, 2, 2, 32, 16), np.uint8), np.zeros((1, 2, 2, 32, 4), np.uint8)
+    packed[2, 1, 1, 1, 3], scales[0, 1, 1, 1, 2] = 7, 9
     p, s, clean = OM.rows_of(packed, scales, 40, 200)
     assert clean and p.shape == (40, 112) and s.shape == (40, 7)
     assert p[33, 5 * 16 + 3] == 7 and s[33, 5] == 9 and int(p.sum()) == 7 and int(s.sum()) == 9
-    packed[1, 3, 1] = 1          # block 7 lies beyond k
+    packed[3, 1, 1] = 1          # block 7 lies beyond k
     assert not OM.rows_of(packed, scales, 40, 200)[2]
 
 

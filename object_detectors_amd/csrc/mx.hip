@@ -11,7 +11,7 @@
 //
 // Kernels
 //  mx_quantize_kernel     a wave takes 8 rows x 256 elements: four lanes per block, 8 elements each, four steps per lane.
-//  mx_dequantize_kernel   the same shape backwards.
+//  mx_dequantize_kernel   8 rows x one step per wave, whole lines written.
 //  mx_stream_kernel       the product of many positions: 128 of them x up to 320 weight rows per workgroup, streamed along k.
 //  mx_wave_planes_kernel  shallow 1x1 convolutions (k <= 128): a wave per 64 positions, everything in registers.
 //  mx_few_kernel          few positions (a single row, one image's deepest maps): the waves of a workgroup share k.
@@ -29,6 +29,7 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 
 struct Packed {};   // x is quantised already
 
@@ -105,60 +106,64 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *x, long long 
   }
 }
 
-template <typename T> __device__ __forceinline__ void store8(T *p, long long n, bool vec, const float (&v)[8]) {
-  if (vec && n >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      ((float4 *)p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      ((float4 *)p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      typedef T t8 __attribute__((ext_vector_type(8)));
-      t8 a;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) a[u] = (T)v[u];
-      *(t8 *)p = a;
-    }
-  } else {
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (u < n) p[u] = (T)v[u];
-  }
-}
-
-// e2m1 code -> value
-__device__ __forceinline__ float code_value(unsigned c) {
-  const unsigned m = c & 7u;
-  const float a = m < 2u ? 0.5f * m : (1.0f + 0.5f * (m & 1u)) * (float)(1u << ((m >> 1) - 1u));
-  return (c & 8u) ? -a : a;
-}
-
+// A wave takes 8 rows x one step.  16-bit results: lane (row, block, quarter) writes 8 of them, a row's eight lanes one line of 128
+// bytes.  fp32: a line is one block, so the eight lanes write block 0, then block 1, four elements each, which they get from the lane
+// that read them.
 template <typename T>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned *packed, const unsigned *scales, long long rows, long long k, unsigned steps,
-                                                            unsigned quads, long long units, bool vec, T *out) {
+                                                            long long units, bool vec, T *out) {
   const int lane = threadIdx.x & 63, quarter = lane & 3, half = (lane >> 2) & 1, r8 = lane >> 3;
   const long long groups = (rows + 31) >> 5;
   for (long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (long long)gridDim.x * 4) {
-    const long long octet = unit / quads;
-    const unsigned quad = (unsigned)(unit - octet * quads);
+    const long long octet = unit / steps;
+    const unsigned step = (unsigned)(unit - octet * steps);
     const long long row = octet * 8 + r8, group = octet >> 2;
-    if (row >= rows) continue;
     const int rg = (int)(octet & 3) * 8 + r8;
-    const unsigned word = scales[((quad * groups + group) * 2 + half) * 32 + rg];
-    unsigned w[4];
+    const unsigned word = packed[(((step * groups + group) * 2 + half) * 32 + rg) * 4 + quarter];   // rows beyond the last are zeros there
+    const unsigned byte = (scales[(((step >> 2) * groups + group) * 2 + half) * 32 + rg] >> (8 * (step & 3))) & 255u;
+    // 2^(byte - 127); the smallest is subnormal, 255 is NaN
+    const float s = byte == 255u ? NAN : (byte ? __uint_as_float(byte << 23) : 0x1p-127f);
+    T *p = out + row * k + step * 64ll;
+    if constexpr (sizeof(T) == 4) {
+      const int i = lane & 7;   // of the row's eight lanes
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned step = quad * 4 + i;
-      w[i] = step < steps ? packed[(((step * groups + group) * 2 + half) * 32 + rg) * 4 + quarter] : 0;
-    }
+      for (int b = 0; b < 2; ++b) {
+        const int from = (lane & ~7) + b * 4 + (i >> 1);
+        const unsigned w = (unsigned)__shfl((int)word, from) >> (16 * (i & 1));
+        const float sb = __shfl(s, from);
+        const f2 lo = __builtin_bit_cast(f2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0)), hi = __builtin_bit_cast(f2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1));
+        const long long left = k - step * 64ll - b * 32 - i * 4;
+        T *q = p + b * 32 + i * 4;
+        if (row < rows) {
+          if (vec && left >= 4) {
+            typedef float f4 __attribute__((ext_vector_type(4)));
+            __builtin_nontemporal_store(f4{lo.x * sb, lo.y * sb, hi.x * sb, hi.y * sb}, (f4 *)q);
+          } else {
+            if (left > 0) q[0] = lo.x * sb;
+            if (left > 1) q[1] = lo.y * sb;
+            if (left > 2) q[2] = hi.x * sb;
+            if (left > 3) q[3] = hi.y * sb;
+          }
+        }
+      }
+    } else {
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      t8 v;
+      const f2 e0 = __builtin_bit_cast(f2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 0)), e1 = __builtin_bit_cast(f2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 1)),
+               e2 = __builtin_bit_cast(f2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 2)), e3 = __builtin_bit_cast(f2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 3));
+      v[0] = (T)(e0.x * s), v[1] = (T)(e0.y * s), v[2] = (T)(e1.x * s), v[3] = (T)(e1.y * s);
+      v[4] = (T)(e2.x * s), v[5] = (T)(e2.y * s), v[6] = (T)(e3.x * s), v[7] = (T)(e3.y * s);
+      const long long left = k - step * 64ll - half * 32 - quarter * 8;
+      T *q = p + half * 32 + quarter * 8;
+      if (row < rows) {
+        if (vec && left >= 8) {
+          __builtin_nontemporal_store(v, (t8 *)q);
+        } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long c0 = ((long long)quad * 4 + i) * 64 + half * 32 + quarter * 8;
-      const unsigned byte = (word >> (8 * i)) & 255u;
-      // 2^(byte - 127); the smallest is subnormal, 255 is NaN
-      const float s = byte == 255u ? NAN : (byte ? __uint_as_float(byte << 23) : 0x1p-127f);
-      float v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = code_value((w[i] >> (4 * u)) & 15u) * s;
-      store8(out + row * k + c0, k - c0, vec, v);
+          for (int u = 0; u < 8; ++u)
+            if (u < left) q[u] = v[u];
+        }
+      }
     }
   }
 }
@@ -251,7 +256,6 @@ constexpr int kWaveSteps = 2;   // deeper ones stream faster: 64 x 192 -> 192 on
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 template <typename T, bool PLANES> struct Raw;   // one step's values of a lane before they are quantised
-typedef float f2 __attribute__((ext_vector_type(2)));
 template <> struct Raw<float, true> {
   f2 v[32];
 };
@@ -841,7 +845,8 @@ template <typename T> void quantize(const void *x, int64_t rows, int64_t k, int6
 }
 template <typename T> void dequantize(const void *packed, const void *scales, int64_t rows, int64_t k, const Units &u, void *out, hipStream_t st) {
   const bool vec = lmi_is_aligned(out, 16) && k * sizeof(T) % 16 == 0;
-  mx_dequantize_kernel<<<u.grid, 256, 0, st>>>((const unsigned *)packed, (const unsigned *)scales, rows, k, u.steps, u.quads, u.units, vec, (T *)out);
+  const long long units = u.units / u.quads * u.steps, wanted = (units + 3) / 4;   // octets x steps
+  mx_dequantize_kernel<<<(unsigned)(wanted < (1 << 23) ? wanted : (1 << 23)), 256, 0, st>>>((const unsigned *)packed, (const unsigned *)scales, rows, k, u.steps, units, vec, (T *)out);
 }
 
 }  // namespace

@@ -794,18 +794,20 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
             raise TypeError("class_logprobs: labels must be int64, int32 or float32 on x's device")
         if tuple(labels.shape) != lead:
             raise ValueError(f"class_logprobs: labels must have shape {lead}")
-    want = {"logprob": (lead, torch.float32)} if labels is not None else {}
-    want["entropy"] = (lead, torch.float32)
+    want = [("entropy", lead, torch.float32)]
+    if labels is not None:
+        want.append(("logprob", lead, torch.float32))
     if top:
-        want["top_logprob"], want["top_index"] = (lead + (top,), torch.float32), (lead + (top,), torch.int32)
-    if out is None:
-        out = {k: torch.empty(s, dtype=d, device=dev) for k, (s, d) in want.items()}
-    else:
-        for k, (s, d) in want.items():
-            t = out.get(k)
-            if t is None or tuple(t.shape) != s or t.dtype != d or not t.is_contiguous() or t.device != dev:
-                raise ValueError(f"class_logprobs: out[{k!r}] must be a contiguous {d} tensor of shape {s} on x's device")
-        out = {k: out[k] for k in want}
+        want += [("top_logprob", lead + (top,), torch.float32), ("top_index", lead + (top,), torch.int32)]
+    res = {}
+    for key, size, dtype in want:
+        if out is None:
+            res[key] = torch.empty(size, dtype=dtype, device=dev)
+            continue
+        t = res[key] = out.get(key)
+        if t is None or t.shape != size or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"class_logprobs: out[{key!r}] must be a contiguous {dtype} tensor of shape {size} on x's device")
+    out = res
     rows = math.prod(lead)
     if rows == 0:
         return out
@@ -901,12 +903,19 @@ def mx_quantize(x: torch.Tensor) -> MxTensor:
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError("mx_quantize: x must hold at least one element in its last dimension")
     shape, k, dev = x.shape, x.shape[-1], x.device
-    rows = math.prod(shape[:-1])
-    packed, scales = (torch.empty(s, dtype=torch.uint8, device=dev) for s in _mx_sizes(shape))
+    size_p, size_s = _mx_sizes(shape)
+    q = MxTensor.__new__(MxTensor)
+    packed = q.packed = torch.empty(size_p, dtype=torch.uint8, device=dev)
+    scales = q.scales = torch.empty(size_s, dtype=torch.uint8, device=dev)
+    q.shape = shape
+    rows = x.numel() // k
     if rows:
-        x, _, stride = _rows_of(x)
+        if x.is_contiguous():
+            stride = k
+        else:
+            x, _, stride = _rows_of(x)
         _launch(_L.lmi_mx_quantize, x.data_ptr(), dev, _FLOAT_DTYPES[x.dtype], rows, k, stride, packed.data_ptr(), scales.data_ptr())
-    return MxTensor(packed, scales, shape)
+    return q
 
 
 def _need_mx(q, name: str) -> None:
@@ -995,7 +1004,7 @@ def mx_linear(x: Union[torch.Tensor, MxTensor], weight: MxTensor, bias: Optional
     if quantised:
         return _mx_product("mx_linear", x.packed.data_ptr(), x.scales.data_ptr(), _lib.LMI_MXFP4, 1, m, k, 0, 0, weight, bias, act, y, _lib.LMI_MX_ROWS)
     stride = k
-    if m:
+    if m and not x.is_contiguous():
         x, _, stride = _rows_of(x)
         if stride >= 1 << 24:
             x = x.contiguous()

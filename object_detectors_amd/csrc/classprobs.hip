@@ -23,6 +23,8 @@
 //                          neighbouring rows' values of one class at a time; the alternatives sit in registers.
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -39,6 +41,7 @@ struct Evidence {
   float *logprob, *entropy, *top_logprob;
   int *top_index;
   unsigned char *ws;
+  int wide;            // the outputs of two rows may be written as one word (planes kernel, top 2)
   int parts;           // parts per row (rows kernel)
   long long part_len;  // classes per part
 };
@@ -119,8 +122,8 @@ __device__ __forceinline__ void softmax_result(const Sums &a, float &ref, float 
     log_s = 0.0f;
     h = 0.0f;
   } else {
-    log_s = logf(a.s);
-    h = log_s - a.t / a.s;
+    log_s = __builtin_amdgcn_logf(a.s) * 0.6931471805599453f;   // s lies in [1, classes]
+    h = fmaf(-a.t, __builtin_amdgcn_rcpf(a.s), log_s);
   }
 }
 
@@ -172,7 +175,7 @@ template <int NT> __device__ __forceinline__ void team_sync() {
 constexpr int kCand = 256;
 template <int NT> struct TeamShared {
   float lane_max[NT / 64][64];
-  float red[NT / 64][2];
+  float red[NT / 64][3];
   u64 best[NT / 64];
   u64 cand[kCand + kMaxTop];
   u64 list[kMaxTop];   // the best so far, descending
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(256) void evidence_team_kernel(const Evidence E, lo
   const int l = threadIdx.x & 15, group = (threadIdx.x & 63) >> 4;
   const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
   bool on = row < rows;
-  const long long o = on ? row / E.n1 : 0, m = on ? row - o * E.n1 : 0;
+  const long long o = on ? (unsigned)row / (unsigned)E.n1 : 0, m = on ? row - o * E.n1 : 0;
   if (on && E.count && m >= E.count[o]) on = false;
   long long i = m;
   if (on && E.index) {
@@ -362,7 +365,7 @@ template <typename T, int NT, int J, int V, int ACT>
 __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, int part, int t, TeamShared<NT> &L) {
   typedef Group<T, V> G;
   const int lane = t & 63, wave = t >> 6;
-  const long long o = row / E.n1, m = row - o * E.n1;
+  const long long o = (unsigned)row / (unsigned)E.n1, m = row - o * E.n1;
   if (E.count && m >= E.count[o]) return;
   long long i = m;
   if (E.index) {
@@ -380,7 +383,7 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
   const int start = V > 1 ? -(int)(((uintptr_t)xp & 15) / sizeof(T)) : 0;
 
   if (t < kMaxTop) L.list[t] = 0;
-  Sums S = {-INFINITY, 0.0f, 0.0f};   // softmax: sums with respect to the team's m; else t = the entropy
+  Sums S = {-INFINITY, 0.0f, 0.0f};   // softmax: this thread's sums with respect to its own m; else t = the entropy
   constexpr int N = J * V;
   const T absent = (T)(ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);   // adds nothing to the sums
   for (long long tile = start; tile < len; tile += NT * N) {
@@ -399,35 +402,37 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
         }
       }
     }
-    float mx = -INFINITY, team_mx = -INFINITY;
-    if (ACT == LMI_PROB_SOFTMAX || E.top) {
+    // a thread's own sums, group by group as the loads arrive: the exponentials of one run beside the loads of the next
+    float mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < N; ++e) mx = fmaxf(mx, G::get(p[e / V], e % V));   // drops NaN
+    for (int j = 0; j < J; ++j) {
+      float g = G::get(p[j], 0);
+#pragma unroll
+      for (int u = 1; u < V; ++u) g = fmaxf(g, G::get(p[j], u));   // drops NaN
+      mx = fmaxf(mx, g);
+      if (ACT == LMI_PROB_SOFTMAX) {
+        rebase(S, fmaxf(S.m, g));
+        const float ref = finite_ref(S.m);
+#pragma unroll
+        for (int u = 0; u < V; ++u) add_value(S, ref, G::get(p[j], u));
+      } else {
+#pragma unroll
+        for (int u = 0; u < V; ++u) S.t += answer_entropy<ACT>(G::get(p[j], u));
+      }
+    }
+    if (E.top) {
       if (NT > 64) {
         L.lane_max[wave][lane] = mx;
         if (t == 0) L.n = 0;
         __syncthreads();
-        float q = mx;
-        for (int w = 0; w < NT / 64; ++w) q = fmaxf(q, L.lane_max[w][lane]);
-        mx = q;   // of this lane in every wave
+        for (int w = 0; w < NT / 64; ++w) mx = fmaxf(mx, L.lane_max[w][lane]);   // of this lane in every wave
       } else if (t == 0) {
         L.n = 0;
       }
-      team_mx = reduce64(mx, MaxF());
-      if (E.top && wave == 0) {   // the top-th best of 64 lane maxima bounds the top-th best of all values from below
+      if (wave == 0) {   // the top-th best of 64 lane maxima bounds the top-th best of all values from below
         const float k = kth_of_lanes(mx, E.top);
         if (lane == 0) L.threshold = k;
       }
-    }
-    forget(p);
-    if (ACT == LMI_PROB_SOFTMAX) {
-      rebase(S, fmaxf(S.m, team_mx));
-      const float ref = finite_ref(S.m);
-#pragma unroll
-      for (int e = 0; e < N; ++e) add_value(S, ref, G::get(p[e / V], e % V));
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) S.t += answer_entropy<ACT>(G::get(p[e / V], e % V));
     }
     if (E.top) {
       team_sync<NT>();
@@ -438,14 +443,21 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
         thr = k != k ? INFINITY : fmaxf(thr, k);
       }
       forget(p);
+      const bool odd = S.t != S.t || (ACT == LMI_PROB_SOFTMAX && S.s != S.s);   // this thread has met a NaN, or an infinity that made one
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float v = G::get(p[e / V], e % V);
-        if (!(v < thr)) {   // NaN too
-          const long long c = first + (e / V) * (NT * V) + e % V;
-          if (c >= 0 && c < len) {
-            const int at = atomicAdd(&L.n, 1);
-            if (at < kCand) L.cand[at] = make_key(order_bits(v), (unsigned)(c0 + c));
+      for (int j = 0; j < J; ++j) {
+        float best = G::get(p[j], 0);
+#pragma unroll
+        for (int u = 1; u < V; ++u) best = fmaxf(best, G::get(p[j], u));
+        if (!(best < thr) || odd) {   // few groups
+#pragma unroll
+          for (int u = 0; u < V; ++u) {
+            const float v = G::get(p[j], u);
+            const long long c = first + j * (NT * V) + u;
+            if (!(v < thr) && c >= 0 && c < len) {   // NaN too
+              const int at = atomicAdd(&L.n, 1);
+              if (at < kCand) L.cand[at] = make_key(order_bits(v), (unsigned)(c0 + c));
+            }
           }
         }
       }
@@ -460,26 +472,31 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
           return make_key(order_bits(to_float(xp[c * (V > 1 ? 1 : E.cs)])), (unsigned)(c0 + c));
         }, (int)(hi - lo), t, E.top);
       }
-    } else if (NT > 64) {
-      __syncthreads();   // lane_max is written again by the next tile
     }
   }
-  // sums over the team
-  S.s = reduce64(S.s, SumF());
+  // sums over the wave, then over the team
+  if (ACT == LMI_PROB_SOFTMAX) {
+    rebase(S, reduce64(S.m, MaxF()));
+    S.s = reduce64(S.s, SumF());
+  }
   S.t = reduce64(S.t, SumF());
   if (NT > 64) {
     if (lane == 0) {
-      L.red[wave][0] = S.s;
-      L.red[wave][1] = S.t;
+      L.red[wave][0] = S.m;
+      L.red[wave][1] = S.s;
+      L.red[wave][2] = S.t;
     }
     __syncthreads();
-    S.s = S.t = 0.0f;
-    for (int w = 0; w < NT / 64; ++w) {
-      S.s += L.red[w][0];
-      S.t += L.red[w][1];
+    if (wave) return;
+    Sums W = {-INFINITY, 0.0f, 0.0f};
+    if (lane < NT / 64) W = Sums{L.red[lane][0], L.red[lane][1], L.red[lane][2]};
+    if (ACT == LMI_PROB_SOFTMAX) {
+      rebase(W, reduce64(W.m, MaxF()));
+      W.s = reduce64(W.s, SumF());
     }
+    W.t = reduce64(W.t, SumF());
+    S = W;
   }
-  if (wave) return;
   if (E.parts > 1) {
     unsigned char *out = E.ws + (row * E.parts + part) * (sizeof(PartHead) + (long long)kMaxTop * 8);
     if (lane == 0) *(PartHead *)out = PartHead{S.m, S.s, S.t, 0.0f};
@@ -517,7 +534,7 @@ __global__ __launch_bounds__(256) void evidence_join_kernel(const Evidence E) {
   __shared__ TeamShared<256> L;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const long long row = blockIdx.x;   // fewer than 128 of them
-  const long long o = row / E.n1, m = row - o * E.n1;
+  const long long o = (unsigned)row / (unsigned)E.n1, m = row - o * E.n1;
   if (E.count && m >= E.count[o]) return;
   const long long i = E.index ? E.index[row] : m;
   if (E.index && (i < 0 || i >= E.index_range)) return;   // written by the parts
@@ -593,13 +610,24 @@ template <int KT> __device__ __forceinline__ void insert(float (&val)[KT], int (
   }
 }
 
+// the two best so far, best first; no branch (almost every element of a wave's 64 rows enters some list)
+__device__ __forceinline__ void insert2(float (&val)[2], int (&cls)[2], float v, int c) {
+  // masks instead of conditions: the compiler makes branches of these
+  const int first = -(int)(v > val[0]), second = -(int)(v > val[1]);
+  const int next = (c & second) | (cls[1] & ~second);
+  val[1] = __builtin_amdgcn_fmed3f(v, val[0], val[1]);
+  cls[1] = (cls[0] & first) | (next & ~first);
+  val[0] = fmaxf(val[0], v);
+  cls[0] = (c & first) | (cls[0] & ~first);
+}
+
 // R rows side by side per thread, read as one word.  The lists are kept by float comparisons; a row that holds a NaN (or an
 // infinity that made one) is gone through again in the order that puts NaN first.
 template <typename T, int ACT, int KT, int R>
 __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) {
   const long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * R;
   if (first >= E.n0 * E.n1) return;
-  const long long o = first / E.n1, i0 = first - o * E.n1;   // R divides n1: the rows share o
+  const long long o = (unsigned)first / (unsigned)E.n1, i0 = first - o * E.n1;   // fewer than 2^31 rows: a 64-bit division costs as much as four classes   // R divides n1: the rows share o
   const T *x = (const T *)E.x + o * E.s0 + i0 * E.s1;
   typedef typename Group<T, R>::type W;
   Sums S[R];
@@ -612,18 +640,26 @@ __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) 
 #pragma unroll
     for (int k = 0; k < KT; ++k) val[r][k] = NAN, cls[r][k] = -1;
   }
-  constexpr int U = 8;
+  constexpr int U = KT <= 2 ? 16 : 8;   // loads in flight, and values per update of m
   const int C = (int)E.classes;
-  for (int c = 0; c < C; c += U) {
+  if constexpr (KT == 2) {   // the two best of class 0 and nothing else: what equals -inf after it comes in class order
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      val[r][0] = to_float(x[r * E.s1]), cls[r][0] = 0;
+      val[r][1] = -INFINITY, cls[r][1] = 1;
+    }
+  }
+  auto take = [&](int c, auto all) {   // U classes from c on, or those of them below C
+    constexpr bool kAll = decltype(all)::value;
     W w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (c + u < C) w[u] = *(const W *)(x + (long long)(c + u) * E.cs);
+      if (kAll || c + u < C) w[u] = *(const W *)(x + (long long)(c + u) * E.cs);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = c + u < C ? Group<T, R>::get(w[u], r) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
+      for (int u = 0; u < U; ++u) v[u] = kAll || c + u < C ? Group<T, R>::get(w[u], r) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
       if (ACT == LMI_PROB_SOFTMAX) {
         float mx = S[r].m;
 #pragma unroll
@@ -636,29 +672,56 @@ __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) 
 #pragma unroll
         for (int u = 0; u < U; ++u) S[r].t += answer_entropy<ACT>(v[u]);
       }
-      if (KT) {
+      if constexpr (KT == 2) {
+        if (c > 0) insert2(val[r], cls[r], v[0], c);
+#pragma unroll
+        for (int u = 1; u < U; ++u)
+          if (kAll || c + u < C) insert2(val[r], cls[r], v[u], c + u);
+      } else if constexpr (KT > 0) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (c + u < C && !(v[u] <= val[r][KL - 1])) insert<KL>(val[r], cls[r], v[u], c + u);
+          if ((kAll || c + u < C) && !(v[u] <= val[r][KL - 1])) insert<KL>(val[r], cls[r], v[u], c + u);
       }
+    }
+  };
+  int c = 0;
+  for (; c + U <= C; c += U) take(c, std::true_type());
+  if (c < C) take(c, std::false_type());
+  float ref[R], log_s[R], h[R], lp[R], best[R][KL];
+  bool plain = true;   // both rows are written, neither holds a NaN
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    ref[r] = log_s[r] = 0.0f;
+    h[r] = S[r].t;
+    if (ACT == LMI_PROB_SOFTMAX) softmax_result(S[r], ref[r], log_s[r], h[r]);
+    lp[r] = NAN;
+    if (E.labels) {
+      const long long l = label_of(E, o, i0 + r);
+      if (l >= 0 && l < C) lp[r] = log_prob<ACT>(to_float(x[r * E.s1 + l * E.cs]), ref[r], log_s[r]);
+    }
+#pragma unroll
+    for (int k = 0; k < KT; ++k) best[r][k] = log_prob<ACT>(val[r][k], ref[r], log_s[r]);
+    if ((E.count && i0 + r >= E.count[o]) || h[r] != h[r]) plain = false;
+  }
+  if constexpr (R == 2 && KT == 2) {   // a word of either output per thread: whole lines leave at once
+    if (E.wide && plain) {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+      typedef float f4 __attribute__((ext_vector_type(4)));
+      typedef int i4 __attribute__((ext_vector_type(4)));
+      *(f2 *)(E.entropy + first) = f2{h[0], h[1]};
+      if (E.logprob) *(f2 *)(E.logprob + first) = f2{lp[0], lp[1]};
+      *(f4 *)(E.top_logprob + first * 2) = f4{best[0][0], best[0][1], best[1][0], best[1][1]};
+      *(i4 *)(E.top_index + first * 2) = i4{cls[0][0], cls[0][1], cls[1][0], cls[1][1]};
+      return;
     }
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const long long row = first + r, i = i0 + r;
-    if (E.count && i >= E.count[o]) continue;
-    float ref = 0.0f, log_s = 0.0f, h = S[r].t;
-    if (ACT == LMI_PROB_SOFTMAX) softmax_result(S[r], ref, log_s, h);
-    if (E.entropy) E.entropy[row] = h;
-    if (E.logprob) {
-      float lp = NAN;
-      if (E.labels) {
-        const long long l = label_of(E, o, i);
-        if (l >= 0 && l < C) lp = log_prob<ACT>(to_float(x[r * E.s1 + l * E.cs]), ref, log_s);
-      }
-      E.logprob[row] = lp;
-    }
-    if (KT && h != h) {   // first the NaNs by class, then the others
+    const long long row = first + r;
+    if (E.count && i0 + r >= E.count[o]) continue;
+    if (E.entropy) E.entropy[row] = h[r];
+    if (E.logprob) E.logprob[row] = lp[r];
+    if (KT && h[r] != h[r]) {   // first the NaNs by class, then the others
       int n = 0;
       for (int c = 0; c < C && n < E.top; ++c) {
         const float v = to_float(x[r * E.s1 + (long long)c * E.cs]);
@@ -677,7 +740,7 @@ __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) 
 #pragma unroll
       for (int k = 0; k < KT; ++k)
         if (n + k < E.top) {
-          if (E.top_logprob) E.top_logprob[row * E.top + n + k] = log_prob<ACT>(val[r][k], ref, log_s);
+          if (E.top_logprob) E.top_logprob[row * E.top + n + k] = log_prob<ACT>(val[r][k], ref[r], log_s[r]);
           if (E.top_index) E.top_index[row * E.top + n + k] = cls[r][k];
         }
       continue;
@@ -685,7 +748,7 @@ __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) 
 #pragma unroll
     for (int k = 0; k < KT; ++k)
       if (k < E.top) {
-        if (E.top_logprob) E.top_logprob[row * E.top + k] = log_prob<ACT>(val[r][k], ref, log_s);
+        if (E.top_logprob) E.top_logprob[row * E.top + k] = best[r][k];
         if (E.top_index) E.top_index[row * E.top + k] = cls[r][k];
       }
   }
@@ -699,8 +762,10 @@ int split_parts(long long rows, long long classes) {
   return (int)(p < 64 ? p : 64);
 }
 
-template <typename T, int ACT, int KT> void launch_planes(const Evidence &E, hipStream_t st) {
+template <typename T, int ACT, int KT> void launch_planes(Evidence E, hipStream_t st) {
   const long long rows = E.n0 * E.n1;
+  E.wide = E.top == 2 && E.entropy && E.top_logprob && E.top_index && lmi_is_aligned(E.entropy, 8) && lmi_is_aligned(E.logprob, 8) &&
+           lmi_is_aligned(E.top_logprob, 16) && lmi_is_aligned(E.top_index, 16);
   if constexpr (sizeof(T) == 2 && KT <= 8) {   // two rows of a 16-bit type in one word
     if (E.s1 == 1 && E.n1 % 2 == 0 && E.cs % 2 == 0 && E.s0 % 2 == 0 && lmi_is_aligned(E.x, 4)) {
       evidence_planes_kernel<T, ACT, KT, 2><<<(unsigned)((rows / 2 + 255) / 256), 256, 0, st>>>(E);
@@ -804,6 +869,7 @@ int lmi_class_logprobs(const lmi_logprob_args *a, void *stream) {
   E.top_logprob = a->top_logprob;
   E.top_index = a->top_index;
   E.ws = (unsigned char *)a->workspace;
+  E.wide = 0;
   E.parts = 1;
   E.part_len = a->classes;
   hipStream_t st = (hipStream_t)stream;

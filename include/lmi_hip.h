@@ -514,7 +514,9 @@ int lmi_class_logprobs(const lmi_logprob_args *args, void *stream);
  *   element at b*x_batch + k*x_stride + p, y contiguous (batch, n, pixels).  x_stride, and the pixels of a plane, stay
  *   below 2^24.
  *   x_dtype LMI_MXFP4: x points at the packed blocks, x_scales at their scales (rows, batch 1, x_stride unused).
- *   y_dtype LMI_F32 | LMI_F16 | LMI_BF16, the type of x unless that is MXFP4.  bias [device] fp32 (n) or NULL.  workspace [device] of lmi_mx_product_workspace_bytes (0: none).
+ *   y_dtype LMI_F32 | LMI_F16 | LMI_BF16, the type of x unless that is MXFP4.  bias [device] fp32 (n) or NULL.
+ *   workspace [device] of lmi_mx_product_workspace_bytes, 16-byte aligned (0: none): float rows that meet many weight rows
+ *   are quantised into it first, with the same result.
  *   This is a 1x1 convolution of the network with its folded batch norm (bias) and SiLU.
  */
 enum lmi_mx_act { LMI_ACT_NONE = 0, LMI_ACT_SILU = 1 };

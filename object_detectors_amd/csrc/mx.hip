@@ -255,15 +255,11 @@ template <int BYTE> __device__ __forceinline__ void mfma2(f16x (&acc)[2], const 
 constexpr int kWaveSteps = 2;   // deeper ones stream faster: 64 x 192 -> 192 on 80 x 80: 80 us here, 68 streamed; 128 -> 640: 141 and 172; 48 -> 32 on 160 x 160: 56 and 84
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-template <typename T, bool PLANES> struct Raw;   // one step's values of a lane before they are quantised
-template <> struct Raw<float, true> {
-  f2 v[32];
-};
-template <typename T> struct Raw<T, true> {
+template <typename T> struct Raw {   // one step's values of a lane before they are quantised: two pixels of 32 channels
   unsigned v[32];
 };
-template <typename T> struct Raw<T, false> {
-  float v[8][8];
+template <> struct Raw<float> {
+  f2 v[32];
 };
 
 // Addresses are a base that is the same for the wave (scalar registers) plus a 32-bit offset of the lane: the launcher sees to it that
@@ -278,7 +274,7 @@ template <typename W> __device__ __forceinline__ const W *at_any(const void *bas
 
 // `in` channels (32 or more: all) of two neighbouring pixels from base + offset on; base is uniform
 template <typename T, bool SCALAR = true>
-__device__ __forceinline__ void load_planes(const T *base, unsigned offset, long long stride, bool live, int in, Raw<T, true> &r) {
+__device__ __forceinline__ void load_planes(const T *base, unsigned offset, long long stride, bool live, int in, Raw<T> &r) {
   typedef typename std::remove_reference<decltype(r.v[0])>::type W;
   if (live && in >= 32) {
 #pragma unroll
@@ -294,7 +290,7 @@ __device__ __forceinline__ void load_planes(const T *base, unsigned offset, long
   }
 }
 // the same value by value; `live` of the two pixels are there
-template <typename T> __device__ __forceinline__ void load_planes_single(const T *base, unsigned offset, long long stride, int live, int in, Raw<T, true> &r) {
+template <typename T> __device__ __forceinline__ void load_planes_single(const T *base, unsigned offset, long long stride, int live, int in, Raw<T> &r) {
   auto put = [&](int u, T a, T b) {
     if constexpr (sizeof(T) == 4) r.v[u] = f2{a, b};
     else r.v[u] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
@@ -323,7 +319,7 @@ template <typename T> __device__ __forceinline__ void load_planes_single(const T
     for (int u = 0; u < 32; ++u) put(u, (T)0.0f, (T)0.0f);
   }
 }
-__device__ __forceinline__ void quantize_raw(const Raw<float, true> &r, uint4 (&f)[2], unsigned (&byte)[2]) {
+__device__ __forceinline__ void quantize_raw(const Raw<float> &r, uint4 (&f)[2], unsigned (&byte)[2]) {
   float a[32];
 #pragma unroll
   for (int u = 0; u < 32; ++u) a[u] = r.v[u].x;
@@ -332,7 +328,7 @@ __device__ __forceinline__ void quantize_raw(const Raw<float, true> &r, uint4 (&
   for (int u = 0; u < 32; ++u) a[u] = r.v[u].y;
   f[1] = quantize_block(a, byte[1]);
 }
-template <typename T> __device__ __forceinline__ void quantize_raw(const Raw<T, true> &r, uint4 (&f)[2], unsigned (&byte)[2]) { quantize_pair16<T>(r.v, f, byte); }
+template <typename T> __device__ __forceinline__ void quantize_raw(const Raw<T> &r, uint4 (&f)[2], unsigned (&byte)[2]) { quantize_pair16<T>(r.v, f, byte); }
 
 // the sums of weight tile nt start at the bias
 __device__ __forceinline__ void start_sums(const Product &P, int nt, int lane, f16x (&acc)[2]) {
@@ -418,7 +414,7 @@ __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P,
   const int S = P.all_steps, half = lane >> 5;
   uint4 f[kWaveSteps][2];
   unsigned sw[2] = {};
-  Raw<T, true> raw;
+  Raw<T> raw;
 #pragma unroll
   for (int s = 0; s < kWaveSteps; ++s) {
     if (s < S) {
@@ -466,7 +462,7 @@ constexpr int kChunkTile = 128;
 template <typename T, bool PLANES, bool VEC> struct Chunk;   // what a thread holds of a chunk
 // planes: two neighbouring pixels x one block
 template <typename T, bool VEC> struct Chunk<T, true, VEC> {
-  Raw<T, true> raw;
+  Raw<T> raw;
   __device__ __forceinline__ void load(const Product &P, const T *x, int live, int chunk) {
     const int pair = threadIdx.x & 63;
     const long long c0 = (4ll * chunk + wave_id()) * 32;   // beyond k: in = 0
@@ -711,7 +707,7 @@ __device__ __forceinline__ void load_few(const Product &P, const T *x, long long
     const int in = (int)(P.k - c0 < 0 ? 0 : P.k - c0 < 32 ? P.k - c0 : 32);
     if constexpr (PLANES) {
       if (P.vec) {
-        Raw<T, true> raw;
+        Raw<T> raw;
         load_planes<T, false>(x + step * 64ll * P.xs1, (unsigned)((lane >> 5) * 32 * P.xs1 + 2 * j) * sizeof(T), P.xs1, 2 * j < live, in, raw);
         quantize_raw(raw, f, byte);
         return;
@@ -849,6 +845,28 @@ template <typename T> void dequantize(const void *packed, const void *scales, in
   mx_dequantize_kernel<<<(unsigned)(wanted < (1 << 23) ? wanted : (1 << 23)), 256, 0, st>>>((const unsigned *)packed, (const unsigned *)scales, rows, k, u.steps, units, vec, (T *)out);
 }
 
+// bytes of a quantised tensor's parts
+struct Sizes {
+  int64_t packed, scales;
+  Sizes(int64_t rows, int64_t k) {
+    const int64_t groups = (rows + 31) / 32, steps = (k + 63) / 64;
+    packed = groups * steps * 1024;
+    scales = groups * ((steps + 3) / 4) * 256;
+  }
+};
+
+// Rows that come as floats and meet many weight rows are quantised once, into the workspace, where they would be quantised again for
+// every 320 weight rows or fewer: 8192 x 1280 -> 2560 (fp16) 34 us, 59 without; 102400 x 640 -> 640 108 and 132; 128 x 1280 -> 32000 41 and
+// 156.  Few pairs of tiles (those that the waves of mx_few_kernel share in one round), 256 weight rows or k <= 128 do not
+// pay for the second kernel: 102400 x 1280 -> 160 98 us, 79 without; 8192 x 96 -> 640 11.4 and 9.9.
+constexpr int64_t kQuantiseN = 256, kQuantiseK = 128;
+bool quantise_first(const lmi_mx_product_args *a) {
+  if (a->layout != LMI_MX_ROWS || !float_type(a->x_dtype) || a->batch < 1 || a->n <= kQuantiseN || a->k <= kQuantiseK) return false;
+  if (a->batch > 1 && a->x_batch != a->pixels * a->x_stride) return false;   // the rows of the next image do not follow
+  if (a->batch >= (1 << 24) || a->pixels < 1 || a->pixels > (1 << 30) / a->batch || a->k >= (1 << 24)) return false;
+  return (a->batch * a->pixels + kTile - 1) / kTile * ((a->n + 31) / 32) >= kFewTilesPacked;
+}
+
 }  // namespace
 
 extern "C" {
@@ -883,7 +901,11 @@ int lmi_mx_dequantize(const uint8_t *packed, const uint8_t *scales, int64_t rows
   return lmi_check_launch("lmi_mx_dequantize");
 }
 
-int64_t lmi_mx_product_workspace_bytes(const lmi_mx_product_args *) { return 0; }
+int64_t lmi_mx_product_workspace_bytes(const lmi_mx_product_args *a) {
+  if (!a || !quantise_first(a)) return 0;
+  Sizes z(a->batch * a->pixels, a->k);
+  return z.packed + z.scales;
+}
 
 int lmi_mx_product(const lmi_mx_product_args *a, void *stream) {
   LMI_REQUIRE(a != nullptr, LMI_ERR_BAD_ARG, "lmi_mx_product: args is NULL");
@@ -920,9 +942,25 @@ int lmi_mx_product(const lmi_mx_product_args *a, void *stream) {
   P.all_steps = (int)((blocks + 1) / 2);
   P.tiles_n = (int)tiles_n;
   hipStream_t st = (hipStream_t)stream;
+  const bool first = quantise_first(a);
+  if (first) {
+    const int64_t m = a->batch * a->pixels;
+    const Sizes z(m, a->k);
+    LMI_REQUIRE(a->workspace && a->workspace_bytes >= z.packed + z.scales, LMI_ERR_WORKSPACE, "lmi_mx_product: workspace of %lld bytes, %lld needed",
+                (long long)a->workspace_bytes, (long long)(z.packed + z.scales));
+    LMI_REQUIRE(lmi_is_aligned(a->workspace, 16), LMI_ERR_ALIGNMENT, "lmi_mx_product: workspace must be 16-byte aligned");
+    uint8_t *packed = (uint8_t *)a->workspace, *scales = packed + z.packed;
+    const int e = lmi_mx_quantize(a->x, a->x_dtype, m, a->k, a->x_stride, packed, scales, stream);
+    if (e != LMI_OK) return e;
+    P.x = packed;
+    P.xs = (const unsigned *)scales;
+    P.pixels = m;
+  }
   if (a->x_dtype == LMI_MXFP4) {
     LMI_REQUIRE(rows && a->batch == 1 && a->x_scales && lmi_is_aligned(a->x, 16) && lmi_is_aligned(a->x_scales, 4), LMI_ERR_BAD_ARG,
                 "lmi_mx_product: quantised x comes as 16-byte aligned rows with their scales, batch 1");
+  }
+  if (first || a->x_dtype == LMI_MXFP4) {
     if (a->y_dtype == LMI_F32) return launch_product<Packed, float, false>(P, a->act, 1, st);
     if (a->y_dtype == LMI_F16) return launch_product<Packed, _Float16, false>(P, a->act, 1, st);
     return launch_product<Packed, __bf16, false>(P, a->act, 1, st);

@@ -958,9 +958,9 @@ def _mx_product(what, x_ptr, x_scales, x_dtype, batch, pixels, k, x_batch, x_str
     return y
 
 
-def _mx_common(what, x, weight, act, k):
+def _mx_common(what, x, weight, bias, act, k):
     _need_mx(weight, "weight")
-    _no_gradient(what, x)
+    _no_gradient(what, x, bias)
     if len(weight.shape) != 2 or weight.shape[1] != k or weight.shape[0] < 1:
         raise ValueError(f"{what}: weight {tuple(weight.shape)} does not fit inputs of {k} channels (out, in)")
     if weight.device != x.device:
@@ -969,11 +969,15 @@ def _mx_common(what, x, weight, act, k):
         raise ValueError(f"{what}: unknown activation {act!r} (None or 'silu')")
 
 
-def _mx_out(what, out, shape, dtype, device, memory_format=torch.contiguous_format):
+def _mx_out(what, out, x, shape, dtype, memory_format=torch.contiguous_format):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device, memory_format=memory_format)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device or not out.is_contiguous(memory_format=memory_format):
+        return torch.empty(shape, dtype=dtype, device=x.device, memory_format=memory_format)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != x.device or not out.is_contiguous(memory_format=memory_format):
         raise ValueError(f"{what}: `out` must be a {dtype} tensor of shape {tuple(shape)} in {memory_format} on x's device")
+    for t in (x.packed, x.scales) if isinstance(x, MxTensor) else (x,):   # every result needs whole rows of x, which others overwrite by then
+        first, last = t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+        if t.numel() and out.numel() and first < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < last:
+            raise ValueError(f"{what}: `out` lies in the memory of x")
     return out
 
 
@@ -998,8 +1002,8 @@ def mx_linear(x: Union[torch.Tensor, MxTensor], weight: MxTensor, bias: Optional
     if not len(x.shape):
         raise ValueError("mx_linear: x must be (..., k)")
     k = x.shape[-1]
-    _mx_common("mx_linear", x.packed if quantised else x, weight, act, k)
-    y = _mx_out("mx_linear", out, tuple(x.shape[:-1]) + (weight.shape[0],), dtype, x.device)
+    _mx_common("mx_linear", x.packed if quantised else x, weight, bias, act, k)
+    y = _mx_out("mx_linear", out, x, tuple(x.shape[:-1]) + (weight.shape[0],), dtype)
     m = math.prod(x.shape[:-1])
     if quantised:
         return _mx_product("mx_linear", x.packed.data_ptr(), x.scales.data_ptr(), _lib.LMI_MXFP4, 1, m, k, 0, 0, weight, bias, act, y, _lib.LMI_MX_ROWS)
@@ -1023,7 +1027,7 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
     if x.ndim != 4:
         raise ValueError("mx_pointwise: x must be (B, k, H, W)")
     b, k, h, w = x.shape
-    _mx_common("mx_pointwise", x, weight, act, k)
+    _mx_common("mx_pointwise", x, weight, bias, act, k)
     n = weight.shape[0]
     sb, sk, sh, sw = x.stride()
     planes = (w == 1 or sw == 1) and (h == 1 or sh == w * (sw if w > 1 else 1)) and h * w > 1
@@ -1035,10 +1039,10 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
         sb, sk, sh, sw = x.stride()
         planes = h * w > 1
     if planes:
-        y = _mx_out("mx_pointwise", out, (b, n, h, w), x.dtype, x.device)
+        y = _mx_out("mx_pointwise", out, x, (b, n, h, w), x.dtype)
         return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], b, h * w, k, sb, sk, weight, bias, act, y, _lib.LMI_MX_PLANES)
     fmt = torch.channels_last if h * w > 1 else torch.contiguous_format   # one pixel: both are the same memory
-    y = _mx_out("mx_pointwise", out, (b, n, h, w), x.dtype, x.device, fmt)
+    y = _mx_out("mx_pointwise", out, x, (b, n, h, w), x.dtype, fmt)
     if h * w == 1:       # an image per row
         return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], 1, b, k, 0, sb, weight, bias, act, y, _lib.LMI_MX_ROWS)
     return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], b, h * w, k, sb, sw if w > 1 else sh, weight, bias, act, y,

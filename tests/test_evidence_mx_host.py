@@ -91,6 +91,10 @@ def test_mx_arguments(L):
                 dict(x_dtype=6, x_scales=4096, layout=1)):
         assert _product(L, **bad) == -1, bad
     assert _product(L, w_packed=4104) == -2
+    many = dict(pixels=4096, k=512, n=512, x_stride=512)          # quantised into the workspace first: it has to be there
+    need = 4096 * 512 // 2 + 4096 * 512 // 32
+    assert _product(L, **many) == -3 and _product(L, **many, workspace=4096, workspace_bytes=need - 1) == -3
+    assert _product(L, **many, workspace=4104, workspace_bytes=need) == -2
     assert _product(L, x_stride=1 << 24) == -4 and _product(L, layout=1, pixels=1 << 24) == -4 and _product(L, pixels=1 << 40) == -4
 
 

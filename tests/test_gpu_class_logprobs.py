@@ -249,6 +249,53 @@ def test_two_streams_agree():
             assert all(torch.equal(r[k], want[i][k]) for k in r)
 
 
+def test_graphs_side_by_side():
+    """Two captured graphs of long rows, whose parts are joined through workspaces, replayed at the same time on two streams."""
+    ops = _ops()
+    data = [_rows(s, 2, 70001, torch.float16, "softmax") for s in (1, 2)]
+    graphs, res = [], []
+    for x, l in data:
+        ops.class_logprobs(x, l, top=4)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res.append([ops.class_logprobs(x, l, top=4) for _ in range(4)])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in data]
+    for i in range(3):
+        for x, _ in data:
+            x.copy_(torch.randn(2, 70001) * (i + 1))
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for (x, l), several in zip(data, res):
+            want = ops.class_logprobs(x, l, top=4)
+            for r in several:
+                assert all(torch.equal(r[k], want[k]) for k in r)
+
+
+def test_count_beyond_the_rows_and_far_labels():
+    """count above M means all rows, below zero none; labels of 64 bits that a 32-bit reading would take for classes are none."""
+    ops = _ops()
+    x = torch.randn(4, 5, 9).cuda()
+    labels = torch.tensor([0, 2 ** 32, -2 ** 32 + 3, 8, 9], dtype=torch.int64).repeat(4, 1).cuda()
+    count = torch.tensor([99, 0, -3, 2], dtype=torch.int32).cuda()
+    full = ops.class_logprobs(x, labels, top=2)
+    assert torch.isnan(full["logprob"])[0].tolist() == [False, True, True, False, True]
+    out = {k: torch.full_like(v, 77) for k, v in full.items()}
+    ops.class_logprobs(x, labels, top=2, count=count, out=out)
+    for k, v in full.items():
+        for b, rows in enumerate((5, 0, 0, 2)):
+            assert torch.equal(out[k][b, :rows].nan_to_num(5), v[b, :rows].nan_to_num(5)) and (out[k][b, rows:] == 77).all()
+    planes = x.transpose(1, 2).contiguous().transpose(1, 2)               # the same rows, classes as planes
+    out = {k: torch.full_like(v, 77) for k, v in full.items()}
+    ops.class_logprobs(planes, labels, top=2, count=count, out=out)
+    for b, rows in enumerate((5, 0, 0, 2)):
+        assert torch.equal(out["top_index"][b, :rows], full["top_index"][b, :rows]) and all((t[b, rows:] == 77).all() for t in out.values())
+
+
 def test_refusals():
     ops = _ops()
     x = torch.randn(4, 6, 9).cuda()

@@ -196,6 +196,128 @@ def test_captured_and_replayed():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n,act", [(2100, 200, 333, "silu"), (1300, 160, 640, None), (130, 1000, 4000, None), (5000, 129, 257, "silu")])
+def test_many_rows_and_weights(m, k, n, act, dtype):
+    """Rows that are quantised once before the product: the same bits as from an MxTensor, whatever their stride and alignment."""
+    ops, dt = _ops(), DTYPES[dtype]
+    g = torch.Generator().manual_seed(m + n)
+    base = torch.randn(m, k + 11, generator=g).to(dt).cuda()
+    w = torch.randn(n, k, generator=g).cuda() / k ** 0.5
+    bias = torch.randn(n, generator=g).cuda()
+    wq = ops.mx_quantize(w)
+    for x in (base[:, 3:3 + k], base[:, :k].contiguous()):
+        y = ops.mx_linear(x, wq, bias, act=act)
+        want, size = OM.product(_np(x), _np(w), _np(bias), act)
+        _close(y, want, size, k, dt, act)
+        assert torch.equal(y, ops.mx_linear(ops.mx_quantize(x), wq, bias, act=act, dtype=dt))
+
+
+@pytest.mark.parametrize("step", [1, 2])
+def test_many_channels_last_images(step):
+    """Images whose rows follow each other, and every other image, whose rows do not."""
+    ops = _ops()
+    base = torch.randn(6, 192, 24, 26).half().cuda().contiguous(memory_format=torch.channels_last)
+    x = base[::step]
+    w = torch.randn(400, 192).cuda() / 14
+    want, size = OM.product(_np(x.permute(0, 2, 3, 1)).reshape(-1, 192), _np(w), None, "silu")
+    y = ops.mx_pointwise(x, ops.mx_quantize(w), act="silu")
+    assert y.is_contiguous(memory_format=torch.channels_last)
+    _close(y.permute(0, 2, 3, 1).reshape(-1, 400), want, size, 192, torch.float16, "silu")
+
+
+def _room(gb):
+    if torch.cuda.mem_get_info()[0] < gb << 30:
+        pytest.skip(f"needs {gb} GB")
+
+
+def test_far_rows():
+    """Inputs, quantised blocks and results beyond 2^32 bytes."""
+    _room(48)
+    ops = _ops()
+    k, m = 1 << 16, (1 << 17) + 40
+    x = torch.zeros(m, k, dtype=torch.float16, device="cuda")          # 17 GB, 4.3 GB of blocks
+    x[-9:].copy_(torch.randn(9, k))
+    want = OM.values(_np(x[-9:]))
+    q = ops.mx_quantize(x)
+    y = ops.mx_dequantize(q, torch.float16)
+    assert np.array_equal(_np(y[-9:]), want) and not y[-100:-9].any()
+    ones = ops.mx_quantize(torch.ones(1, k, device="cuda"))            # sums of rows
+    for z in (ops.mx_linear(q, ones), ops.mx_linear(x, ones)):
+        _close(z[-9:], want.sum(1, keepdims=True), np.abs(want).sum(1, keepdims=True), k, z.dtype, None)
+        assert not z[:-9].any()
+
+
+def test_far_results():
+    _room(16)
+    ops = _ops()
+    x, w = torch.randn(40000, 70).half().cuda(), torch.randn((1 << 16) + 8, 70).cuda()
+    y = ops.mx_linear(x, ops.mx_quantize(w))                            # 5.2 GB
+    want, size = OM.product(_np(x[-4:]), _np(w[-70:]))
+    _close(y[-4:, -70:], want, size, 70, torch.float16, None)
+
+
+def test_far_maps():
+    """Planes and images beyond 2^32 bytes."""
+    _room(32)
+    ops = _ops()
+    x = torch.zeros(9, 640, 700, 702, dtype=torch.float16, device="cuda")   # 5.7 GB
+    x[-1].copy_(torch.randn(640, 700, 702))
+    w = torch.randn(8, 640).cuda() / 25
+    y = ops.mx_pointwise(x, ops.mx_quantize(w))
+    part = _np(x[-1, :, -2:]).reshape(640, -1).T
+    want, size = OM.product(part, _np(w))
+    _close(y[-1, :, -2:].reshape(8, -1).t(), want, size, 640, torch.float16, None)
+    assert not y[:-1].any()
+    big = torch.randn(1, 70, 2000, 2002).half().cuda()                     # channels 8 MB apart; 5.2 GB of results
+    wb = torch.randn(650, 70).cuda()
+    z = ops.mx_pointwise(big, ops.mx_quantize(wb))
+    want, size = OM.product(_np(big[0, :, -1]).T, _np(wb))
+    _close(z[0, :, -1].t(), want, size, 70, torch.float16, None)
+
+
+def test_graphs_side_by_side():
+    """Two captured graphs of products with workspaces, replayed at the same time on two streams."""
+    ops = _ops()
+    wq = ops.mx_quantize(torch.randn(640, 320).cuda())
+    xs = [torch.randn(3000, 320).half().cuda() for _ in range(2)]
+    for x in xs:
+        ops.mx_linear(x, wq)
+    torch.cuda.synchronize()
+    graphs, res = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res.append([ops.mx_linear(x, wq, act="silu") for _ in range(4)])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in xs]
+    for i in range(3):
+        for x in xs:
+            x.copy_(torch.randn(3000, 320))
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for x, r in zip(xs, res):
+            want = ops.mx_linear(x, wq, act="silu")
+            assert all(torch.equal(t, want) for t in r)
+
+
+def test_out_over_x_is_refused():
+    ops = _ops()
+    wq = ops.mx_quantize(torch.randn(64, 64).cuda())
+    x, m = torch.randn(10, 64).cuda(), torch.randn(2, 64, 4, 4).cuda()
+    cl = m.contiguous(memory_format=torch.channels_last)
+    for call in (lambda: ops.mx_linear(x, wq, out=x), lambda: ops.mx_linear(x[:6], wq, out=x[4:]), lambda: ops.mx_pointwise(m, wq, out=m),
+                 lambda: ops.mx_pointwise(cl, wq, out=cl)):
+        with pytest.raises(ValueError, match="memory of x"):
+            call()
+    assert torch.equal(ops.mx_linear(x[:5], wq, out=x[5:]), ops.mx_linear(x[:5].clone(), wq))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.mx_linear(x, wq, torch.zeros(64, device="cuda", requires_grad=True))
+
+
 def test_refusals():
     ops = _ops()
     x, w = torch.randn(4, 64).cuda(), ops.mx_quantize(torch.randn(8, 64).cuda())

@@ -598,11 +598,11 @@ __global__ __launch_bounds__(256, sizeof(Y) == 2 && NT <= (PLANES ? 2 : 1) ? 3 :
 #pragma unroll
     for (int j = 0; j < NW; ++j) wsb[B][4 * j + wave][lane] = ws_reg[j];
     hold.template put<B>(xb[B], xs[B]);
-    __syncthreads();
     if (c + 1 < chunks) {
       load_part(c + 1, std::integral_constant<int, 1 - B>());
       hold.load(P, x, live, c + 1);
     }
+    __syncthreads();
     const unsigned sb0 = xs[B][2 * wp][lane], sb1 = xs[B][2 * wp + 1][lane];
     unsigned sa[NT];
 #pragma unroll

@@ -474,9 +474,9 @@ int64_t lmi_trace_contours_host(const uint64_t *words, int64_t m, const int32_t 
  * Outputs [device], any of them NULL if not wanted, contiguous: logprob (n0,n1), entropy (n0,n1) fp32; top_logprob fp32 and
  * top_index int32 (n0,n1,top), best first, equal values in the order of their classes, NaN before everything else.
  * 0 <= top <= min(classes, LMI_MAX_TOP).  `workspace` [device] of lmi_class_logprobs_workspace_bytes; none is needed below
- * LMI_LOGPROB_SPLIT_FROM classes or from 128 rows on.
+ * LMI_LOGPROB_SPLIT_FROM classes or from 256 rows on.
  */
-#define LMI_LOGPROB_SPLIT_FROM 8193
+#define LMI_LOGPROB_SPLIT_FROM 16385
 enum lmi_prob_activation { LMI_PROB_SOFTMAX = 0, LMI_PROB_SIGMOID = 1, LMI_PROB_NONE = 2 };
 typedef struct lmi_logprob_args {
   const void *x;
@@ -493,7 +493,7 @@ typedef struct lmi_logprob_args {
   void *workspace;
   int64_t workspace_bytes;
 } lmi_logprob_args;
-int64_t lmi_class_logprobs_workspace_bytes(int64_t rows, int64_t classes, int64_t class_stride, int top);
+int64_t lmi_class_logprobs_workspace_bytes(int64_t rows, int64_t classes, int64_t class_stride, int x_dtype);
 int lmi_class_logprobs(const lmi_logprob_args *args, void *stream);
 
 /* ------------------------------------------------------------------------------------------

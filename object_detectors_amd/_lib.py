@@ -52,7 +52,7 @@ class lmi_point_op(C.Structure):
 
 LMI_PROB_SOFTMAX, LMI_PROB_SIGMOID, LMI_PROB_NONE = 0, 1, 2
 LMI_MAX_TOP = 32
-LMI_LOGPROB_SPLIT_FROM = 8193
+LMI_LOGPROB_SPLIT_FROM = 16385
 
 
 class lmi_logprob_args(C.Structure):

@@ -19,8 +19,7 @@
 //                          lane maxima is a lower bound of the answer; what reaches it (a few dozen of thousands) goes to LDS and
 //                          is ranked there by counting.
 //  evidence_join_kernel    joins the parts of long rows, the same way.
-//  evidence_planes_kernel  one thread per row (16-bit types: two), for rows that lie side by side (class planes): a wave reads
-//                          neighbouring rows' values of one class at a time; the alternatives sit in registers.
+//  evidence_planes_kernel  one thread per row, for many rows that lie side by side (class planes); the alternatives sit in registers.
 #include <hip/hip_fp16.h>
 
 #include <type_traits>
@@ -41,7 +40,7 @@ struct Evidence {
   float *logprob, *entropy, *top_logprob;
   int *top_index;
   unsigned char *ws;
-  int wide;            // the outputs of two rows may be written as one word (planes kernel, top 2)
+  int pairs;           // a row's two alternatives may be written as one word (planes kernel)
   int parts;           // parts per row (rows kernel)
   long long part_len;  // classes per part
 };
@@ -268,22 +267,24 @@ __device__ __forceinline__ void store_nan(const Evidence &E, long long row, int 
   }
 }
 
-// 16 lanes per row, class j * 16 + l in value j of lane l
+// 16 lanes per row, class j * 16 + l in value j of lane l.  64 x 300 kept rows of 80 classes (fp32, an anchor plane apart): 28.6 us
+// for 1.1 million scattered sectors of 64 bytes, 2.6 TB/s of what DRAM moves for them; one image's 300 rows: 6.7 us, two
+// dependent loads and the arithmetic of one wave.  A wave per row took 52 and 17 us: fewer rows, and so sectors, in flight.
 template <typename T, int J, int ACT>
-__global__ __launch_bounds__(256) void evidence_team_kernel(const Evidence E, long long rows) {
+__device__ __forceinline__ void evidence_team(const Evidence &E, long long row, long long rows) {
   const int l = threadIdx.x & 15, group = (threadIdx.x & 63) >> 4;
-  const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
   bool on = row < rows;
-  const long long o = on ? (unsigned)row / (unsigned)E.n1 : 0, m = on ? row - o * E.n1 : 0;
-  if (on && E.count && m >= E.count[o]) on = false;
-  long long i = m;
-  if (on && E.index) {
-    i = E.index[row];
-    if (i < 0 || i >= E.index_range) {
-      store_nan(E, row, l);
-      on = false;
-    }
+  const long long at = on ? row : 0, o = (unsigned)at / (unsigned)E.n1, m = at - o * E.n1;
+  // count, index and label are on their way together: one latency instead of three (64 x 300 rows of 80 classes: 31.5 -> 29.1 us)
+  const int count = E.count ? E.count[o] : 0;
+  long long i = E.index ? E.index[at] : m;
+  long long label = E.labels ? label_of(E, o, m) : -1;
+  if (E.count && m >= count) on = false;
+  if (on && E.index && (i < 0 || i >= E.index_range)) {
+    store_nan(E, row, l);
+    on = false;
   }
+  if (!on) i = 0;
   const T *x = (const T *)E.x + o * E.s0 + i * E.s1;
   const int C = (int)E.classes;
   float v[J];
@@ -292,13 +293,11 @@ __global__ __launch_bounds__(256) void evidence_team_kernel(const Evidence E, lo
     const int c = j * 16 + l;
     v[j] = on && c < C ? to_float(x[c * E.cs]) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
   }
-  long long label = -1;
-  float lx = 0.0f;
-  if (on && E.labels && l == 0) {
-    label = label_of(E, o, m);
-    if (label >= C) label = -1;
-    if (label >= 0) lx = to_float(x[label * E.cs]);
-  }
+  if (label >= C) label = -1;
+  float lx = 0.0f;   // the label's value, from the lane that has it
+#pragma unroll
+  for (int j = 0; j < J; ++j) lx = label >> 4 == j ? v[j] : lx;
+  lx = __shfl(lx, (int)label & 15, 16);
   float ref = 0.0f, log_s = 0.0f, h = 0.0f;
   if (ACT == LMI_PROB_SOFTMAX) {
     float mx = v[0];
@@ -344,10 +343,19 @@ __global__ __launch_bounds__(256) void evidence_team_kernel(const Evidence E, lo
   }
 }
 
+template <typename T, int J, int ACT>
+__global__ __launch_bounds__(256) void evidence_team_kernel(const Evidence E, long long rows) {
+  for (long long first = (long long)blockIdx.x * 16; first < rows; first += (long long)gridDim.x * 16)   // more rows than a grid holds: several each
+    evidence_team<T, J, ACT>(E, first + (threadIdx.x >> 4), rows);
+}
+
 struct alignas(16) PartHead {
   float m, s, t, pad;
 };
 
+// 511 rows of 32001 classes (bf16, top 10): 17.1 us, 1.9 TB/s -- every workgroup's row is in registers at once (two per CU, all of them
+// resident), so it is the sum of loading (5.3 us), some 11 vector instructions a value (5) and the tail from the row's threshold to its
+// ranked list (5): the two rows of a CU run in step.  2 rows of 200001 (fp32, top 20) in 25 parts: 16.
 // V > 1: classes lie side by side and are read in aligned 16-byte groups (the row may start anywhere; the groups at its two ends
 // are read value by value).  V == 1: any class stride.
 template <typename T, int V> struct Group {
@@ -533,7 +541,7 @@ template <typename T, int ACT>
 __global__ __launch_bounds__(256) void evidence_join_kernel(const Evidence E) {
   __shared__ TeamShared<256> L;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const long long row = blockIdx.x;   // fewer than 128 of them
+  const long long row = blockIdx.x;   // fewer than 256 of them
   const long long o = (unsigned)row / (unsigned)E.n1, m = row - o * E.n1;
   if (E.count && m >= E.count[o]) return;
   const long long i = E.index ? E.index[row] : m;
@@ -621,186 +629,160 @@ __device__ __forceinline__ void insert2(float (&val)[2], int (&cls)[2], float v,
   cls[0] = (c & first) | (cls[0] & ~first);
 }
 
-// R rows side by side per thread, read as one word.  The lists are kept by float comparisons; a row that holds a NaN (or an
-// infinity that made one) is gone through again in the order that puts NaN first.
-template <typename T, int ACT, int KT, int R>
+// A thread per row, for rows side by side: a wave reads neighbouring rows' values of one class at a time.  The lists are kept by float
+// comparisons; a row that holds a NaN (or an infinity that made one) is gone through again in the order that puts NaN first.
+// 64 x 4 x 8400 rows of 16 bins (fp16, top 2): 32.9 us, 4.2 TB/s of 138 MB; the instructions that keep two best beside the softmax
+// take as long as the loads.  Two rows of a 16-bit type per thread, read as one word, halve the loads and the threads: no better here
+// (35.8 us) and worse for longer lists (64 x 8400 x 80, top 5: 90 us, 71 with one).
+template <typename T, int ACT, int KT>
 __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) {
-  const long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * R;
-  if (first >= E.n0 * E.n1) return;
-  const long long o = (unsigned)first / (unsigned)E.n1, i0 = first - o * E.n1;   // fewer than 2^31 rows: a 64-bit division costs as much as four classes   // R divides n1: the rows share o
-  const T *x = (const T *)E.x + o * E.s0 + i0 * E.s1;
-  typedef typename Group<T, R>::type W;
-  Sums S[R];
+  const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (row >= E.n0 * E.n1) return;
+  const long long o = (unsigned)row / (unsigned)E.n1, i = row - o * E.n1;   // fewer than 2^31 rows: a 64-bit division costs as much as four classes
+  if (E.count && i >= E.count[o]) return;
+  const T *x = (const T *)E.x + o * E.s0 + i * E.s1;
+  Sums S = {-INFINITY, 0.0f, 0.0f};
   constexpr int KL = KT ? KT : 1;
-  float val[R][KL];
-  int cls[R][KL];
+  float val[KL];
+  int cls[KL];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    S[r] = Sums{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < KT; ++k) val[r][k] = NAN, cls[r][k] = -1;
-  }
+  for (int k = 0; k < KT; ++k) val[k] = NAN, cls[k] = -1;
   constexpr int U = KT <= 2 ? 16 : 8;   // loads in flight, and values per update of m
   const int C = (int)E.classes;
   if constexpr (KT == 2) {   // the two best of class 0 and nothing else: what equals -inf after it comes in class order
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      val[r][0] = to_float(x[r * E.s1]), cls[r][0] = 0;
-      val[r][1] = -INFINITY, cls[r][1] = 1;
-    }
+    val[0] = to_float(x[0]), cls[0] = 0;
+    val[1] = -INFINITY, cls[1] = 1;
   }
   auto take = [&](int c, auto all) {   // U classes from c on, or those of them below C
     constexpr bool kAll = decltype(all)::value;
-    W w[U];
+    T w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (kAll || c + u < C) w[u] = *(const W *)(x + (long long)(c + u) * E.cs);
+      if (kAll || c + u < C) w[u] = x[(long long)(c + u) * E.cs];
+    float v[U];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float v[U];
+    for (int u = 0; u < U; ++u) v[u] = kAll || c + u < C ? to_float(w[u]) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
+    if (ACT == LMI_PROB_SOFTMAX) {
+      float mx = S.m;
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = kAll || c + u < C ? Group<T, R>::get(w[u], r) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
-      if (ACT == LMI_PROB_SOFTMAX) {
-        float mx = S[r].m;
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, v[u]);
+      rebase(S, mx);
+      const float ref = finite_ref(mx);
 #pragma unroll
-        for (int u = 0; u < U; ++u) mx = fmaxf(mx, v[u]);
-        rebase(S[r], mx);
-        const float ref = finite_ref(mx);
+      for (int u = 0; u < U; ++u) add_value(S, ref, v[u]);
+    } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) add_value(S[r], ref, v[u]);
-      } else {
+      for (int u = 0; u < U; ++u) S.t += answer_entropy<ACT>(v[u]);
+    }
+    if constexpr (KT == 2) {
+      if (c > 0) insert2(val, cls, v[0], c);
 #pragma unroll
-        for (int u = 0; u < U; ++u) S[r].t += answer_entropy<ACT>(v[u]);
-      }
-      if constexpr (KT == 2) {
-        if (c > 0) insert2(val[r], cls[r], v[0], c);
+      for (int u = 1; u < U; ++u)
+        if (kAll || c + u < C) insert2(val, cls, v[u], c + u);
+    } else if constexpr (KT > 0) {
 #pragma unroll
-        for (int u = 1; u < U; ++u)
-          if (kAll || c + u < C) insert2(val[r], cls[r], v[u], c + u);
-      } else if constexpr (KT > 0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if ((kAll || c + u < C) && !(v[u] <= val[r][KL - 1])) insert<KL>(val[r], cls[r], v[u], c + u);
-      }
+      for (int u = 0; u < U; ++u)
+        if ((kAll || c + u < C) && !(v[u] <= val[KL - 1])) insert<KL>(val, cls, v[u], c + u);
     }
   };
   int c = 0;
   for (; c + U <= C; c += U) take(c, std::true_type());
   if (c < C) take(c, std::false_type());
-  float ref[R], log_s[R], h[R], lp[R], best[R][KL];
-  bool plain = true;   // both rows are written, neither holds a NaN
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    ref[r] = log_s[r] = 0.0f;
-    h[r] = S[r].t;
-    if (ACT == LMI_PROB_SOFTMAX) softmax_result(S[r], ref[r], log_s[r], h[r]);
-    lp[r] = NAN;
-    if (E.labels) {
-      const long long l = label_of(E, o, i0 + r);
-      if (l >= 0 && l < C) lp[r] = log_prob<ACT>(to_float(x[r * E.s1 + l * E.cs]), ref[r], log_s[r]);
+  float ref = 0.0f, log_s = 0.0f, h = S.t;
+  if (ACT == LMI_PROB_SOFTMAX) softmax_result(S, ref, log_s, h);
+  if (E.entropy) E.entropy[row] = h;
+  if (E.logprob) {
+    const long long l = E.labels ? label_of(E, o, i) : -1;
+    E.logprob[row] = l >= 0 && l < C ? log_prob<ACT>(to_float(x[l * E.cs]), ref, log_s) : NAN;
+  }
+  int n = 0;
+  if (KT && h != h) {   // first the NaNs by class, then the others
+    for (int c = 0; c < C && n < E.top; ++c) {
+      const float v = to_float(x[(long long)c * E.cs]);
+      if (v != v) {
+        if (E.top_logprob) E.top_logprob[row * E.top + n] = NAN;
+        if (E.top_index) E.top_index[row * E.top + n] = c;
+        ++n;
+      }
     }
 #pragma unroll
-    for (int k = 0; k < KT; ++k) best[r][k] = log_prob<ACT>(val[r][k], ref[r], log_s[r]);
-    if ((E.count && i0 + r >= E.count[o]) || h[r] != h[r]) plain = false;
+    for (int k = 0; k < KT; ++k) val[k] = NAN, cls[k] = -1;
+    for (int c = 0; c < C; ++c) {
+      const float v = to_float(x[(long long)c * E.cs]);
+      if (v == v && !(v <= val[KL - 1])) insert<KL>(val, cls, v, c);
+    }
   }
-  if constexpr (R == 2 && KT == 2) {   // a word of either output per thread: whole lines leave at once
-    if (E.wide && plain) {
+  if constexpr (KT == 2) {
+    if (E.pairs && n == 0) {   // a row's two results as one word
       typedef float f2 __attribute__((ext_vector_type(2)));
-      typedef float f4 __attribute__((ext_vector_type(4)));
-      typedef int i4 __attribute__((ext_vector_type(4)));
-      *(f2 *)(E.entropy + first) = f2{h[0], h[1]};
-      if (E.logprob) *(f2 *)(E.logprob + first) = f2{lp[0], lp[1]};
-      *(f4 *)(E.top_logprob + first * 2) = f4{best[0][0], best[0][1], best[1][0], best[1][1]};
-      *(i4 *)(E.top_index + first * 2) = i4{cls[0][0], cls[0][1], cls[1][0], cls[1][1]};
+      typedef int i2 __attribute__((ext_vector_type(2)));
+      *(f2 *)(E.top_logprob + row * 2) = f2{log_prob<ACT>(val[0], ref, log_s), log_prob<ACT>(val[1], ref, log_s)};
+      *(i2 *)(E.top_index + row * 2) = i2{cls[0], cls[1]};
       return;
     }
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const long long row = first + r;
-    if (E.count && i0 + r >= E.count[o]) continue;
-    if (E.entropy) E.entropy[row] = h[r];
-    if (E.logprob) E.logprob[row] = lp[r];
-    if (KT && h[r] != h[r]) {   // first the NaNs by class, then the others
-      int n = 0;
-      for (int c = 0; c < C && n < E.top; ++c) {
-        const float v = to_float(x[r * E.s1 + (long long)c * E.cs]);
-        if (v != v) {
-          if (E.top_logprob) E.top_logprob[row * E.top + n] = NAN;
-          if (E.top_index) E.top_index[row * E.top + n] = c;
-          ++n;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < KT; ++k) val[r][k] = NAN, cls[r][k] = -1;
-      for (int c = 0; c < C; ++c) {
-        const float v = to_float(x[r * E.s1 + (long long)c * E.cs]);
-        if (v == v && !(v <= val[r][KL - 1])) insert<KL>(val[r], cls[r], v, c);
-      }
-#pragma unroll
-      for (int k = 0; k < KT; ++k)
-        if (n + k < E.top) {
-          if (E.top_logprob) E.top_logprob[row * E.top + n + k] = log_prob<ACT>(val[r][k], ref[r], log_s[r]);
-          if (E.top_index) E.top_index[row * E.top + n + k] = cls[r][k];
-        }
-      continue;
+  for (int k = 0; k < KT; ++k)
+    if (n + k < E.top) {
+      if (E.top_logprob) E.top_logprob[row * E.top + n + k] = log_prob<ACT>(val[k], ref, log_s);
+      if (E.top_index) E.top_index[row * E.top + n + k] = cls[k];
     }
-#pragma unroll
-    for (int k = 0; k < KT; ++k)
-      if (k < E.top) {
-        if (E.top_logprob) E.top_logprob[row * E.top + k] = best[r][k];
-        if (E.top_index) E.top_index[row * E.top + k] = cls[r][k];
-      }
-  }
 }
 
-// parts per row: long rows of a batch too small to fill the chip are cut into parts of at least 4096 values, at most 64 (one
-// per lane of the joining wave)
-int split_parts(long long rows, long long classes) {
-  if (rows >= 128 || classes < LMI_LOGPROB_SPLIT_FROM) return 1;
-  const long long p = (classes + 4095) / 4096;
+// Parts per row.  A row of up to two tiles of a workgroup of 512 (fp32: 32704 values) is read by one, as fast as parts and their join
+// (16 x 32001 bf16: 11 us, 19 in parts of 4096); longer ones of a batch too small to fill the chip are cut into parts of about a tile of 256
+// threads, at most 64, one per lane of the joining wave
+// (in parts and in one piece, bf16: 2 x 70001 16 and 24 us, 16 x 200001 16 and 50, 100 x 70001 20 and 27, 255 x 70001 30 and 29; 2 x 200001 fp32 16 and 75)
+int split_parts(long long rows, long long classes, long long class_stride, int size) {
+  const long long unit = class_stride == 1 ? 255 * (128 / size) : 2 * 256 * 8;
+  if (rows >= 256 || classes < LMI_LOGPROB_SPLIT_FROM || classes <= 4 * unit) return 1;
+  const long long p = (classes + unit - 1) / unit;
   return (int)(p < 64 ? p : 64);
 }
 
 template <typename T, int ACT, int KT> void launch_planes(Evidence E, hipStream_t st) {
   const long long rows = E.n0 * E.n1;
-  E.wide = E.top == 2 && E.entropy && E.top_logprob && E.top_index && lmi_is_aligned(E.entropy, 8) && lmi_is_aligned(E.logprob, 8) &&
-           lmi_is_aligned(E.top_logprob, 16) && lmi_is_aligned(E.top_index, 16);
-  if constexpr (sizeof(T) == 2 && KT <= 8) {   // two rows of a 16-bit type in one word
-    if (E.s1 == 1 && E.n1 % 2 == 0 && E.cs % 2 == 0 && E.s0 % 2 == 0 && lmi_is_aligned(E.x, 4)) {
-      evidence_planes_kernel<T, ACT, KT, 2><<<(unsigned)((rows / 2 + 255) / 256), 256, 0, st>>>(E);
-      return;
-    }
-  }
-  evidence_planes_kernel<T, ACT, KT, 1><<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(E);
+  E.pairs = E.top == 2 && E.top_logprob && E.top_index && lmi_is_aligned(E.top_logprob, 8) && lmi_is_aligned(E.top_index, 8);
+  evidence_planes_kernel<T, ACT, KT><<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(E);
 }
+
+constexpr long long kMaxGrid = 1 << 22;   // workgroups: with their threads below 2^32
 
 template <typename T, int ACT> int launch(const Evidence &E0, hipStream_t st) {
   Evidence E = E0;
   const long long rows = E.n0 * E.n1;
-  // rows side by side and few classes each, or many rows: a thread per row
-  const bool planes = !E.index && E.classes <= 65536 && ((E.cs != 1 && E.s1 < E.cs && (rows >= 4096 || E.classes <= 64)) || E.classes <= 8);
+  // Rows side by side: a thread per row where there are enough of them for the chip, the more the longer their lists (fp16, us here and with 16
+  // lanes per row: 8400 x 80, top 2 6.9 and 5.9, top 5 28 and 7.5; 4 x 8400 x 80, top 2 7.9 and 12, top 5 24 and 15; 4 x 8400 x 40, top 5
+  // 11 and 13; 16 x 8400 x 80, top 5 35 and 40).  Lists of more than eight gain little at best (64 x 8400 x 64, top 20: 225 and 314, x 128
+  // 411 and 352).  Up to 8 classes always (64 x 8400 of 4, top 2: 9.7 and 45).
+  const long long enough = E.top <= 2 ? 16384 : E.classes <= 40 ? 32768 : 131072;
+  const bool planes = !E.index && E.classes <= 65536 && E.top <= 8 && (E.classes <= 8 || (E.cs != 1 && E.s1 < E.cs && rows >= enough));
   if (planes) {
     if (E.top == 0) launch_planes<T, ACT, 0>(E, st);
     else if (E.top <= 2) launch_planes<T, ACT, 2>(E, st);
-    else if (E.top <= 8) launch_planes<T, ACT, 8>(E, st);
-    else launch_planes<T, ACT, 32>(E, st);
+    else launch_planes<T, ACT, 8>(E, st);
     return lmi_check_launch("lmi_class_logprobs");
   }
   if (E.classes <= 128) {
-    const unsigned g = (unsigned)((rows + 15) / 16);
+    const long long teams = (rows + 15) / 16;
+    const unsigned g = (unsigned)(teams < kMaxGrid ? teams : kMaxGrid);
     if (E.classes <= 32) evidence_team_kernel<T, 2, ACT><<<g, 256, 0, st>>>(E, rows);
     else evidence_team_kernel<T, 8, ACT><<<g, 256, 0, st>>>(E, rows);
     return lmi_check_launch("lmi_class_logprobs");
   }
-  E.parts = split_parts(rows, E.classes);
+  E.parts = split_parts(rows, E.classes, E.cs, sizeof(T));
   E.part_len = (E.classes + E.parts - 1) / E.parts;
-  const long long cap = 1 << 22;   // grid x workgroup size stays below 2^32
-  const dim3 g((unsigned)(rows < cap ? rows : cap), (unsigned)E.parts), g4((unsigned)((rows + 3) / 4 < cap ? (rows + 3) / 4 : cap), (unsigned)E.parts);
+  const dim3 g((unsigned)(rows < kMaxGrid ? rows : kMaxGrid), (unsigned)E.parts);
+  const dim3 g4((unsigned)((rows + 3) / 4 < kMaxGrid ? (rows + 3) / 4 : kMaxGrid), (unsigned)E.parts);
   constexpr int V = 16 / sizeof(T);   // 128 bytes of a row per thread
   if (E.cs == 1) {
-    if (E.part_len <= 63 * 8 * V) evidence_rows_kernel<T, 64, 8, V, ACT><<<g4, 256, 0, st>>>(E);
-    else if (E.parts > 1) evidence_rows_kernel<T, 256, 8, V, ACT><<<g, 256, 0, st>>>(E);
+    // The smallest team that holds a row (or part) in one go; with many rows, whose teams fill the chip anyway, a smaller one that
+    // goes over the row in tiles (bf16, top 5, a wave / 256 / 512 threads: 512 x 8000 18 / 12 / 14 us, 512 x 32001 49 / 20 / 16,
+    // 2048 x 8000 22 / 26 / 46, 2048 x 32001 61 / 47 / 50, 16384 x 8000 94 / 169 / 334, 16384 x 32001 297 / 297 / 330).
+    constexpr long long kWave = 63 * 8 * V, kFour = 255 * 8 * V;   // a tile may start up to 15 bytes before its values
+    const bool many = rows * E.parts >= 2048;
+    if (E.part_len <= (many ? 2 * kWave : kWave)) evidence_rows_kernel<T, 64, 8, V, ACT><<<g4, 256, 0, st>>>(E);
+    else if (E.part_len <= kFour || many) evidence_rows_kernel<T, 256, 8, V, ACT><<<g, 256, 0, st>>>(E);
     else evidence_rows_kernel<T, 512, 8, V, ACT><<<g, 512, 0, st>>>(E);
   } else {
     if (E.part_len <= 512) evidence_rows_kernel<T, 64, 8, 1, ACT><<<g4, 256, 0, st>>>(E);
@@ -820,11 +802,9 @@ template <typename T> int launch_act(const Evidence &E, int act, hipStream_t st)
 
 extern "C" {
 
-int64_t lmi_class_logprobs_workspace_bytes(int64_t rows, int64_t classes, int64_t class_stride, int top) {
-  (void)class_stride;
-  (void)top;
+int64_t lmi_class_logprobs_workspace_bytes(int64_t rows, int64_t classes, int64_t class_stride, int x_dtype) {
   if (rows <= 0 || classes <= 0) return 0;
-  const int parts = split_parts(rows, classes);
+  const int parts = split_parts(rows, classes, class_stride, x_dtype == LMI_F32 ? 4 : 2);
   return parts > 1 ? rows * parts * (int64_t)(sizeof(PartHead) + kMaxTop * 8) : 0;
 }
 
@@ -844,7 +824,7 @@ int lmi_class_logprobs(const lmi_logprob_args *a, void *stream) {
   LMI_REQUIRE(!a->labels || (a->label_dtype == LMI_F32 || a->label_dtype == LMI_I32 || a->label_dtype == LMI_I64), LMI_ERR_BAD_ARG,
               "lmi_class_logprobs: labels must be fp32, int32 or int64");
   LMI_REQUIRE(!a->index || a->index_range > 0, LMI_ERR_BAD_ARG, "lmi_class_logprobs: index without a range");
-  const int64_t need = lmi_class_logprobs_workspace_bytes(a->n0 * a->n1, a->classes, a->class_stride, a->top);
+  const int64_t need = lmi_class_logprobs_workspace_bytes(a->n0 * a->n1, a->classes, a->class_stride, a->x_dtype);
   LMI_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), LMI_ERR_WORKSPACE,
               "lmi_class_logprobs: workspace of %lld bytes, %lld needed", (long long)a->workspace_bytes, (long long)need);
   LMI_REQUIRE(need == 0 || lmi_is_aligned(a->workspace, 16), LMI_ERR_ALIGNMENT, "lmi_class_logprobs: workspace must be 16-byte aligned");
@@ -869,7 +849,7 @@ int lmi_class_logprobs(const lmi_logprob_args *a, void *stream) {
   E.top_logprob = a->top_logprob;
   E.top_index = a->top_index;
   E.ws = (unsigned char *)a->workspace;
-  E.wide = 0;
+  E.pairs = 0;
   E.parts = 1;
   E.part_len = a->classes;
   hipStream_t st = (hipStream_t)stream;

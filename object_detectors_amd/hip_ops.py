@@ -836,7 +836,7 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
             l0, l1 = n1, 1
     workspace, need = None, 0
     if c >= _lib.LMI_LOGPROB_SPLIT_FROM:
-        need = int(_L.lmi_class_logprobs_workspace_bytes(n0 * n1, c, cs, top))
+        need = int(_L.lmi_class_logprobs_workspace_bytes(n0 * n1, c, cs, _FLOAT_DTYPES[x.dtype]))
         if need:   # not from the shared cache: two captured graphs that run side by side must not share it
             workspace = torch.empty((need,), dtype=torch.uint8, device=dev)
     args = _lib.LOGPROB_ARGS.pack(

@@ -59,8 +59,8 @@ def test_class_logprobs_arguments(L):
                 dict(x_dtype=2), dict(class_stride=0), dict(stride1=-1), dict(labels=4096, label_dtype=2), dict(index=4096)):
         assert _probs(L, **bad) == -1, bad
     assert _probs(L, classes=1 << 31) == -4 and _probs(L, n0=1 << 20, n1=1 << 12) == -4
-    need = lib.lmi_class_logprobs_workspace_bytes(2, 200001, 1, 5)
-    assert need > 0 and lib.lmi_class_logprobs_workspace_bytes(2, 80, 1, 5) == 0
+    need = lib.lmi_class_logprobs_workspace_bytes(2, 200001, 1, 0)
+    assert need > 0 and lib.lmi_class_logprobs_workspace_bytes(2, 80, 1, 0) == 0
     assert _probs(L, classes=200001, n1=2) == -3
     assert _probs(L, classes=200001, n1=2, workspace=4096, workspace_bytes=need - 1) == -3
     assert _probs(L, classes=200001, n1=2, workspace=4104, workspace_bytes=need) == -2

@@ -84,6 +84,26 @@ def test_planes(b, g, c, a, top, activation, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,g,c,a,top,activation", [(2, 1, 63, 8201, 32, "softmax"), (4, 1, 39, 8201, 8, "softmax"), (1, 4, 16, 4200, 2, "softmax"), (1, 1, 80, 16400, 2, "none"),
+                                                    (3, 1, 33, 5500, 0, "sigmoid"), (16, 1, 70, 8200, 5, "softmax"), (4, 1, 300, 4100, 1, "softmax")])
+def test_many_planes(b, g, c, a, top, activation, dtype):
+    test_planes(b, g, c, a, top, activation, dtype)
+
+
+@pytest.mark.parametrize("c,rows,top", [(5, 24, 3), (20, 16800, 2), (20, 33600, 7), (64, 16800, 20), (70, 132000, 5)])
+def test_many_planes_of_odd_values(c, rows, top):
+    """The odd values again, in rows that lie side by side, so many that each has a thread of its own."""
+    x, gen = _odd_rows(c)
+    labels = torch.randint(0, c, (12,), generator=gen)
+    planes = x.t().repeat(1, rows // 12).contiguous().cuda()
+    r = _ops().class_logprobs(planes.t(), labels.repeat(rows // 12).cuda(), top=top)
+    _check({k: v[:12] for k, v in r.items()}, x, labels, top, "softmax", sequential=c + 8)
+    for v in r.values():
+        v = v.reshape(rows // 12, -1).nan_to_num(nan=123.0)
+        assert (v == v[0]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("b,nc,a,m,top,activation", [(1, 80, 8400, 300, 5, "none"), (4, 3, 525, 17, 3, "sigmoid"), (2, 131, 1701, 64, 32, "softmax"),
                                                      (2, 1, 40, 5, 1, "none")])
 def test_gathered(b, nc, a, m, top, activation, dtype):
@@ -111,10 +131,7 @@ def test_gathered(b, nc, a, m, top, activation, dtype):
             assert (v[i, n:] == 7).all()
 
 
-@pytest.mark.parametrize("c", [5, 100, 1500, 20000, 70000])
-@pytest.mark.parametrize("layout", ["rows", "planes"])
-def test_masked_and_odd_values(c, layout):
-    """Masked classes, rows with nothing left, the type's lowest value as a mask, equal values, infinities and NaN."""
+def _odd_rows(c):
     gen = torch.Generator().manual_seed(c)
     x = torch.randn(12, c, generator=gen)
     x[1, torch.rand(c, generator=gen) < 0.9] = -float("inf")
@@ -129,6 +146,14 @@ def test_masked_and_odd_values(c, layout):
     x[10] = -float("inf")
     x[10, c - 1] = 3.0                                    # one class left
     x[11] = torch.arange(c).flip(0) * 0.001               # sorted
+    return x, gen
+
+
+@pytest.mark.parametrize("c", [5, 100, 1500, 20000, 70000])
+@pytest.mark.parametrize("layout", ["rows", "planes"])
+def test_masked_and_odd_values(c, layout):
+    """Masked classes, rows with nothing left, the type's lowest value as a mask, equal values, infinities and NaN."""
+    x, gen = _odd_rows(c)
     x = x.cuda()
     if layout == "planes":
         x = x.t().contiguous().t()
@@ -210,6 +235,29 @@ def test_far_rows_of_a_large_tensor():
     _check(_ops().class_logprobs(x[-3:], labels, top=3), x[-3:], labels, 3, "softmax")
     r = _ops().class_logprobs(x, torch.zeros(n, dtype=torch.int64, device="cuda"))
     _check({k: v[-3:] for k, v in r.items()}, x[-3:], torch.zeros(3, dtype=torch.int64), 0, "softmax")
+
+
+def test_more_rows_than_a_grid_holds():
+    """2^28 rows of 9 classes, 16 lanes each."""
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    n = (1 << 28) + 40
+    x = torch.zeros(n, 9, dtype=torch.float16, device="cuda")
+    x[-5:].copy_(torch.randn(5, 9))
+    x[1 << 20].copy_(torch.randn(9))
+    r = _ops().class_logprobs(x)["entropy"]
+    for at in (slice(n - 9, n), slice((1 << 20) - 2, (1 << 20) + 2)):
+        _check({"entropy": r[at]}, x[at], None, 0, "softmax")
+    assert int((r == r[0]).sum()) == n - 6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,c,top", [(2100, 5000, 5), (2050, 17000, 8), (300, 40000, 3), (255, 70003, 6)])
+def test_many_long_rows(n, c, top, dtype):
+    """Rows that a team goes over in tiles, or in parts, many of them; the last ones are checked."""
+    x, labels = _rows(c, n, c, DTYPES[dtype], "softmax")
+    r = _ops().class_logprobs(x, labels, top=top)
+    _check({k: v[-20:] for k, v in r.items()}, x[-20:], labels[-20:], top, "softmax")
 
 
 def test_captured_and_replayed():

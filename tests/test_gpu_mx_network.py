@@ -82,6 +82,27 @@ def test_every_layer_of_a_forward(dtype, channels_last):
         assert (np.abs(got - want) <= tol).all(), name
 
 
+def test_the_head_too():
+    """head=True takes the head's 1x1 layers as well, those without norm and activation included; a second call finds none."""
+    net = _net("segment").cuda()
+    plain = {name: (m.weight.detach().flatten(1).clone(), m.bias.detach().clone()) for name, m in net.named_modules()
+             if isinstance(m, torch.nn.Conv2d) and m.kernel_size == (1, 1) and m.bias is not None}
+    few = sum(isinstance(m, torch.nn.Conv2d) and m.kernel_size == (1, 1) for m in net.modules())
+    assert net.quantize_pointwise(head=True) == few and net.quantize_pointwise(head=True) == 0
+    mods = {name: m for name, m in net.named_modules() if isinstance(m, MxPointwise)}
+    assert len(plain) == 9 and set(plain) < set(mods)
+    seen = {}
+    for name in plain:
+        mods[name].register_forward_hook(lambda m, a, y, name=name: seen.update({name: (a[0], y)}))
+    with torch.inference_mode():
+        net(torch.rand(2, 3, 96, 160, device="cuda"))
+    for name, (w, b) in plain.items():
+        a, y = seen[name]
+        want, size = OM.product(a.permute(0, 2, 3, 1).reshape(-1, w.shape[1]).double().cpu().numpy(), w.double().cpu().numpy(), b.double().cpu().numpy())
+        got = y.permute(0, 2, 3, 1).reshape(-1, w.shape[0]).double().cpu().numpy()
+        assert (np.abs(got - want) <= (w.shape[1] + 8) * 2.0 ** -23 * size + 1e-37).all(), name
+
+
 @pytest.mark.parametrize("task", ["detect", "segment", "pose", "obb"])
 @pytest.mark.parametrize("fp16", [False, True])
 def test_predict_with_evidence(tmp_path, task, fp16):

@@ -14,7 +14,7 @@
 //  mx_dequantize_kernel   8 rows x one step per wave, whole lines written.
 //  mx_stream_kernel       the product of many positions that come as floats: 128 of them x up to 320 weight rows per workgroup, streamed along k.
 //  mx_rows_kernel         the product of many quantised rows: 128 or 256 of them per workgroup.
-//  mx_wave_planes_kernel  shallow 1x1 convolutions (k <= 128): a wave per 64 positions, everything in registers.
+//  mx_wave_planes_kernel  shallow 1x1 convolutions (k <= 64): a wave per 64 positions, everything in registers.
 //  mx_few_kernel          few positions (a single row, one image's deepest maps): the waves of a workgroup share k.
 #include <hip/hip_fp16.h>
 
@@ -253,9 +253,6 @@ template <int BYTE> __device__ __forceinline__ void mfma2(f16x (&acc)[2], const 
   acc[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a), operand(b1), acc[1], 4, 4, BYTE, (int)sa, BYTE, (int)sb1);
 }
 
-// One wave, 64 positions, all of k (at most 128) in registers: what a lane quantises is its operand.  No LDS, no barrier: the waves of
-// a CU drift apart, so that some load while others multiply.
-constexpr int kWaveSteps = 2;   // deeper ones stream faster: 64 x 192 -> 192 on 80 x 80: 80 us here, 68 streamed; 128 -> 640: 141 and 172; 48 -> 32 on 160 x 160: 56 and 84
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 template <typename T> struct Raw {   // one step's values of a lane before they are quantised: two pixels of 32 channels
@@ -403,6 +400,9 @@ __device__ __forceinline__ void store_rows(const Product &P, Y *y, long long p0,
   }
 }
 
+// One wave, 64 positions, k of one step (at most 64), everything in registers: what a lane quantises is its operand.  No LDS, no barrier: the
+// waves of a CU drift apart, so that some load while others multiply.  Bound by HBM: 64 x 64 -> 32 on 160 x 160 58 us, 5.4 TB/s (69 streamed);
+// 16 x 48 -> 32 on 160 x 160 17.5 and 21.  Two steps held that way stream faster: 16 x 128 -> 64 on 80 x 80 13.6 us, 11 streamed.
 template <typename T>
 __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P, int act, long long tiles) {
   const int lane = threadIdx.x & 63;
@@ -412,23 +412,12 @@ __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P,
   const long long p0 = (long long)(tile % P.tiles_pixels) * kTile;
   const int live = (int)(P.pixels - p0 < kTile ? P.pixels - p0 : kTile);
   const T *x = (const T *)P.x + image * P.xb + p0;
-  const unsigned offset = (unsigned)((lane >> 5) * 32 * P.xs1 + 2 * (lane & 31)) * sizeof(T);
-  const bool mine = 2 * (lane & 31) < live;
-  const int S = P.all_steps, half = lane >> 5;
-  uint4 f[kWaveSteps][2];
-  unsigned sw[2] = {};
+  const int half = lane >> 5, left = (int)P.k - 32 * half;
   Raw<T> raw;
-#pragma unroll
-  for (int s = 0; s < kWaveSteps; ++s) {
-    if (s < S) {
-      const int left = (int)(P.k - 64ll * s) - 32 * half;
-      load_planes<T>(x + 64ll * s * P.xs1, offset, P.xs1, mine, left < 0 ? 0 : left, raw);
-      unsigned byte[2];
-      quantize_raw(raw, f[s], byte);
-      sw[0] |= byte[0] << (8 * s);
-      sw[1] |= byte[1] << (8 * s);
-    }
-  }
+  load_planes<T>(x, (unsigned)(half * 32 * P.xs1 + 2 * (lane & 31)) * sizeof(T), P.xs1, 2 * (lane & 31) < live, left < 0 ? 0 : left, raw);
+  uint4 f[2];
+  unsigned byte[2];
+  quantize_raw(raw, f, byte);
   const int wl = weight_lane(lane);
   const int nt0 = blockIdx.y * P.split_n;
   const int nt1 = nt0 + P.split_n < P.tiles_n ? nt0 + P.split_n : P.tiles_n;
@@ -436,13 +425,7 @@ __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P,
   for (int nt = nt0; nt < nt1; ++nt) {
     f16x acc[2];
     start_sums(P, nt, lane, acc);
-    const uint4 *w = P.w + nt * 64ll + wl;
-    const unsigned sa = P.ws[nt * 64 + wl];
-    uint4 a[kWaveSteps];
-#pragma unroll
-    for (int s = 0; s < kWaveSteps; ++s) a[s] = w[(s < S ? s : S - 1) * (long long)P.tiles_n * 64];
-    mfma2<0>(acc, a[0], sa, f[0][0], f[0][1], sw[0], sw[1]);
-    if (S > 1) mfma2<1>(acc, a[1], sa, f[1][0], f[1][1], sw[0], sw[1]);
+    mfma2<0>(acc, P.w[nt * 64ll + wl], P.ws[nt * 64ll + wl], f[0], f[1], byte[0], byte[1]);
     store_planes<T>(P, y, p0, live, nt, lane, act, true, acc);
   }
 }
@@ -459,7 +442,8 @@ template <typename T> void launch_wave_planes(Product P, int act, long long batc
 // Streaming product: 128 positions x up to 64 * NT weight rows per workgroup, k in chunks of two steps.  While the matrix instructions run
 // on one chunk, the next chunk's activations and weights are on their way to registers (loads straight to LDS would be waited for
 // before the next read of any LDS); an activation block is quantised by the thread that loaded it.  Waves are dealt 2 (positions) x 2 (weight rows), each 64 positions x 32 * NT
-// rows of sums in registers: a fragment read from LDS serves 2 or NT matrix instructions.
+// rows of sums in registers: a fragment read from LDS serves 2 or NT matrix instructions.  Bound by HBM: 64 x 1280 -> 320 on 80 x 80 (fp16, 1.31 GB) 270 us, 4.9 TB/s; two
+// workgroups per CU hold 64 KB of loads in flight and stop for each other at every chunk, which costs the rest to 6.2 TB/s.
 constexpr int kChunkTile = 128;
 
 template <typename T, bool PLANES, bool VEC> struct Chunk;   // what a thread holds of a chunk
@@ -662,7 +646,7 @@ template <typename T, typename Y, bool PLANES, bool VEC> void launch_stream(Prod
 // Quantised rows: 64 * WP of them x 32 * NT * 4 / WP weight rows per workgroup, a wave 64 x 32 * NT.  The weights go through LDS; a wave's rows, which
 // at most one other wave needs, come straight into the operands, a chunk of two steps ahead: with both through LDS its traffic (84 KB
 // per chunk for 655 k products of 64) kept it as busy as the matrix units, 8192 x 2560 -> 2560 took 49 us instead of 44.  What
-// bounds it: the matrix units are busy for half of the time of a deep product (3.9 of the 8.9 PFLOP/s that a loop of
+// bounds it: the matrix units are busy for half of the time of a deep product (3.8 of the 8.9 PFLOP/s that a loop of
 // nothing else reaches: 8192 x 10240 -> 2560 in 112 us, 1.2 us per chunk), the rest are the waits of two workgroups per CU for
 // each other's loads; touching lines two chunks ahead, chunks in two sets of registers with smaller tiles, and priorities changed
 // nothing or cost; the first loads and 42 MB of results take 15 of the 44 us.
@@ -809,9 +793,11 @@ template <typename Y, int WP> void launch_rows(const Product &P, int act, hipStr
 // Few positions: 64 of them x 32 weight rows per workgroup, its eight waves share k.  A wave loads its steps' blocks straight into the
 // operands -- no LDS, no barrier before the sums meet; a workgroup's time is the latency of a load or two.
 constexpr int kFewWaves = 8;
-// up to this many pairs of tiles (about a thousand: 4 x 320 -> 320 on 40 x 40, 100 x 10 of them, 11.3 us here and 11.7 streamed; 16 x 640 -> 640
-// on 20 x 20, 112 x 20, 31 and 21); quantised rows stream sooner (1024 x 1280 x 1280, 16 x 40: 10.7 and 7.6)
-constexpr long long kFewTiles = 1024, kFewTilesPacked = 320;
+// Up to this many pairs of tiles, two workgroups per CU (us here and streamed, fp16: 640 -> 320 on 40 x 40, 25 x 10 of them, 7.9 and 9.9;
+// 320 -> 160 on 80 x 80, 100 x 5, 7.1 and 7.6; 4 x 640 -> 640 on 20 x 20, 28 x 20, 12.6 and 10.7; 4 x 320 -> 320 on 40 x 40, 100 x 10, 12.1 and
+// 9.5; 2000 rows of 1280 -> 160, 32 x 5, 10.4 and 24); quantised rows stream sooner (512 x 5120 -> 640, 8 x 20: 11 and 20; 2048 x 320 ->
+// 320, 32 x 10: 6.2 and 4.5)
+constexpr long long kFewTiles = 512, kFewTilesPacked = 320;
 
 // blocks kb = 2 * step + (lane >> 5) of the lane's two positions
 template <typename T, bool PLANES>
@@ -925,7 +911,7 @@ template <typename T, typename Y, bool PLANES> int launch_product(Product P, int
     return lmi_check_launch("lmi_mx_product");
   }
   if constexpr (PLANES) {
-    if (P.vec && P.all_steps <= kWaveSteps && tiles >= 512) {
+    if (P.vec && P.all_steps == 1 && tiles >= 512) {
       launch_wave_planes<T>(P, act, batch, st);
       return lmi_check_launch("lmi_mx_product");
     }

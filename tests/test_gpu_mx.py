@@ -113,7 +113,8 @@ def test_linear(m, k, n, act, dtype):
 @pytest.mark.parametrize("layout", ["planes", "channels_last", "slice"])
 @pytest.mark.parametrize("b,k,n,h,w,act", [(1, 1, 1, 1, 1, None), (1, 640, 640, 20, 20, "silu"), (3, 400, 75, 7, 13, "silu"), (2, 48, 16, 1, 5, None),
                                            (2, 33, 40, 9, 1, "silu"), (4, 96, 64, 40, 24, None), (1, 80, 32, 160, 96, "silu"), (5, 64, 80, 1, 1, "silu"),
-                                           (1, 2600, 70, 3, 11, None), (2, 5000, 33, 4, 4, "silu")])
+                                           (1, 2600, 70, 3, 11, None), (2, 5000, 33, 4, 4, "silu"),
+                                           (2, 48, 40, 160, 128, "silu"), (1, 33, 16, 200, 168, None), (1, 64, 65, 182, 181, "silu")])
 def test_pointwise(b, k, n, h, w, act, layout, dtype):
     ops, dt = _ops(), DTYPES[dtype]
     g = torch.Generator().manual_seed(k + n)

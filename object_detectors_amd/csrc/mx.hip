@@ -968,7 +968,7 @@ struct Sizes {
 };
 
 // Rows that come as floats and meet many weight rows are quantised once, into the workspace, where they would be quantised again for
-// every 320 weight rows or fewer: 8192 x 1280 -> 2560 (fp16) 34 us, 59 without; 102400 x 640 -> 640 108 and 132; 128 x 1280 -> 32000 41 and
+// every 320 weight rows or fewer: 8192 x 1280 -> 2560 (fp16) 34 us, 59 without; 102400 x 1280 -> 640 149 and 183; 128 x 1280 -> 32000 42 and
 // 156.  Few pairs of tiles (those that the waves of mx_few_kernel share in one round), 256 weight rows or k <= 128 do not
 // pay for the second kernel: 102400 x 1280 -> 160 98 us, 79 without; 8192 x 96 -> 640 11.4 and 9.9.
 constexpr int64_t kQuantiseN = 256, kQuantiseK = 128;

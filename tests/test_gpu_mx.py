@@ -214,6 +214,21 @@ def test_many_rows_and_weights(m, k, n, act, dtype):
         assert torch.equal(y, ops.mx_linear(ops.mx_quantize(x), wq, bias, act=act, dtype=dt))
 
 
+@pytest.mark.parametrize("m,n", [(5003, 165), (9001, 700)])
+@pytest.mark.parametrize("k", [33, 65, 192, 257, 321, 448, 512])
+def test_many_quantised_rows(m, n, k):
+    """One to eight steps of 64 along k, rows and weight rows that end inside a tile; either number of rows per workgroup."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(m + k)
+    x, w = torch.randn(m, k, generator=g).cuda(), torch.randn(n, k, generator=g).cuda()
+    bias = torch.randn(n, generator=g).cuda()
+    guard = torch.full((m * n + 64,), 5.0, dtype=torch.bfloat16, device="cuda")
+    y = ops.mx_linear(ops.mx_quantize(x), ops.mx_quantize(w), bias, dtype=torch.bfloat16, out=guard[32:32 + m * n].view(m, n))
+    want, size = OM.product(_np(x), _np(w), _np(bias))
+    _close(y, want, size, k, torch.bfloat16, None)
+    assert (guard[:32] == 5).all() and (guard[-32:] == 5).all()
+
+
 @pytest.mark.parametrize("step", [1, 2])
 def test_many_channels_last_images(step):
     """Images whose rows follow each other, and every other image, whose rows do not."""

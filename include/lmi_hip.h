@@ -512,7 +512,7 @@ int lmi_class_logprobs(const lmi_logprob_args *args, void *stream);
  *   w quantised.  The positions m are (batch, pixels).  layout LMI_MX_ROWS (a linear layer, channels-last maps): x
  *   element (b, p, k) at b*x_batch + p*x_stride + k, y contiguous (batch, pixels, n).  LMI_MX_PLANES (NCHW maps): x
  *   element at b*x_batch + k*x_stride + p, y contiguous (batch, n, pixels).  x_stride, and the pixels of a plane, stay
- *   below 2^24.
+ *   below 2^24; maps of one pixel are rows.
  *   x_dtype LMI_MXFP4: x points at the packed blocks, x_scales at their scales (rows, batch 1, x_stride unused).
  *   y_dtype LMI_F32 | LMI_F16 | LMI_BF16, the type of x unless that is MXFP4.  bias [device] fp32 (n) or NULL.
  *   workspace [device] of lmi_mx_product_workspace_bytes, 16-byte aligned (0: none): float rows that meet many weight rows

@@ -183,7 +183,6 @@ struct Product {
   int tiles_n;            // tiles of 32 weight rows
   int split_n;            // tiles of 32 weight rows per wave (mx_wave_planes_kernel)
   int all_steps;          // steps of 64 along k
-  int vec;                // x allows wide loads: planes, two pixels; rows, 16 bytes
 };
 
 constexpr int kTile = 64;   // positions of a wave
@@ -264,24 +263,28 @@ template <> struct Raw<float> {
 
 // Addresses are a base that is the same for the wave (scalar registers) plus a 32-bit offset of the lane: the launcher sees to it that
 // 32 channels or rows fit.
-template <typename W> __device__ __forceinline__ W at(const void *base, unsigned offset) {
+template <typename W, int ALIGN = sizeof(W)> __device__ __forceinline__ W at(const void *base, unsigned offset) {
   typedef const __attribute__((address_space(1))) char *global;
+  typedef W word __attribute__((aligned(ALIGN)));
   global b = (global)base;
   asm("" : "+s"(b));   // kept in scalar registers: without this the sum goes to a pair of vector registers per load
-  return *(const __attribute__((address_space(1))) W *)(b + offset);
+  return *(const __attribute__((address_space(1))) word *)(b + offset);
 }
-template <typename W> __device__ __forceinline__ const W *at_any(const void *base, unsigned offset) { return (const W *)((const char *)base + offset); }   // a base of the lane's own
+template <typename W, int ALIGN = sizeof(W)> __device__ __forceinline__ W at_any(const void *base, unsigned offset) {   // a base of the lane's own
+  typedef W word __attribute__((aligned(ALIGN)));
+  return *(const word *)((const char *)base + offset);
+}
 
-// `in` channels (32 or more: all) of two neighbouring pixels from base + offset on; base is uniform
+// `in` channels (32 or more: all) of two neighbouring pixels from base + offset on, one word at whatever address; base is uniform
 template <typename T, bool SCALAR = true>
 __device__ __forceinline__ void load_planes(const T *base, unsigned offset, long long stride, bool live, int in, Raw<T> &r) {
   typedef typename std::remove_reference<decltype(r.v[0])>::type W;
   if (live && in >= 32) {
 #pragma unroll
-    for (int u = 0; u < 32; ++u) r.v[u] = SCALAR ? at<W>(base + u * stride, offset) : *at_any<W>(base + u * stride, offset);
+    for (int u = 0; u < 32; ++u) r.v[u] = SCALAR ? at<W, sizeof(T)>(base + u * stride, offset) : at_any<W, sizeof(T)>(base + u * stride, offset);
   } else if (live && in > 0) {   // the last channels: all loads at once, those beyond read the first again
 #pragma unroll
-    for (int u = 0; u < 32; ++u) r.v[u] = *at_any<W>(base + (u < in ? u * stride : 0), offset);
+    for (int u = 0; u < 32; ++u) r.v[u] = at_any<W, sizeof(T)>(base + (u < in ? u * stride : 0), offset);
 #pragma unroll
     for (int u = 0; u < 32; ++u) r.v[u] = u < in ? r.v[u] : W{};
   } else {
@@ -289,34 +292,19 @@ __device__ __forceinline__ void load_planes(const T *base, unsigned offset, long
     for (int u = 0; u < 32; ++u) r.v[u] = W{};
   }
 }
-// the same value by value; `live` of the two pixels are there
-template <typename T> __device__ __forceinline__ void load_planes_single(const T *base, unsigned offset, long long stride, int live, int in, Raw<T> &r) {
-  auto put = [&](int u, T a, T b) {
-    if constexpr (sizeof(T) == 4) r.v[u] = f2{a, b};
-    else r.v[u] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
-  };
-  const unsigned next = offset + (live > 1 ? sizeof(T) : 0);   // what is not there reads a neighbour that is
-  if (live > 0 && in >= 32) {
-#pragma unroll
-    for (int u = 0; u < 32; ++u) put(u, at<T>(base + u * stride, offset), at<T>(base + u * stride, next));
-    if (live == 1) {
-#pragma unroll
-      for (int u = 0; u < 32; ++u) {
-        if constexpr (sizeof(T) == 4) r.v[u].y = 0.0f;
-        else r.v[u] &= 0xffffu;
-      }
-    }
-  } else if (live > 0 && in > 0) {
-#pragma unroll
-    for (int u = 0; u < 32; ++u) put(u, *at_any<T>(base + (u < in ? u * stride : 0), offset), *at_any<T>(base + (u < in ? u * stride : 0), next));
+// Planes of odd size (640 -> 320 on 37 x 37 fp16 8.3 us, value by value 24; 64 x 320 -> 320 on 79 x 79 190 and 359): the pair that reaches beyond its plane, `live` == 1, is read one
+// pixel earlier, in the same plane, which has at least two; move_pair puts its pixel where it belongs.
+template <typename T, bool SCALAR = true>
+__device__ __forceinline__ void load_planes_odd(const T *base, unsigned offset, long long stride, int live, int in, Raw<T> &r) {
+  load_planes<T, SCALAR>(base - 1, offset + (live == 1 ? 0 : sizeof(T)), stride, live > 0, in, r);
+}
+template <typename T> __device__ __forceinline__ void move_pair(Raw<T> &r, bool late) {
+  if (late) {
 #pragma unroll
     for (int u = 0; u < 32; ++u) {
-      if constexpr (sizeof(T) == 4) r.v[u] = f2{u < in ? r.v[u].x : 0.0f, u < in && live > 1 ? r.v[u].y : 0.0f};
-      else r.v[u] = u < in ? (live > 1 ? r.v[u] : r.v[u] & 0xffffu) : 0u;
+      if constexpr (sizeof(T) == 4) r.v[u] = f2{r.v[u].y, 0.0f};
+      else r.v[u] >>= 16;
     }
-  } else {
-#pragma unroll
-    for (int u = 0; u < 32; ++u) put(u, (T)0.0f, (T)0.0f);
   }
 }
 __device__ __forceinline__ void quantize_raw(const Raw<float> &r, uint4 (&f)[2], unsigned (&byte)[2]) {
@@ -344,7 +332,7 @@ __device__ __forceinline__ void start_sums(const Product &P, int nt, int lane, f
 // planes: a lane holds 16 weight rows' results of two neighbouring positions.  Results are not read again soon: stored past the caches
 // (the 160 x 160 maps of a batch of 64, 48 -> 32 channels: 75 -> 56 us with the sums starting at the bias).
 template <typename Y>
-__device__ __forceinline__ void store_planes(const Product &P, Y *y, long long p0, int live, int nt, int lane, int act, bool vec, const f16x (&acc)[2]) {
+__device__ __forceinline__ void store_planes(const Product &P, Y *y, long long p0, int live, int nt, int lane, int act, bool even, const f16x (&acc)[2]) {
   const int px = 2 * (lane & 31), n0 = 16 * (lane >> 5);
   const long long left = P.n - nt * 32ll - n0;
   const unsigned offset = (unsigned)(n0 * P.pixels + px) * sizeof(Y);
@@ -357,13 +345,10 @@ __device__ __forceinline__ void store_planes(const Product &P, Y *y, long long p
       v1 = activate<LMI_ACT_SILU>(v1);
     }
     typedef Y y2 __attribute__((ext_vector_type(2)));
-    if (vec) {
-      if (px < live && i < left) __builtin_nontemporal_store(y2{(Y)v0, (Y)v1}, (y2 *)((char *)(base + i * P.pixels) + offset));
-    } else if (i < left) {
-      Y *q = base + (n0 + i) * P.pixels + px;
-      if (px < live) q[0] = (Y)v0;
-      if (px + 1 < live) q[1] = (Y)v1;
-    }
+    typedef y2 pair __attribute__((aligned(sizeof(Y))));
+    Y *q = (Y *)((char *)(base + i * P.pixels) + offset);
+    if ((even ? px : px + 1) < live && i < left) __builtin_nontemporal_store(y2{(Y)v0, (Y)v1}, (pair *)q);
+    if (!even && px + 1 == live && i < left) *q = (Y)v0;   // the last of a plane of odd size
   }
 }
 
@@ -403,7 +388,7 @@ __device__ __forceinline__ void store_rows(const Product &P, Y *y, long long p0,
 // One wave, 64 positions, k of one step (at most 64), everything in registers: what a lane quantises is its operand.  No LDS, no barrier: the
 // waves of a CU drift apart, so that some load while others multiply.  Bound by HBM: 64 x 64 -> 32 on 160 x 160 58 us, 5.4 TB/s (69 streamed);
 // 16 x 48 -> 32 on 160 x 160 17.5 and 21.  Two steps held that way stream faster: 16 x 128 -> 64 on 80 x 80 13.6 us, 11 streamed.
-template <typename T>
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P, int act, long long tiles) {
   const int lane = threadIdx.x & 63;
   const unsigned tile = blockIdx.x * 4 + wave_id();
@@ -414,7 +399,14 @@ __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P,
   const T *x = (const T *)P.x + image * P.xb + p0;
   const int half = lane >> 5, left = (int)P.k - 32 * half;
   Raw<T> raw;
-  load_planes<T>(x, (unsigned)(half * 32 * P.xs1 + 2 * (lane & 31)) * sizeof(T), P.xs1, 2 * (lane & 31) < live, left < 0 ? 0 : left, raw);
+  const unsigned offset = (unsigned)(half * 32 * P.xs1 + 2 * (lane & 31)) * sizeof(T);
+  const int here = live - 2 * (lane & 31);
+  if constexpr (VEC) {
+    load_planes<T>(x, offset, P.xs1, here > 0, left < 0 ? 0 : left, raw);
+  } else {
+    load_planes_odd<T>(x, offset, P.xs1, here, left < 0 ? 0 : left, raw);
+    move_pair<T>(raw, here == 1);
+  }
   uint4 f[2];
   unsigned byte[2];
   quantize_raw(raw, f, byte);
@@ -426,17 +418,17 @@ __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P,
     f16x acc[2];
     start_sums(P, nt, lane, acc);
     mfma2<0>(acc, P.w[nt * 64ll + wl], P.ws[nt * 64ll + wl], f[0], f[1], byte[0], byte[1]);
-    store_planes<T>(P, y, p0, live, nt, lane, act, true, acc);
+    store_planes<T>(P, y, p0, live, nt, lane, act, VEC, acc);
   }
 }
 
-template <typename T> void launch_wave_planes(Product P, int act, long long batch, hipStream_t st) {
+template <typename T, bool VEC> void launch_wave_planes(Product P, int act, long long batch, hipStream_t st) {
   P.tiles_pixels = (unsigned)((P.pixels + kTile - 1) / kTile);
   const long long tiles = batch * P.tiles_pixels;
   const long long split = tiles < 2048 ? (2048 + tiles - 1) / tiles : 1;
   P.split_n = (int)((P.tiles_n + split - 1) / split);
   const dim3 grid((unsigned)((tiles + 3) / 4), (unsigned)((P.tiles_n + P.split_n - 1) / P.split_n));
-  mx_wave_planes_kernel<T><<<grid, 256, 0, st>>>(P, act, tiles);
+  mx_wave_planes_kernel<T, VEC><<<grid, 256, 0, st>>>(P, act, tiles);
 }
 
 // Streaming product: 128 positions x up to 64 * NT weight rows per workgroup, k in chunks of two steps.  While the matrix instructions run
@@ -450,18 +442,24 @@ template <typename T, bool PLANES, bool VEC> struct Chunk;   // what a thread ho
 // planes: two neighbouring pixels x one block
 template <typename T, bool VEC> struct Chunk<T, true, VEC> {
   Raw<T> raw;
+  bool late = false;
   __device__ __forceinline__ void load(const Product &P, const T *x, int live, int chunk) {
     const int pair = threadIdx.x & 63;
     const long long c0 = (4ll * chunk + wave_id()) * 32;   // beyond k: in = 0
     const int in = c0 < P.k ? (int)(P.k - c0 < 32 ? P.k - c0 : 32) : 0;
-    if constexpr (VEC) load_planes<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, 2 * pair < live, in, raw);
-    else load_planes_single<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, live - 2 * pair, in, raw);
+    if constexpr (VEC) {
+      load_planes<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, 2 * pair < live, in, raw);
+    } else {
+      load_planes_odd<T>(x + c0 * P.xs1, 2 * pair * sizeof(T), P.xs1, live - 2 * pair, in, raw);
+      late = live - 2 * pair == 1;
+    }
   }
-  template <int P> __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) const {
+  template <int P> __device__ __forceinline__ void put(uint4 (&xb)[2][4][64], unsigned (&xs)[4][64]) {
     const int pair = threadIdx.x & 63, kl = wave_id();
     const int sub = (pair >> 5) * 2, at = (kl & 1) * 32 + (pair & 31);
     uint4 f[2];
     unsigned byte[2];
+    if constexpr (!VEC) move_pair<T>(raw, late);
     quantize_raw(raw, f, byte);
 #pragma unroll
     for (int px = 0; px < 2; ++px) {
@@ -624,10 +622,10 @@ __global__ __launch_bounds__(256, sizeof(Y) == 2 && NT <= (PLANES ? 2 : 1) ? 3 :
 template <typename T, typename Y, bool PLANES, bool VEC> void launch_stream(Product P, int act, long long batch, hipStream_t st) {
   P.tiles_pixels = (unsigned)((P.pixels + kChunkTile - 1) / kChunkTile);
   const long long tiles = batch * P.tiles_pixels;
-  // as many weight rows per workgroup as the registers hold beside a chunk (fp32 and single loads hold more): 1280 -> 320 on 64 maps of 80 x 80
+  // as many weight rows per workgroup as the registers hold beside a chunk (fp32 and rows read value by value hold more): 1280 -> 320 on 64 maps of 80 x 80
   // with 5 tiles per wave 302 us, with 3 or 4 and the activations read twice through the L2 415;
   // fp32 rows with 4 spill 100 bytes a lane and are faster all the same: 102400 x 1280 -> 256 183 us, 208 with 3
-  constexpr int kMaxNT = !VEC ? 3 : PLANES && sizeof(Y) == 2 ? 5 : 4;
+  constexpr int kMaxNT = PLANES && sizeof(Y) == 2 ? 5 : VEC || PLANES ? 4 : 3;
   int splits = (P.tiles_n + 2 * kMaxNT - 1) / (2 * kMaxNT);
   while (tiles * splits < 256 && splits * 2 <= P.tiles_n) splits *= 2;
   int nt = (P.tiles_n + 2 * splits - 1) / (2 * splits);
@@ -800,7 +798,7 @@ constexpr int kFewWaves = 8;
 constexpr long long kFewTiles = 512, kFewTilesPacked = 320;
 
 // blocks kb = 2 * step + (lane >> 5) of the lane's two positions
-template <typename T, bool PLANES>
+template <typename T, bool PLANES, bool VEC>
 __device__ __forceinline__ void load_few(const Product &P, const T *x, long long p0, int live, int step, int lane, uint4 (&f)[2], unsigned (&byte)[2]) {
   const int j = lane & 31;
   if constexpr (__is_same(T, Packed)) {
@@ -816,22 +814,24 @@ __device__ __forceinline__ void load_few(const Product &P, const T *x, long long
     const long long c0 = step * 64ll + (lane >> 5) * 32;
     const int in = (int)(P.k - c0 < 0 ? 0 : P.k - c0 < 32 ? P.k - c0 : 32);
     if constexpr (PLANES) {
-      if (P.vec) {
-        Raw<T> raw;
-        load_planes<T, false>(x + step * 64ll * P.xs1, (unsigned)((lane >> 5) * 32 * P.xs1 + 2 * j) * sizeof(T), P.xs1, 2 * j < live, in, raw);
-        quantize_raw(raw, f, byte);
-        return;
+      Raw<T> raw;
+      const T *base = x + step * 64ll * P.xs1;
+      const unsigned offset = (unsigned)((lane >> 5) * 32 * P.xs1 + 2 * j) * sizeof(T);
+      if constexpr (VEC) {
+        load_planes<T, false>(base, offset, P.xs1, 2 * j < live, in, raw);
+      } else {
+        load_planes_odd<T, false>(base, offset, P.xs1, live - 2 * j, in, raw);
+        move_pair<T>(raw, live - 2 * j == 1);
       }
+      quantize_raw(raw, f, byte);
+      return;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int px = 32 * h + j;
-      const long long stride = PLANES ? P.xs1 : 1;
-      const T *base = x + step * 64ll * stride;
-      const unsigned offset = (unsigned)((lane >> 5) * 32 * stride + px * (PLANES ? 1 : P.xs1)) * sizeof(T);
-      const T *q = at_any<T>(base, offset);
+      const T *q = (const T *)((const char *)(x + step * 64ll) + (unsigned)((lane >> 5) * 32 + px * P.xs1) * sizeof(T));
       float v[32];
-      if (!PLANES && P.vec && px < live && in == 32) {
+      if (VEC && px < live && in == 32) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           float e[8];
@@ -841,10 +841,10 @@ __device__ __forceinline__ void load_few(const Product &P, const T *x, long long
         }
       } else if (px < live && in == 32) {
 #pragma unroll
-        for (int u = 0; u < 32; ++u) v[u] = to_float(*at_any<T>(base + u * stride, offset));
-      } else if (px < live && in > 0) {   // all loads at once: channels beyond the last read the first again
+        for (int u = 0; u < 32; ++u) v[u] = to_float(q[u]);
+      } else if (px < live && in > 0) {   // all loads at once: elements beyond the last read the first again
 #pragma unroll
-        for (int u = 0; u < 32; ++u) v[u] = to_float(*at_any<T>(base + (u < in ? u * stride : 0), offset));
+        for (int u = 0; u < 32; ++u) v[u] = to_float(q[u < in ? u : 0]);
 #pragma unroll
         for (int u = 0; u < 32; ++u) v[u] = u < in ? v[u] : 0.0f;
       } else {
@@ -856,7 +856,7 @@ __device__ __forceinline__ void load_few(const Product &P, const T *x, long long
   }
 }
 
-template <typename T, typename Y, bool PLANES>
+template <typename T, typename Y, bool PLANES, bool VEC>
 __global__ __launch_bounds__(64 * kFewWaves, 4) void mx_few_kernel(const Product P, int act) {
   __shared__ float part[kFewWaves][32][64];
   const int lane = threadIdx.x & 63, wave = wave_id(), S = P.all_steps;
@@ -872,11 +872,20 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void mx_few_kernel(const Product
     const unsigned sa = ws[(s >> 2) * 64ll * P.tiles_n] >> (8 * (s & 3));
     uint4 f[2];
     unsigned byte[2];
-    if constexpr (__is_same(T, Packed)) load_few<T, PLANES>(P, nullptr, p0, live, s, lane, f, byte);
-    else load_few<T, PLANES>(P, (const T *)P.x + image * P.xb + (PLANES ? p0 : p0 * P.xs1), p0, live, s, lane, f, byte);
+    if constexpr (__is_same(T, Packed)) load_few<T, PLANES, VEC>(P, nullptr, p0, live, s, lane, f, byte);
+    else load_few<T, PLANES, VEC>(P, (const T *)P.x + image * P.xb + (PLANES ? p0 : p0 * P.xs1), p0, live, s, lane, f, byte);
     mfma2<0>(acc, a, sa, f[0], f[1], byte[0], byte[1]);
   }
   const int waves = S < kFewWaves ? S : kFewWaves;
+  constexpr int R = 2048 / (64 * kFewWaves);   // results per thread
+  float bias[R] = {};
+  if (P.bias) {   // on their way before the sums meet
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long n = nt * 32ll + 16 * (lane >> 5) + ((r * kFewWaves + wave) & 15);
+      bias[r] = P.bias[n < P.n ? n : P.n - 1];
+    }
+  }
   if (wave < waves) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) part[wave][i][lane] = acc[i >> 4][i & 15];
@@ -884,35 +893,31 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void mx_few_kernel(const Product
   __syncthreads();
   Y *y = (Y *)P.y + image * P.pixels * P.n;
 #pragma unroll
-  for (int r = 0; r < 2048 / (64 * kFewWaves); ++r) {   // sums of the waves, in their order
+  for (int r = 0; r < R; ++r) {   // sums of the waves, in their order
     const int i = r * kFewWaves + wave;
-    const int px = PLANES && P.vec ? 2 * (lane & 31) + (i >> 4) : 32 * (i >> 4) + (lane & 31);
+    const int px = PLANES ? 2 * (lane & 31) + (i >> 4) : 32 * (i >> 4) + (lane & 31);
     const long long n = nt * 32ll + 16 * (lane >> 5) + (i & 15);
     float v = 0.0f;
-    for (int q = 0; q < waves; ++q) v += part[q][i][lane];
+#pragma unroll
+    for (int q = 0; q < kFewWaves; ++q) v += q < waves ? part[q][i][lane] : 0.0f;
     if (px < live && n < P.n) {
-      v += P.bias ? P.bias[n] : 0.0f;
+      v += bias[r];
       if (act) v = activate<LMI_ACT_SILU>(v);
       y[PLANES ? n * P.pixels + p0 + px : (p0 + px) * P.n + n] = (Y)v;
     }
   }
 }
 
-template <typename T, typename Y, bool PLANES> int launch_product(Product P, int act, long long batch, hipStream_t st) {
-  if constexpr (!__is_same(T, Packed)) {
-    const uintptr_t align = PLANES ? 2 * sizeof(T) : 16;
-    P.vec = (uintptr_t)P.x % align == 0 && P.xb * sizeof(T) % align == 0 && P.xs1 * sizeof(T) % align == 0;
-    if (PLANES) P.vec = P.vec && P.pixels % 2 == 0 && (uintptr_t)P.y % align == 0;
-  }
+template <typename T, typename Y, bool PLANES, bool VEC> int launch_by_size(Product P, int act, long long batch, hipStream_t st) {
   P.tiles_pixels = (unsigned)((P.pixels + kTile - 1) / kTile);
   const long long tiles = batch * P.tiles_pixels;
   if (tiles * P.tiles_n <= (__is_same(T, Packed) ? kFewTilesPacked : kFewTiles)) {
-    mx_few_kernel<T, Y, PLANES><<<dim3((unsigned)tiles, (unsigned)P.tiles_n), 64 * kFewWaves, 0, st>>>(P, act);
+    mx_few_kernel<T, Y, PLANES, VEC><<<dim3((unsigned)tiles, (unsigned)P.tiles_n), 64 * kFewWaves, 0, st>>>(P, act);
     return lmi_check_launch("lmi_mx_product");
   }
   if constexpr (PLANES) {
-    if (P.vec && P.all_steps == 1 && tiles >= 512) {
-      launch_wave_planes<T>(P, act, batch, st);
+    if (P.all_steps == 1 && tiles >= 512) {
+      launch_wave_planes<T, VEC>(P, act, batch, st);
       return lmi_check_launch("lmi_mx_product");
     }
   }
@@ -921,10 +926,19 @@ template <typename T, typename Y, bool PLANES> int launch_product(Product P, int
     if (P.pixels >= 1024 && (P.pixels + 255) / 256 * ((P.tiles_n + 4) / 5) >= 128) launch_rows<Y, 4>(P, act, st);
     else launch_rows<Y, 2>(P, act, st);
   } else {
-    if (P.vec) launch_stream<T, Y, PLANES, true>(P, act, batch, st);
-    else launch_stream<T, Y, PLANES, false>(P, act, batch, st);
+    launch_stream<T, Y, PLANES, VEC>(P, act, batch, st);
   }
   return lmi_check_launch("lmi_mx_product");
+}
+
+// VEC: rows, whole 16-byte words; planes, an even size
+template <typename T, typename Y, bool PLANES> int launch_product(const Product &P, int act, long long batch, hipStream_t st) {
+  bool vec = true;
+  if constexpr (PLANES) vec = P.pixels % 2 == 0;
+  else if constexpr (!__is_same(T, Packed)) vec = (uintptr_t)P.x % 16 == 0 && P.xb * sizeof(T) % 16 == 0 && P.xs1 * sizeof(T) % 16 == 0;
+  if (vec) return launch_by_size<T, Y, PLANES, true>(P, act, batch, st);
+  if constexpr (!__is_same(T, Packed)) return launch_by_size<T, Y, PLANES, false>(P, act, batch, st);
+  return LMI_OK;
 }
 
 bool float_type(int d) { return d == LMI_F32 || d == LMI_F16 || d == LMI_BF16; }
@@ -1037,6 +1051,7 @@ int lmi_mx_product(const lmi_mx_product_args *a, void *stream) {
   LMI_REQUIRE(lmi_is_aligned(a->w_packed, 16) && lmi_is_aligned(a->w_scales, 4), LMI_ERR_ALIGNMENT,
               "lmi_mx_product: w_packed must be 16-byte, w_scales 4-byte aligned");
   Product P = {};
+  LMI_REQUIRE(rows || a->pixels > 1, LMI_ERR_BAD_ARG, "lmi_mx_product: maps of one position are rows (LMI_MX_ROWS)");
   P.x = a->x;
   P.xs = (const unsigned *)a->x_scales;
   P.pixels = a->pixels;

@@ -90,6 +90,7 @@ def test_mx_arguments(L):
                 dict(layout=2), dict(x_stride=-1), dict(x_dtype=6, x_scales=None), dict(x_dtype=6, x_scales=4096, batch=2),
                 dict(x_dtype=6, x_scales=4096, layout=1)):
         assert _product(L, **bad) == -1, bad
+    assert _product(L, layout=1, pixels=1) == -1                 # maps of one pixel are rows
     assert _product(L, w_packed=4104) == -2
     many = dict(pixels=4096, k=512, n=512, x_stride=512)          # quantised into the workspace first: it has to be there
     need = 4096 * 512 // 2 + 4096 * 512 // 32

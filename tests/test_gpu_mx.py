@@ -114,7 +114,8 @@ def test_linear(m, k, n, act, dtype):
 @pytest.mark.parametrize("b,k,n,h,w,act", [(1, 1, 1, 1, 1, None), (1, 640, 640, 20, 20, "silu"), (3, 400, 75, 7, 13, "silu"), (2, 48, 16, 1, 5, None),
                                            (2, 33, 40, 9, 1, "silu"), (4, 96, 64, 40, 24, None), (1, 80, 32, 160, 96, "silu"), (5, 64, 80, 1, 1, "silu"),
                                            (1, 2600, 70, 3, 11, None), (2, 5000, 33, 4, 4, "silu"),
-                                           (2, 48, 40, 160, 128, "silu"), (1, 33, 16, 200, 168, None), (1, 64, 65, 182, 181, "silu")])
+                                           (2, 48, 40, 160, 128, "silu"), (1, 33, 16, 200, 168, None), (1, 64, 65, 182, 181, "silu"),
+                                           (3, 50, 40, 121, 101, "silu"), (2, 200, 330, 83, 61, None), (5, 40, 33, 1, 3, None), (2, 129, 64, 1, 65, "silu")])
 def test_pointwise(b, k, n, h, w, act, layout, dtype):
     ops, dt = _ops(), DTYPES[dtype]
     g = torch.Generator().manual_seed(k + n)
@@ -290,6 +291,23 @@ def test_far_maps():
     z = ops.mx_pointwise(big, ops.mx_quantize(wb))
     want, size = OM.product(_np(big[0, :, -1]).T, _np(wb))
     _close(z[0, :, -1].t(), want, size, 70, torch.float16, None)
+
+
+def test_odd_maps_end_where_they_end():
+    """Planes of odd size, the last ending with its allocation's last element, at addresses that are no multiple of a pair."""
+    ops = _ops()
+    for k, n, h, w in ((40, 24, 7, 9), (64, 40, 181, 183), (130, 70, 61, 83)):
+        wt = torch.randn(n, k).cuda() / k ** 0.5
+        wq = ops.mx_quantize(wt)
+        for dt in DTYPES.values():
+            buf = torch.full((1 + 2 * k * h * w,), float("nan"), dtype=dt, device="cuda")
+            x = buf[1:].view(2, k, h, w)
+            x.copy_(torch.randn(2, k, h, w))
+            guard = torch.full((2 * n * h * w + 3,), 5.0, dtype=dt, device="cuda")
+            y = ops.mx_pointwise(x, wq, out=guard[1:-2].view(2, n, h, w))
+            want, size = OM.product(_np(x.permute(0, 2, 3, 1)).reshape(-1, k), _np(wt))
+            _close(y.permute(0, 2, 3, 1).reshape(-1, n), want, size, k, dt, None)
+            assert guard[0] == 5 and (guard[-2:] == 5).all()
 
 
 def test_graphs_side_by_side():

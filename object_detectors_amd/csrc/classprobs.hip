@@ -631,7 +631,7 @@ __device__ __forceinline__ void insert2(float (&val)[2], int (&cls)[2], float v,
 
 // A thread per row, for rows side by side: a wave reads neighbouring rows' values of one class at a time.  The lists are kept by float
 // comparisons; a row that holds a NaN (or an infinity that made one) is gone through again in the order that puts NaN first.
-// 64 x 4 x 8400 rows of 16 bins (fp16, top 2): 32.9 us, 4.2 TB/s of 138 MB; the instructions that keep two best beside the softmax
+// 64 x 4 x 8400 rows of 16 bins (fp16, top 2): 31 us, 4.4 TB/s of 138 MB; the instructions that keep two best beside the softmax
 // take as long as the loads.  Two rows of a 16-bit type per thread, read as one word, halve the loads and the threads: no better here
 // (35.8 us) and worse for longer lists (64 x 8400 x 80, top 5: 90 us, 71 with one).
 template <typename T, int ACT, int KT>

@@ -267,8 +267,8 @@ __device__ __forceinline__ void store_nan(const Evidence &E, long long row, int 
   }
 }
 
-// 16 lanes per row, class j * 16 + l in value j of lane l.  64 x 300 kept rows of 80 classes (fp32, an anchor plane apart): 28.6 us
-// for 1.1 million scattered sectors of 64 bytes, 2.6 TB/s of what DRAM moves for them; one image's 300 rows: 6.7 us, two
+// 16 lanes per row, class j * 16 + l in value j of lane l.  64 x 300 kept rows of 80 classes (fp32, an anchor plane apart): 28 us
+// for 1.1 million scattered sectors of 64 bytes (68 MB), 2.4 TB/s; one image's 300 rows: 6.7 us, two
 // dependent loads and the arithmetic of one wave.  A wave per row took 52 and 17 us: fewer rows, and so sectors, in flight.
 template <typename T, int J, int ACT>
 __device__ __forceinline__ void evidence_team(const Evidence &E, long long row, long long rows) {

@@ -72,7 +72,7 @@ template <typename T, bool VEC> __device__ __forceinline__ void load8(const T *p
   }
 }
 
-// Bound by HBM: 409600 x 320 fp16 (331 MB in and out) 64 - 75 us, 4.4 - 5.2 TB/s; 640 x 2560 fp32 4 us, little above an empty kernel.
+// Bound by HBM: 409600 x 320 fp16 (331 MB in and out) 64 - 75 us, 4.4 - 5.2 TB/s; 640 x 2560 fp32 4 us.
 // lane = (row of the octet, block of the step, quarter of the block).  The wave reads 8 rows x 128 bytes (16-bit types) per step and writes 8 x 16
 // bytes side by side for either block; the scale bytes of its four steps leave as one word.
 template <typename T, bool VEC>
@@ -790,7 +790,7 @@ template <typename Y, int WP> void launch_rows(const Product &P, int act, hipStr
 
 // Few positions: 64 of them x 32 weight rows per workgroup, its eight waves share k.  A wave loads its steps' blocks straight into the
 // operands -- no LDS, no barrier before the sums meet; a workgroup's time is the latency of a load or two: a row of 1280 -> 1000 6.4 us, 640 -> 640
-// on 20 x 20 7.1, an empty kernel some 2.5.
+// on 20 x 20 7.1.
 constexpr int kFewWaves = 8;
 // Up to this many pairs of tiles, two workgroups per CU (us here and streamed, fp16: 640 -> 320 on 40 x 40, 25 x 10 of them, 7.9 and 9.9;
 // 320 -> 160 on 80 x 80, 100 x 5, 7.1 and 7.6; 4 x 640 -> 640 on 20 x 20, 28 x 20, 12.6 and 10.7; 4 x 320 -> 320 on 40 x 40, 100 x 10, 12.1 and

@@ -1034,7 +1034,8 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
     if planes and w == 1 and h > 1:
         planes = sh == 1
     rows = (k == 1 or sk == 1) and not planes and (h == 1 or w == 1 or sh == w * sw)
-    if (not planes and not rows) or (sk if planes else sw) >= 1 << 24:
+    step = sk if planes else sb if h * w == 1 else sw if w > 1 else sh   # between neighbouring channels or rows
+    if (not planes and not rows) or step >= 1 << 24:
         x = x.contiguous()
         sb, sk, sh, sw = x.stride()
         planes = h * w > 1

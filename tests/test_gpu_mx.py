@@ -145,6 +145,19 @@ def test_pointwise_odd_strides():
         _close(ops.mx_pointwise(x, wq).permute(0, 2, 3, 1).reshape(-1, 24), want, size, 40, torch.float16, None)
 
 
+def test_one_pixel_of_far_images():
+    """A pixel of every image of a channels-last batch whose images lie 2^24 elements apart, and of planes."""
+    ops = _ops()
+    w = torch.randn(20, 256).cuda() / 16
+    wq = ops.mx_quantize(w)
+    base = torch.randn(3, 256, 1, 1).half().cuda().expand(3, 256, 260, 260)
+    for fmt in (torch.channels_last, torch.contiguous_format):
+        x = base.contiguous(memory_format=fmt)
+        for v in (x[:, :, :1, :1], x[:, :, 259:, 259:]):
+            want, size = OM.product(_np(v).reshape(3, 256), _np(w))
+            _close(ops.mx_pointwise(v, wq).reshape(3, 20), want, size, 256, torch.float16, None)
+
+
 def test_non_finite_blocks_stay_in_their_row():
     """A NaN or an infinity makes the results of its own position NaN, and no other's."""
     ops = _ops()

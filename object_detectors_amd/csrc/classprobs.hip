@@ -5,8 +5,10 @@
 // kept, the distance bins behind every box side, or plain rows of a classifier.
 //
 // Mathematics, one pass over a row: m = max x, s = sum e^(x-m), t = sum e^(x-m)(x-m), kept up to date as m grows
-// (s *= e^(m-m'), t = (t + s(m-m')) e^(m-m')); then log Z = m + log s and H = log s - t/s.  s and t are sums of at most
-// some hundred terms per lane, added up over the lanes in fp32; values are fp32 whatever the input type.
+// (s *= e^(m-m'), t = (t + s(m-m')) e^(m-m')); then log Z = m + log s and H = log s - t/s.  Values and sums are fp32 whatever the input type.
+// A lane adds up at most 64 terms one after another; where it has more, the sums of such groups are added, and small steps of m applied, with
+// what each addition loses carried along, since a long sum of like terms rounds all of them the same way (30011 classes in a thread one by
+// one: log s 3e-4 off, an entropy of 16000 by 4; by groups within the bound of a sum of 64 terms, for any length).
 // The alternatives are ordered by a 64-bit key: the value's bits made monotonic above, the complemented class below, so
 // that equal values fall in class order and no two keys are equal (the result does not depend on the order of atomics).
 //
@@ -110,6 +112,36 @@ __device__ __forceinline__ void rebase(Sums &a, float m2) {
   }
   a.m = m2;
 }
+// A row's sums over many groups of values: what each addition loses (Kahan) is carried along.
+struct LongSums {
+  Sums a = {-INFINITY, 0.0f, 0.0f};
+  float lost_s = 0.0f, lost_t = 0.0f;
+  __device__ static __forceinline__ void add(float &sum, float &lost, float v) {
+    const float y = v - lost, n = sum + y;
+    lost = (n - sum) - y;
+    sum = n;
+  }
+  // a group's sums, with respect to g.m >= m
+  __device__ __forceinline__ void add(const Sums &g) {
+    if (a.m != g.m) {
+      const float d = a.m - g.m;
+      if (d > -0.25f) {   // a row that climbs slowly takes thousands of such steps: s += s(e^d - 1), e^d - 1 by its series, likewise t
+        const float r = d * fmaf(d, fmaf(d, fmaf(d, fmaf(d, fmaf(d, 1.0f / 720, 1.0f / 120), 1.0f / 24), 1.0f / 6), 0.5f), 1.0f);
+        add(a.t, lost_t, fmaf(a.t, r, a.s * d * (1.0f + r)));
+        add(a.s, lost_s, a.s * r);
+        a.m = g.m;
+      } else {            // what came before fades with every such step
+        const float f = a.m == -INFINITY ? 1.0f : exp_fast(d);
+        lost_s *= f;
+        lost_t *= f;
+        rebase(a, g.m);
+      }
+    }
+    add(a.s, lost_s, g.s);
+    add(a.t, lost_t, g.t);
+  }
+  __device__ __forceinline__ void add_entropy(float h) { add(a.t, lost_t, h); }
+};
 __device__ __forceinline__ void add_value(Sums &a, float ref, float x) {
   const float z = x - ref, e = exp_fast(z);
   a.s += e;
@@ -391,7 +423,7 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
   const int start = V > 1 ? -(int)(((uintptr_t)xp & 15) / sizeof(T)) : 0;
 
   if (t < kMaxTop) L.list[t] = 0;
-  Sums S = {-INFINITY, 0.0f, 0.0f};   // softmax: this thread's sums with respect to its own m; else t = the entropy
+  LongSums total;   // softmax: this thread's sums with respect to its own m; else t = the entropy
   constexpr int N = J * V;
   const T absent = (T)(ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);   // adds nothing to the sums
   for (long long tile = start; tile < len; tile += NT * N) {
@@ -412,6 +444,7 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
     }
     // a thread's own sums, group by group as the loads arrive: the exponentials of one run beside the loads of the next
     float mx = -INFINITY;
+    Sums S = {total.a.m, 0.0f, 0.0f};   // of this tile
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       float g = G::get(p[j], 0);
@@ -428,6 +461,9 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
         for (int u = 0; u < V; ++u) S.t += answer_entropy<ACT>(G::get(p[j], u));
       }
     }
+    const bool odd = S.t != S.t || (ACT == LMI_PROB_SOFTMAX && S.s != S.s);   // this thread's part of the tile holds a NaN, or an infinity that made one
+    if (ACT == LMI_PROB_SOFTMAX) total.add(S);
+    else total.add_entropy(S.t);
     if (E.top) {
       if (NT > 64) {
         L.lane_max[wave][lane] = mx;
@@ -451,7 +487,6 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
         thr = k != k ? INFINITY : fmaxf(thr, k);
       }
       forget(p);
-      const bool odd = S.t != S.t || (ACT == LMI_PROB_SOFTMAX && S.s != S.s);   // this thread has met a NaN, or an infinity that made one
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         float best = G::get(p[j], 0);
@@ -483,6 +518,7 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
     }
   }
   // sums over the wave, then over the team
+  Sums S = total.a;
   if (ACT == LMI_PROB_SOFTMAX) {
     rebase(S, reduce64(S.m, MaxF()));
     S.s = reduce64(S.s, SumF());
@@ -641,7 +677,7 @@ __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) 
   const long long o = (unsigned)row / (unsigned)E.n1, i = row - o * E.n1;   // fewer than 2^31 rows: a 64-bit division costs as much as four classes
   if (E.count && i >= E.count[o]) return;
   const T *x = (const T *)E.x + o * E.s0 + i * E.s1;
-  Sums S = {-INFINITY, 0.0f, 0.0f};
+  LongSums total;
   constexpr int KL = KT ? KT : 1;
   float val[KL];
   int cls[KL];
@@ -663,16 +699,19 @@ __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) 
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] = kAll || c + u < C ? to_float(w[u]) : (ACT == LMI_PROB_NONE ? 0.0f : -INFINITY);
     if (ACT == LMI_PROB_SOFTMAX) {
-      float mx = S.m;
+      float mx = total.a.m;
 #pragma unroll
       for (int u = 0; u < U; ++u) mx = fmaxf(mx, v[u]);
-      rebase(S, mx);
-      const float ref = finite_ref(mx);
+      Sums S = {mx, 0.0f, 0.0f};
+      const float ref = finite_ref(S.m);
 #pragma unroll
       for (int u = 0; u < U; ++u) add_value(S, ref, v[u]);
+      total.add(S);
     } else {
+      float h = 0.0f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) S.t += answer_entropy<ACT>(v[u]);
+      for (int u = 0; u < U; ++u) h += answer_entropy<ACT>(v[u]);
+      total.add_entropy(h);
     }
     if constexpr (KT == 2) {
       if (c > 0) insert2(val, cls, v[0], c);
@@ -688,8 +727,8 @@ __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) 
   int c = 0;
   for (; c + U <= C; c += U) take(c, std::true_type());
   if (c < C) take(c, std::false_type());
-  float ref = 0.0f, log_s = 0.0f, h = S.t;
-  if (ACT == LMI_PROB_SOFTMAX) softmax_result(S, ref, log_s, h);
+  float ref = 0.0f, log_s = 0.0f, h = total.a.t;
+  if (ACT == LMI_PROB_SOFTMAX) softmax_result(total.a, ref, log_s, h);
   if (E.entropy) E.entropy[row] = h;
   if (E.logprob) {
     const long long l = E.labels ? label_of(E, o, i) : -1;

@@ -363,3 +363,67 @@ def test_refusals():
                       (ValueError, lambda: ops.class_logprobs(x, out={"entropy": torch.empty(6, 4).cuda().t()}))):
         with pytest.raises(err):
             call()
+
+
+def _flat_rows(c):
+    """12 rows of c classes where many values are equal or climb slowly -- a long fp32 sum of such terms rounds every one of them the
+    same way --, beside a few that differ."""
+    gen = torch.Generator().manual_seed(c)
+    x = torch.empty(12, c)
+    for r, level in enumerate((-0.7, -3.3, -6.1, -8.0, -9.7)):
+        x[r] = level
+        x[r, (r * 37 + 5) % c] = 0.0                      # one peak above a flat background
+    x[5] = 1.3                                            # all equal
+    x[6] = torch.linspace(-1, 1, c)                       # climbs
+    x[7] = torch.linspace(-12, 9, c)
+    x[8] = torch.linspace(9, -12, c)                      # falls
+    x[9] = torch.randn(c, generator=gen)
+    x[10] = torch.where(torch.rand(c, generator=gen) < 0.9, -float("inf"), 0.7)
+    x[11] = torch.linspace(-40, 40, c)
+    return x
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", ["softmax", "sigmoid", "none"])
+@pytest.mark.parametrize("c,rows,top", [(8009, 16800, 2), (30011, 16800, 1), (4001, 132000, 5)])
+def test_long_planes_of_flat_values(c, rows, top, activation, dtype):
+    """Thousands of classes as planes, a thread per row: the error does not grow with the number of classes.  `sequential`: 16 terms added one
+    after another, the sum of such groups with what each addition loses carried along (4), steps of the maximum below 0.25 likewise, larger
+    ones 4 each, the earlier of them fading with e^-0.25 (4 / (1 - e^-0.25) = 18): 64 covers it."""
+    x = _flat_rows(c)
+    if activation == "none":
+        x = torch.sigmoid(x)
+    x = x.to(DTYPES[dtype])
+    labels = torch.tensor([(r * 37 + 5) % c for r in range(12)])
+    planes = x.t().contiguous().cuda().repeat(1, rows // 12)
+    r = _ops().class_logprobs(planes.t(), labels.repeat(rows // 12).cuda(), top=top, activation=activation)
+    for v in r.values():
+        v = v.reshape(rows // 12, -1).nan_to_num(nan=123.0)
+        assert (v == v[0]).all()
+    _check({k: v[:12] for k, v in r.items()}, x, labels, top, activation, sequential=64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,c", [(1, (1 << 27) + 1), (3, (1 << 25) + 77), (2049, 400009)])
+def test_very_long_flat_rows(rows, c, dtype):
+    """The same for rows whose classes lie side by side, by closed forms: a peak of 0 above c - 1 values v; 64 values of a thread's
+    added one after another at most, the rest as above.  Entropies of independent classes: c - 1 equal ones and the peak's."""
+    dt = DTYPES[dtype]
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    for level in (-0.703125, -3.3125):                   # exact in all three types
+        x = torch.full((1, c), level, dtype=dt, device="cuda")
+        x[0, 5] = 0.0
+        x = x.expand(rows, c)
+        labels = torch.full((rows,), 5, dtype=torch.int64, device="cuda")
+        r = _ops().class_logprobs(x, labels)
+        s = 1 + (c - 1) * np.exp(level)
+        log_s = np.log(s)
+        h = log_s - (c - 1) * np.exp(level) * level / s
+        unit = (64 + 64 + 8 + 4 * (np.log(c) + 1)) * ULP
+        assert (r["logprob"].cpu().double() + log_s).abs().max() <= unit + 4 * ULP * log_s
+        assert (r["entropy"].cpu().double() - h).abs().max() <= unit * (2 + 2 * (np.log(c) + 1))
+        e = np.log1p(np.exp(level)) - level * np.exp(level) / (1 + np.exp(level))
+        r = _ops().class_logprobs(x, labels, activation="sigmoid")
+        want = (c - 1) * e + np.log(2)
+        assert (r["entropy"].cpu().double() - want).abs().max() <= want * (2 * abs(level) + 12 + 64 + 64) * ULP

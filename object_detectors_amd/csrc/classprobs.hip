@@ -481,6 +481,7 @@ __device__ __forceinline__ void evidence_row(const Evidence &E, long long row, i
     if (E.top) {
       team_sync<NT>();
       float thr = L.threshold;
+      if (ACT == LMI_PROB_NONE && thr == 0.0f) thr = -INFINITY;   // perhaps the zeros of lanes without a class: values below zero may be the best there are
       const u64 kept = L.list[E.top - 1];
       if (kept) {
         const float k = order_value((unsigned)(kept >> 32));   // a NaN there: only NaNs can still be better

@@ -427,3 +427,15 @@ def test_very_long_flat_rows(rows, c, dtype):
         r = _ops().class_logprobs(x, labels, activation="sigmoid")
         want = (c - 1) * e + np.log(2)
         assert (r["entropy"].cpu().double() - want).abs().max() <= want * (2 * abs(level) + 12 + 64 + 64) * ULP
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,c,top", [(3, 129, 32), (5, 300, 7), (2, 2100, 32), (2, 20000, 32), (1, 70001, 32), (40, 131, 1)])
+def test_values_that_are_no_probabilities(n, c, top, dtype):
+    """Values below zero have no logarithm, but an order and a class: the alternatives name classes that exist."""
+    x = -1 - torch.rand(n, c, generator=torch.Generator().manual_seed(c))
+    x[-1] = 0.0                                           # and a row of zeros
+    x[-1, 7] = -0.5
+    x = x.to(DTYPES[dtype]).cuda()
+    labels = torch.zeros(n, dtype=torch.int64).cuda()
+    _check(_ops().class_logprobs(x, labels, top=top, activation="none"), x, labels, top, "none")

@@ -1030,6 +1030,10 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
     _mx_common("mx_pointwise", x, weight, bias, act, k)
     n = weight.shape[0]
     sb, sk, sh, sw = x.stride()
+    if b == 1:        # strides of dimensions of one element say nothing, however large
+        sb = k * h * w
+    if k == 1:
+        sk = h * w
     planes = (w == 1 or sw == 1) and (h == 1 or sh == w * (sw if w > 1 else 1)) and h * w > 1
     if planes and w == 1 and h > 1:
         planes = sh == 1
@@ -1037,7 +1041,7 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
     step = sk if planes else sb if h * w == 1 else sw if w > 1 else sh   # between neighbouring channels or rows
     if (not planes and not rows) or step >= 1 << 24:
         x = x.contiguous()
-        sb, sk, sh, sw = x.stride()
+        sb, sk, sh, sw = k * h * w, h * w, w, 1
         planes = h * w > 1
     if planes:
         y = _mx_out("mx_pointwise", out, x, (b, n, h, w), x.dtype)

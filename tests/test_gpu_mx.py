@@ -384,3 +384,28 @@ def test_refusals():
                       (TypeError, lambda: ops.mx_dequantize(x)), (TypeError, lambda: ops.mx_dequantize(w, torch.int8))):
         with pytest.raises(err):
             call()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_of_single_images_and_channels(dtype):
+    """Strides of dimensions of one element say nothing, however large: a pixel of one far-strided image, one channel of planes and of
+    channels-last maps, single images of every layout."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(3)
+    dt = DTYPES[dtype]
+    big = torch.zeros(1, 160, 160, 1280, dtype=dt, device="cuda")
+    big[:, 5, 7] = torch.randn(1280, generator=g).to(dt).cuda()
+    pixel = big.permute(0, 3, 1, 2)[:, :, 5:6, 7:8]
+    assert pixel.stride()[0] >= 1 << 24 and pixel.is_contiguous()
+    few = torch.randn(2, 3, 5, 7, generator=g).to(dt).cuda()
+    wide = lambda h, w: torch.as_strided(few, (1, 1, h, w), (1 << 25, 1 << 26, w, 1))
+    views = [pixel, wide(5, 7), wide(1, 6), wide(6, 1), wide(1, 1), torch.as_strided(few, (2, 1, 3, 5), (105, 1 << 27, 7, 1)),
+             torch.as_strided(few, (2, 1, 1, 1), (105, 1 << 27, 1 << 26, 1 << 25)), torch.as_strided(few, (1, 3, 5, 7), (1 << 30, 1, 21, 3)),
+             few[:1], few[:1].contiguous(memory_format=torch.channels_last)]
+    for v in views:
+        b, k, h, w = v.shape
+        weight = torch.randn(21, k, generator=g).cuda() / k ** 0.5
+        want, size = OM.product(_np(v.permute(0, 2, 3, 1)).reshape(-1, k), _np(weight))
+        got = ops.mx_pointwise(v, ops.mx_quantize(weight))
+        assert got.shape == (b, 21, h, w)
+        _close(got.permute(0, 2, 3, 1).reshape(-1, 21), want, size, k, dt, None)

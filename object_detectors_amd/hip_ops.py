@@ -751,6 +751,25 @@ def _two_strides(t: torch.Tensor, nd: int):
     return n[0], n[1], st[0], st[1]
 
 
+def _span(t: torch.Tensor):
+    """First byte of t and the one behind its last (t not empty)."""
+    first = t.data_ptr()
+    last = t.numel() - 1 if t.is_contiguous() else sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return first, first + (last + 1) * t.element_size()
+
+
+def _apart(what: str, results: dict, inputs: dict) -> None:
+    """Refuses results that lie in the memory of an input or of one another (None and empty tensors lie nowhere)."""
+    spans = [(name, *_span(t)) for name, t in inputs.items() if t is not None and t.numel()]
+    for name, t in results.items():
+        if t.numel():
+            first, last = _span(t)
+            for other, a, b in spans:
+                if first < b and a < last:
+                    raise ValueError(f"{what}: {name} lies in the memory of {other}")
+            spans.append((name, first, last))
+
+
 def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: int = 0, activation: str = "softmax",
                    index: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None, out: Optional[dict] = None) -> dict:
     """Log probability of given classes, entropy, and the `top` best classes of every row of x (..., C), classes last,
@@ -764,7 +783,7 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
     index (B, M) int32: row (b, m) is read at x[b, index[b, m]] of x (B, A, C) -- `anchor` of nms_v8; labels and results are
     (B, M) then.  count (B,) int32: rows m >= count[b] are skipped and the results there left as they are (unspecified in
     fresh ones).
-    out: a previous result of the same shapes to write into instead of allocating.
+    out: a previous result of the same shapes to write into instead of allocating; not in the memory of x, labels, index or count.
     Returns dict(logprob (...) if labels are given, entropy (...), and for top > 0 top_logprob, top_index (..., top)): fp32 and int32, best
     first, equal values in class order, NaN first.  Inference only: inputs that require a gradient are refused."""
     _need_cuda(x, "x")
@@ -807,10 +826,12 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
         t = res[key] = out.get(key)
         if t is None or t.shape != size or t.dtype != dtype or t.device != dev or not t.is_contiguous():
             raise ValueError(f"class_logprobs: out[{key!r}] must be a contiguous {dtype} tensor of shape {size} on x's device")
-    out = res
+    given, out = out is not None, res
     rows = math.prod(lead)
     if rows == 0:
         return out
+    if given:
+        _apart("class_logprobs", {f"out[{key!r}]": t for key, t in out.items()}, {"x": x, "labels": labels, "index": index, "count": count})
     if index is not None or count is not None:   # the two leading dimensions mean what they say
         if x.ndim != 3:
             raise ValueError("class_logprobs: count needs x (B,M,C)")

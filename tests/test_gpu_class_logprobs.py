@@ -439,3 +439,35 @@ def test_values_that_are_no_probabilities(n, c, top, dtype):
     x = x.to(DTYPES[dtype]).cuda()
     labels = torch.zeros(n, dtype=torch.int64).cuda()
     _check(_ops().class_logprobs(x, labels, top=top, activation="none"), x, labels, top, "none")
+
+
+def test_results_over_inputs_are_refused():
+    ops = _ops()
+    x = torch.randn(4, 6, 9).cuda()
+    labels, index, count = torch.zeros(4, 6).cuda(), torch.zeros(4, 6, dtype=torch.int32).cuda(), torch.full((4,), 6, dtype=torch.int32).cuda()
+    fresh = lambda: {"entropy": torch.zeros(4, 6).cuda(), "logprob": torch.zeros(4, 6).cuda(), "top_logprob": torch.zeros(4, 6, 1).cuda(),
+                     "top_index": torch.zeros(4, 6, 1, dtype=torch.int32).cuda()}
+    call = lambda out: ops.class_logprobs(x, labels, top=1, index=index, count=count, out=out)
+    call(fresh())
+    flat = x.view(-1)
+    for key, t in (("entropy", flat[20:44].view(4, 6)), ("top_logprob", flat[:24].view(4, 6, 1)), ("logprob", labels), ("top_index", index.unsqueeze(-1)),
+                   ("top_index", count.new_zeros(30)[:24].view(4, 6, 1))):
+        out = fresh()
+        out[key] = t
+        if key == "top_index" and t.data_ptr() != index.data_ptr():
+            call(out)                                     # a part of a larger tensor is fine
+            continue
+        with pytest.raises(ValueError, match="memory of"):
+            call(out)
+    out = fresh()
+    out["logprob"] = out["entropy"]                       # two results in one place
+    with pytest.raises(ValueError, match="memory of"):
+        call(out)
+    both = torch.zeros(2, 4, 6).cuda()                    # side by side is fine
+    out = dict(fresh(), entropy=both[0], logprob=both[1])
+    want = call(fresh())
+    assert all(torch.equal(v, want[k]) for k, v in call(out).items())
+    one = torch.zeros(1, dtype=torch.int32).cuda()
+    with pytest.raises(ValueError, match="memory of"):
+        ops.class_logprobs(x[:1, :1], top=1, count=one, out={"entropy": torch.zeros(1, 1).cuda(), "top_logprob": torch.zeros(1, 1, 1).cuda(),
+                                                            "top_index": one.view(1, 1, 1)})

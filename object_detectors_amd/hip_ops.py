@@ -990,15 +990,14 @@ def _mx_common(what, x, weight, bias, act, k):
         raise ValueError(f"{what}: unknown activation {act!r} (None or 'silu')")
 
 
-def _mx_out(what, out, x, shape, dtype, memory_format=torch.contiguous_format):
+def _mx_out(what, out, x, weight, bias, shape, dtype, memory_format=torch.contiguous_format):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=x.device, memory_format=memory_format)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != x.device or not out.is_contiguous(memory_format=memory_format):
         raise ValueError(f"{what}: `out` must be a {dtype} tensor of shape {tuple(shape)} in {memory_format} on x's device")
-    for t in (x.packed, x.scales) if isinstance(x, MxTensor) else (x,):   # every result needs whole rows of x, which others overwrite by then
-        first, last = t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-        if t.numel() and out.numel() and first < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < last:
-            raise ValueError(f"{what}: `out` lies in the memory of x")
+    if out.numel():   # every result needs whole rows of x and of the weights, which others overwrite by then
+        parts = {"x": x.packed, "x's scales": x.scales} if isinstance(x, MxTensor) else {"x": x}
+        _apart(what, {"`out`": out}, {**parts, "weight": weight.packed, "weight's scales": weight.scales, "bias": bias})
     return out
 
 
@@ -1006,7 +1005,8 @@ def mx_linear(x: Union[torch.Tensor, MxTensor], weight: MxTensor, bias: Optional
               dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x weight^T + bias) with both factors in MXFP4 and fp32 sums: x (..., k) is quantised as `mx_quantize` does it, on the
     fly, or comes quantised (MxTensor); weight MxTensor (n, k); bias fp32 (n,); act None | 'silu'.
-    dtype: of the result, x's own (which it must be if given) or, for an MxTensor, float32 unless said otherwise.  Inference only."""
+    dtype: of the result, x's own (which it must be if given) or, for an MxTensor, float32 unless said otherwise.
+    out: a tensor to write into, not in the memory of x, weight or bias.  Inference only."""
     quantised = isinstance(x, MxTensor)
     if quantised:
         _need_mx(x, "x")
@@ -1024,7 +1024,7 @@ def mx_linear(x: Union[torch.Tensor, MxTensor], weight: MxTensor, bias: Optional
         raise ValueError("mx_linear: x must be (..., k)")
     k = x.shape[-1]
     _mx_common("mx_linear", x.packed if quantised else x, weight, bias, act, k)
-    y = _mx_out("mx_linear", out, x, tuple(x.shape[:-1]) + (weight.shape[0],), dtype)
+    y = _mx_out("mx_linear", out, x, weight, bias, tuple(x.shape[:-1]) + (weight.shape[0],), dtype)
     m = math.prod(x.shape[:-1])
     if quantised:
         return _mx_product("mx_linear", x.packed.data_ptr(), x.scales.data_ptr(), _lib.LMI_MXFP4, 1, m, k, 0, 0, weight, bias, act, y, _lib.LMI_MX_ROWS)
@@ -1041,7 +1041,8 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A 1x1 convolution in MXFP4: x (B, k, H, W) fp32 / fp16 / bf16, quantised on the fly in blocks of 32 channels of a pixel,
     weight MxTensor (n, k), bias fp32 (n,), act None | 'silu', fp32 sums.  Returns (B, n, H, W) of x's dtype, channels-last
-    if x is.  Channel slices of a larger map (`chunk` along dim 1) are read in place.  Inference only."""
+    if x is.  Channel slices of a larger map (`chunk` along dim 1) are read in place.  out: a tensor to write into, not in the memory of x,
+    weight or bias.  Inference only."""
     _need_cuda(x, "x")
     if x.dtype not in _FLOAT_DTYPES:
         raise TypeError("mx_pointwise: x must be float32, float16 or bfloat16")
@@ -1065,10 +1066,10 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
         sb, sk, sh, sw = k * h * w, h * w, w, 1
         planes = h * w > 1
     if planes:
-        y = _mx_out("mx_pointwise", out, x, (b, n, h, w), x.dtype)
+        y = _mx_out("mx_pointwise", out, x, weight, bias, (b, n, h, w), x.dtype)
         return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], b, h * w, k, sb, sk, weight, bias, act, y, _lib.LMI_MX_PLANES)
     fmt = torch.channels_last if h * w > 1 else torch.contiguous_format   # one pixel: both are the same memory
-    y = _mx_out("mx_pointwise", out, x, (b, n, h, w), x.dtype, fmt)
+    y = _mx_out("mx_pointwise", out, x, weight, bias, (b, n, h, w), x.dtype, fmt)
     if h * w == 1:       # an image per row
         return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], 1, b, k, 0, sb, weight, bias, act, y, _lib.LMI_MX_ROWS)
     return _mx_product("mx_pointwise", x.data_ptr(), None, _FLOAT_DTYPES[x.dtype], b, h * w, k, sb, sw if w > 1 else sh, weight, bias, act, y,

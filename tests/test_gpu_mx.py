@@ -409,3 +409,17 @@ def test_strides_of_single_images_and_channels(dtype):
         got = ops.mx_pointwise(v, ops.mx_quantize(weight))
         assert got.shape == (b, 21, h, w)
         _close(got.permute(0, 2, 3, 1).reshape(-1, 21), want, size, k, dt, None)
+
+
+def test_results_over_weights_and_biases_are_refused():
+    ops = _ops()
+    w = torch.randn(64, 64).cuda()
+    wq, bias = ops.mx_quantize(w), torch.randn(64).cuda()
+    x, m = torch.randn(1, 64).cuda(), torch.randn(1, 64, 4, 4).cuda()
+    over = wq.packed.view(-1).view(torch.float32)
+    scales = wq.scales.view(-1).view(torch.float32)
+    for call in (lambda: ops.mx_linear(x, wq, bias, out=bias.view(1, 64)), lambda: ops.mx_linear(x, wq, out=over[:64].view(1, 64)),
+                 lambda: ops.mx_linear(x, wq, out=scales[64:].view(1, 64)), lambda: ops.mx_pointwise(m[:, :, :1, :1], wq, bias, out=bias.view(1, 64, 1, 1)),
+                 lambda: ops.mx_pointwise(m[:, :, :1, 1:2], wq, out=over[:64].view(1, 64, 1, 1))):
+        with pytest.raises(ValueError, match="memory of"):
+            call()

@@ -722,8 +722,19 @@ def _launch(entry, args, device: torch.device, *more) -> None:
         check(status)
 
 
+def _not_traced(what: str) -> None:
+    """A trace (torch.jit.trace, make_fx) records torch's own operations: of the ones below it would keep the allocation of the result and not the kernel
+    that fills it.  Refused.  (torch.compile breaks its graph at the calls below and runs them as they are.)"""
+    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None):
+        raise RuntimeError(f"{what} cannot be traced: its kernel would be missing from the graph")
+
+
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
 def _no_gradient(what: str, *tensors) -> None:
-    """The operators below serve inference: a graph they would silently cut is refused."""
+    """The operators below serve inference: a graph they would silently cut is refused, and a trace."""
+    _not_traced(what)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() / inference_mode(), or detach its inputs")
 
@@ -948,6 +959,7 @@ def _need_mx(q, name: str) -> None:
 def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values an MxTensor stands for (exact in fp32 and, within its range, bf16; fp16 rounds what lies outside its range)."""
     _need_mx(q, "q")
+    _not_traced("mx_dequantize")
     if dtype not in _FLOAT_DTYPES:
         raise TypeError("mx_dequantize: dtype must be float32, float16 or bfloat16")
     y = torch.empty(q.shape, dtype=dtype, device=q.device)

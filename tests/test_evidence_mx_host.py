@@ -132,3 +132,21 @@ def test_oracle_evidence_by_hand():
     assert np.allclose(r["entropy"], np.log(2)) and np.allclose(r["logprob"], np.log(0.5)) and r["top_index"].tolist() == [[2, 0, 1]]
     r = OC.evidence([[0.0, 1000.0]], [1], 1, "sigmoid")
     assert np.allclose(r["entropy"], np.log(2)) and r["logprob"][0] == 0 and r["top_index"].tolist() == [[1]]
+
+
+def test_traces_are_refused():
+    """What the operators' common check says where a trace is under way (entry points: the GPU tests)."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from object_detectors_amd import hip_ops as ops
+
+    def f(t):
+        ops._no_gradient("mx_linear", t, None)
+        return t + 1
+    x = torch.zeros(3)
+    f(x)
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(f, x, check_trace=False)
+        with pytest.raises(RuntimeError, match="trace"):
+            make_fx(f)(x)
+    f(x)

@@ -423,3 +423,23 @@ def test_results_over_weights_and_biases_are_refused():
                  lambda: ops.mx_pointwise(m[:, :, :1, 1:2], wq, out=over[:64].view(1, 64, 1, 1))):
         with pytest.raises(ValueError, match="memory of"):
             call()
+
+
+def test_tracing_is_refused():
+    """A trace would hold the allocation of the result and not the product."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from object_detectors_amd.nets.yolov8 import ConvBNAct, MxPointwise
+    ops = _ops()
+    x = torch.randn(1, 64, 4, 4).cuda()
+    net = torch.nn.Sequential(MxPointwise.of(ConvBNAct(64, 32).eval().cuda())).eval()
+    with torch.no_grad():
+        want = net(x)
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(net, x, check_trace=False)
+        assert torch.equal(net(x), want)                  # and nothing stays behind
+    q = ops.mx_quantize(torch.randn(8, 64).cuda())
+    for f in (lambda t: ops.class_logprobs(t)["entropy"], lambda t: ops.mx_dequantize(ops.mx_quantize(t)), lambda t: ops.mx_linear(t, q)):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(f, torch.randn(3, 64).cuda(), check_trace=False)
+        with pytest.raises(RuntimeError, match="trace"):
+            make_fx(f)(torch.randn(3, 64).cuda())

@@ -15,6 +15,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import LMI_F16, LMI_F32, LMI_U8, check, lmi_frame
@@ -733,8 +734,10 @@ _PROXY = torch._C._TorchDispatchModeKey.PROXY
 
 
 def _no_gradient(what: str, *tensors) -> None:
-    """The operators below serve inference: a graph they would silently cut is refused, and a trace."""
+    """The operators below serve inference: a graph they would silently cut is refused, and so are tangents of forward mode, and a trace."""
     _not_traced(what)
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it on the primals (torch.autograd.forward_ad.unpack_dual)")
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() / inference_mode(), or detach its inputs")
 

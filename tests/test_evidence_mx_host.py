@@ -150,3 +150,16 @@ def test_traces_are_refused():
         with pytest.raises(RuntimeError, match="trace"):
             make_fx(f)(x)
     f(x)
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    from object_detectors_amd import hip_ops as ops
+    x = torch.zeros(3)
+    with torch.no_grad(), fw.dual_level():
+        ops._no_gradient("mx_linear", x, None)
+        d = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops._no_gradient("mx_linear", d, None), lambda: ops._no_gradient("mx_linear", x, d)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+    ops._no_gradient("mx_linear", x)

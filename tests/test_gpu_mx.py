@@ -443,3 +443,18 @@ def test_tracing_is_refused():
             torch.jit.trace(f, torch.randn(3, 64).cuda(), check_trace=False)
         with pytest.raises(RuntimeError, match="trace"):
             make_fx(f)(torch.randn(3, 64).cuda())
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+    ops = _ops()
+    x, w = torch.randn(4, 64).cuda(), ops.mx_quantize(torch.randn(8, 64).cuda())
+    with torch.no_grad(), fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        bias = fw.make_dual(torch.zeros(8).cuda(), torch.ones(8).cuda())
+        maps = d.view(1, 64, 2, 2)
+        for call in (lambda: ops.class_logprobs(d), lambda: ops.mx_quantize(d), lambda: ops.mx_linear(d, w), lambda: ops.mx_linear(x, w, bias),
+                     lambda: ops.mx_pointwise(maps, w)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        ops.mx_linear(x, w)                               # what carries no tangent passes

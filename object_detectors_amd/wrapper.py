@@ -24,6 +24,7 @@ from typing import Union
 import numpy as np
 import torch
 
+from ._lib import LMI_MAX_TOP
 from .segments import masks2segments
 
 
@@ -80,7 +81,7 @@ class Yolov8Core:
     sync_time_info = False
     # > 0: results also carry, per detection, 'logprobs' (log probability of its class), 'entropy' (summed over the classes'
     # yes / no answers) and 'alternatives' (that many best classes as (name, log probability), best first) -- one more
-    # kernel on the rows NMS kept (hip_ops.class_logprobs).
+    # kernel on the rows NMS kept (hip_ops.class_logprobs).  At most 32 (all classes, if the model has fewer).
     alternatives = 0
     # True: the network's 1x1 convolutions (backbone and neck) run in MXFP4 (this package's own networks; set before construction)
     mx_weights = False
@@ -101,6 +102,7 @@ class Yolov8Core:
                 raise TypeError(f'mx_weights needs one of this package\'s networks, not {type(self.model).__name__}')
             self.model.quantize_pointwise()
         self.names = self.model.names
+        self._alternatives(len(self.names))
         self._thres_cache = {}
 
     # ---- forward / helpers (model.py:75-108) -----------------------------------------------------
@@ -258,9 +260,16 @@ class Yolov8Core:
     # ---- additive: evidence of the kept detections ----------------------------------------------
     _EVIDENCE = ('logprobs', 'entropy', 'alternatives')
 
+    def _alternatives(self, nc):
+        """How many alternatives of `nc` classes are wanted; refused where the kernel does not return so many."""
+        k = min(int(self.alternatives), nc)
+        if k > LMI_MAX_TOP:
+            raise ValueError(f'alternatives={self.alternatives} of {nc} classes: at most {LMI_MAX_TOP}')
+        return k
+
     def _evidence(self, preds, det, count, anchor, nc):
         """[logprob, entropy, top_logprob, top_index] of the NMS rows on the device, [] unless `alternatives` is set."""
-        k = min(int(self.alternatives), nc)
+        k = self._alternatives(nc)
         if k <= 0:
             return []
         r = _hip_ops().class_logprobs(preds[:, 4:4 + nc].transpose(1, 2), det[:, :, 5], top=k, activation='none', index=anchor, count=count)
@@ -285,6 +294,7 @@ class Yolov8Core:
     @torch.inference_mode()
     def postprocess(self, preds, img, orig_imgs, conf: Union[float, dict], iou=0.45, agnostic=False, max_det=300, return_segments=True,
                     _masks_on_device=False, _with_index=False):
+        self._alternatives(len(self.model.names))
         if isinstance(preds, (list, tuple)):
             predict_mask = preds[0].shape[1] != 4 + len(self.model.names)
         elif isinstance(preds, torch.Tensor):
@@ -519,6 +529,7 @@ class Yolov8PoseCore(Yolov8Core):
 
     @torch.inference_mode()
     def postprocess(self, preds, img, orig_imgs, conf: Union[float, dict], iou=0.45, agnostic=False, max_det=300):
+        self._alternatives(len(self.model.names))
         if isinstance(preds, (list, tuple)):
             preds = preds[0]
         if not isinstance(preds, torch.Tensor):
@@ -608,6 +619,7 @@ class Yolov8ObbCore(Yolov8Core):
 
     @torch.inference_mode()
     def postprocess(self, preds, img, orig_imgs, conf: Union[float, dict], iou=0.45, agnostic=False, max_det=300):
+        self._alternatives(len(self.model.names))
         if not isinstance(preds, (torch.Tensor, list, tuple)):
             self.logger.error(f'Prediction type {type(preds)} not supported expected torch.Tensor or list')
             raise TypeError(f'Prediction type {type(preds)} not supported expected torch.Tensor or list')

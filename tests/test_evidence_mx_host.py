@@ -163,3 +163,39 @@ def test_tangents_are_refused():
             with pytest.raises(RuntimeError, match="no gradient"):
                 call()
     ops._no_gradient("mx_linear", x)
+
+
+def test_alternatives_beyond_the_operators_limit():
+    """Refused when the model is built or before anything else is done with a prediction, not halfway; never for models of few classes."""
+    from object_detectors_amd.wrapper import Yolov8Core, Yolov8ObbCore, Yolov8PoseCore
+    for base in (Yolov8Core, Yolov8PoseCore, Yolov8ObbCore):
+        m = base.__new__(base)
+        m.device = torch.device("cpu")
+        m.model = type("Net", (), {"names": {i: str(i) for i in range(40)}, "kpt_shape": (1, 2)})()
+        call = lambda: m.postprocess(torch.zeros(1, 44, 8), torch.zeros(1, 3, 8, 8), [np.zeros((8, 8, 3), np.uint8)], 0.2)
+        m.alternatives = 33
+        with pytest.raises(ValueError, match="alternatives"):
+            call()
+        for fine in (32, 0, -1):
+            m.alternatives = fine
+            with pytest.raises((RuntimeError, ValueError)) as e:
+                call()                                    # there is no GPU path here; the count is not what stops it
+            assert "alternatives" not in str(e.value)
+        m.alternatives = 1000                             # all of them, if they are few
+        m.model.names = {0: "a", 1: "b"}
+        with pytest.raises((RuntimeError, ValueError)) as e:
+            call()
+        assert "alternatives" not in str(e.value)
+
+
+def test_alternatives_beyond_the_limit_at_construction(tmp_path):
+    from object_detectors_amd.nets.yolov8 import YoloV8
+    from object_detectors_amd.wrapper import Yolov8Core
+    names = {i: str(i) for i in range(40)}
+    path = str(tmp_path / "w.pt")
+    torch.save({"format": "lmi-yolov8-torch", "scale": "n", "nc": 40, "seg": False, "names": names, "state_dict": YoloV8("n", 40, names=names).state_dict()}, path)
+
+    class Model(Yolov8Core):
+        alternatives = 33
+    with pytest.raises(ValueError, match="alternatives"):
+        Model.__new__(Model)._init(path, device="cpu")

@@ -46,9 +46,19 @@ class MxPointwise(nn.Module):
         self.register_buffer("bias", bias.float().contiguous())
         self.size, self.act = tuple(weight.shape), act
 
+    @staticmethod
+    def misfit(m):
+        """Why m cannot become such a layer (None: it can)."""
+        if isinstance(m, ConvBNAct) and not isinstance(m.act, (nn.SiLU, nn.Identity)):
+            return f"no activation {type(m.act).__name__}"
+        return None
+
     @classmethod
     def of(cls, m):
-        """From a ConvBNAct or an nn.Conv2d with a 1x1 kernel."""
+        """From a ConvBNAct (SiLU or no activation) or an nn.Conv2d with a 1x1 kernel."""
+        why = cls.misfit(m)
+        if why:
+            raise TypeError(f"MxPointwise: {why}")
         conv = m.conv if isinstance(m, ConvBNAct) else m
         w = conv.weight.detach().float().flatten(1)
         bias = torch.zeros(w.shape[0], device=w.device) if conv.bias is None else conv.bias.detach().float()
@@ -217,7 +227,7 @@ class YoloV8(nn.Module):
     @torch.no_grad()
     def quantize_pointwise(self, head=False):
         """Replaces the 1x1 convolutions of backbone and neck (head=True: the head's last layers too) by their MXFP4 form, in
-        place.  The model must be in eval mode and on the GPU.  Returns how many were replaced."""
+        place; those whose activation it lacks stay as they are.  The model must be in eval mode and on the GPU.  Returns how many were replaced."""
         if self.training:
             raise RuntimeError("quantize_pointwise folds the batch norms: call eval() first")
         todo = []
@@ -228,7 +238,8 @@ class YoloV8(nn.Module):
                 continue
             for key, m in parent.named_children():
                 conv = m.conv if isinstance(m, ConvBNAct) else m
-                if isinstance(conv, nn.Conv2d) and conv.kernel_size == (1, 1) and conv.stride == (1, 1) and conv.groups == 1:
+                if isinstance(conv, nn.Conv2d) and conv.kernel_size == (1, 1) and conv.stride == (1, 1) and conv.groups == 1 \
+                        and not MxPointwise.misfit(m):
                     todo.append((parent, key, m))
         for parent, key, m in todo:
             setattr(parent, key, MxPointwise.of(m))

@@ -199,3 +199,20 @@ def test_alternatives_beyond_the_limit_at_construction(tmp_path):
         alternatives = 33
     with pytest.raises(ValueError, match="alternatives"):
         Model.__new__(Model)._init(path, device="cpu")
+
+
+def test_activations_that_the_products_lack_stay_as_they_are(monkeypatch):
+    """quantize_pointwise replaces what the quantised layer can stand for, and nothing else."""
+    from object_detectors_amd.nets.yolov8 import ConvBNAct, MxPointwise, YoloV8
+    with pytest.raises(TypeError, match="ReLU"):
+        m = ConvBNAct(8, 8).eval()
+        m.act = torch.nn.ReLU()
+        MxPointwise.of(m)
+    net = YoloV8("n", 2).eval()
+    mine = [m for name, m in net.named_modules() if isinstance(m, ConvBNAct) and m.conv.kernel_size == (1, 1) and not name.startswith("head")]
+    for i, m in enumerate(mine):
+        m.act = torch.nn.ReLU() if i % 3 == 0 else torch.nn.Identity() if i % 3 == 1 else m.act
+    taken = []
+    monkeypatch.setattr(MxPointwise, "of", classmethod(lambda cls, m: taken.append(m) or torch.nn.Identity()))
+    assert net.quantize_pointwise() == len(taken) == sum(i % 3 != 0 for i in range(len(mine)))
+    assert all(m not in taken and any(m is q for q in net.modules()) for m in mine[::3])

@@ -49,6 +49,10 @@ class MxPointwise(nn.Module):
     @staticmethod
     def misfit(m):
         """Why m cannot become such a layer (None: it can)."""
+        conv = m.conv if isinstance(m, ConvBNAct) else m
+        if not isinstance(conv, nn.Conv2d) or conv.kernel_size != (1, 1) or conv.stride != (1, 1) or conv.groups != 1 \
+                or conv.padding not in ((0, 0), "same", "valid"):   # with a 1x1 kernel "same" pads nothing
+            return "not a 1x1 convolution without stride, groups and padding"
         if isinstance(m, ConvBNAct) and not isinstance(m.act, (nn.SiLU, nn.Identity)):
             return f"no activation {type(m.act).__name__}"
         return None
@@ -227,7 +231,7 @@ class YoloV8(nn.Module):
     @torch.no_grad()
     def quantize_pointwise(self, head=False):
         """Replaces the 1x1 convolutions of backbone and neck (head=True: the head's last layers too) by their MXFP4 form, in
-        place; those whose activation it lacks stay as they are.  The model must be in eval mode and on the GPU.  Returns how many were replaced."""
+        place; those with padding, or an activation it lacks, stay as they are.  The model must be in eval mode and on the GPU.  Returns how many were replaced."""
         if self.training:
             raise RuntimeError("quantize_pointwise folds the batch norms: call eval() first")
         todo = []
@@ -237,9 +241,7 @@ class YoloV8(nn.Module):
             if isinstance(parent, ConvBNAct):
                 continue
             for key, m in parent.named_children():
-                conv = m.conv if isinstance(m, ConvBNAct) else m
-                if isinstance(conv, nn.Conv2d) and conv.kernel_size == (1, 1) and conv.stride == (1, 1) and conv.groups == 1 \
-                        and not MxPointwise.misfit(m):
+                if not MxPointwise.misfit(m):
                     todo.append((parent, key, m))
         for parent, key, m in todo:
             setattr(parent, key, MxPointwise.of(m))

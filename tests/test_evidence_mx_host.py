@@ -216,3 +216,21 @@ def test_activations_that_the_products_lack_stay_as_they_are(monkeypatch):
     monkeypatch.setattr(MxPointwise, "of", classmethod(lambda cls, m: taken.append(m) or torch.nn.Identity()))
     assert net.quantize_pointwise() == len(taken) == sum(i % 3 != 0 for i in range(len(mine)))
     assert all(m not in taken and any(m is q for q in net.modules()) for m in mine[::3])
+
+
+def test_padded_convolutions_stay_as_they_are(monkeypatch):
+    from object_detectors_amd.nets.yolov8 import ConvBNAct, MxPointwise, YoloV8
+    padded = torch.nn.Conv2d(8, 8, 1, padding=1)
+    with pytest.raises(TypeError, match="1x1"):
+        MxPointwise.of(padded)
+    with pytest.raises(TypeError, match="1x1"):
+        MxPointwise.of(torch.nn.Conv2d(8, 8, 3))
+    net = YoloV8("n", 2).eval()
+    mine = [m for name, m in net.named_modules() if isinstance(m, ConvBNAct) and m.conv.kernel_size == (1, 1) and not name.startswith("head")]
+    mine[0].conv.padding = (1, 1)
+    mine[1].conv.padding = (0, 2)
+    mine[2].conv = torch.nn.Conv2d(mine[2].conv.in_channels, mine[2].conv.out_channels, 1, bias=False, padding="same")     # adds nothing
+    taken = []
+    monkeypatch.setattr(MxPointwise, "of", classmethod(lambda cls, m: taken.append(m) or torch.nn.Identity()))
+    assert net.quantize_pointwise() == len(taken) == len(mine) - 2
+    assert mine[0] not in taken and mine[1] not in taken and mine[2] in taken

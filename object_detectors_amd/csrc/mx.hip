@@ -932,14 +932,15 @@ template <typename T, typename Y, bool PLANES, bool VEC> int launch_by_size(Prod
   return lmi_check_launch("lmi_mx_product");
 }
 
-// VEC: rows, whole 16-byte words; planes, an even size
+// VEC: rows, whole 16-byte words (quantised ones are nothing else); planes, an even size
 template <typename T, typename Y, bool PLANES> int launch_product(const Product &P, int act, long long batch, hipStream_t st) {
-  bool vec = true;
-  if constexpr (PLANES) vec = P.pixels % 2 == 0;
-  else if constexpr (!__is_same(T, Packed)) vec = (uintptr_t)P.x % 16 == 0 && P.xb * sizeof(T) % 16 == 0 && P.xs1 * sizeof(T) % 16 == 0;
-  if (vec) return launch_by_size<T, Y, PLANES, true>(P, act, batch, st);
-  if constexpr (!__is_same(T, Packed)) return launch_by_size<T, Y, PLANES, false>(P, act, batch, st);
-  return LMI_OK;
+  if constexpr (__is_same(T, Packed)) {
+    return launch_by_size<T, Y, PLANES, true>(P, act, batch, st);
+  } else {
+    const bool vec = PLANES ? P.pixels % 2 == 0 : (uintptr_t)P.x % 16 == 0 && P.xb * sizeof(T) % 16 == 0 && P.xs1 * sizeof(T) % 16 == 0;
+    if (vec) return launch_by_size<T, Y, PLANES, true>(P, act, batch, st);
+    return launch_by_size<T, Y, PLANES, false>(P, act, batch, st);
+  }
 }
 
 bool float_type(int d) { return d == LMI_F32 || d == LMI_F16 || d == LMI_BF16; }
@@ -984,8 +985,8 @@ struct Sizes {
 
 // Rows that come as floats and meet many weight rows are quantised once, into the workspace, where they would be quantised again for
 // every 320 weight rows or fewer: 8192 x 1280 -> 2560 (fp16) 34 us, 59 without; 102400 x 1280 -> 640 149 and 183; 128 x 1280 -> 32000 42 and
-// 156.  Few pairs of tiles (those that the waves of mx_few_kernel share in one round), 256 weight rows or k <= 128 do not
-// pay for the second kernel: 102400 x 1280 -> 160 98 us, 79 without; 8192 x 96 -> 640 11.4 and 9.9.
+// 156.  From 320 pairs of tiles on that pays whichever kernel multiplies then (2048 x 1280 -> 320, 320 pairs, both times mx_few_kernel: 10.7 us, as
+// floats 15.4; k = 2560 14.3 and 25.5; k = 256 8.6 and 7.4).  Fewer pairs, 256 weight rows or k <= 128 do not pay for the second kernel: 102400 x 1280 -> 160 98 us, 79 without; 8192 x 96 -> 640 11.4 and 9.9.
 constexpr int64_t kQuantiseN = 256, kQuantiseK = 128;
 bool quantise_first(const lmi_mx_product_args *a) {
   if (a->layout != LMI_MX_ROWS || !float_type(a->x_dtype) || a->batch < 1 || a->n <= kQuantiseN || a->k <= kQuantiseK) return false;

@@ -473,6 +473,7 @@ int64_t lmi_trace_contours_host(const uint64_t *words, int64_t m, const int32_t 
  * [0, classes) gives NaN.
  * Outputs [device], any of them NULL if not wanted, contiguous: logprob (n0,n1), entropy (n0,n1) fp32; top_logprob fp32 and
  * top_index int32 (n0,n1,top), best first, equal values in the order of their classes, NaN before everything else.
+ * Each in memory of its own: a result over an input or another result is refused (LMI_ERR_BAD_ARG).
  * 0 <= top <= min(classes, LMI_MAX_TOP).  `workspace` [device] of lmi_class_logprobs_workspace_bytes; none is needed below
  * LMI_LOGPROB_SPLIT_FROM classes or from 256 rows on.
  */

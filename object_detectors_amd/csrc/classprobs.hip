@@ -838,6 +838,37 @@ template <typename T> int launch_act(const Evidence &E, int act, hipStream_t st)
   return launch<T, LMI_PROB_NONE>(E, st);
 }
 
+// memory of a call, as addresses [first, last)
+struct Range {
+  const char *name;
+  uintptr_t first, last;
+};
+// `elements` of `size` bytes each from p on, the last dimension's among them; then two more dimensions
+Range range_of(const char *name, const void *p, int64_t size, int64_t elements, int64_t n0 = 1, int64_t s0 = 0, int64_t n1 = 1, int64_t s1 = 0) {
+  if (!p) return {name, 0, 0};
+  int64_t low = 0, high = elements;
+  for (const int64_t d : {(n0 - 1) * s0, (n1 - 1) * s1}) (d < 0 ? low : high) += d;
+  return {name, (uintptr_t)p + low * size, (uintptr_t)p + high * size};
+}
+// the first result that lies in the memory of an input or of a result before it
+bool overlapping(const lmi_logprob_args *a, const char *&result, const char *&other) {
+  const int64_t rows = a->n0 * a->n1, label = a->label_dtype == LMI_I64 ? 8 : 4;
+  const Range all[] = {range_of("x", a->x, a->x_dtype == LMI_F32 ? 4 : 2, (a->classes - 1) * a->class_stride + 1, a->n0, a->stride0,
+                                a->index ? a->index_range : a->n1, a->stride1),
+                       range_of("labels", a->labels, label, 1, a->n0, a->label_stride0, a->n1, a->label_stride1),
+                       range_of("index", a->index, 4, rows), range_of("count", a->count, 4, a->n0), range_of("logprob", a->logprob, 4, rows),
+                       range_of("entropy", a->entropy, 4, rows), range_of("top_logprob", a->top_logprob, 4, rows * a->top),
+                       range_of("top_index", a->top_index, 4, rows * a->top)};
+  for (int i = 4; i < 8; ++i)
+    for (int j = 0; j < i; ++j)
+      if (all[i].first < all[j].last && all[j].first < all[i].last && all[i].first < all[i].last) {
+        result = all[i].name;
+        other = all[j].name;
+        return true;
+      }
+  return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -868,6 +899,8 @@ int lmi_class_logprobs(const lmi_logprob_args *a, void *stream) {
   LMI_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), LMI_ERR_WORKSPACE,
               "lmi_class_logprobs: workspace of %lld bytes, %lld needed", (long long)a->workspace_bytes, (long long)need);
   LMI_REQUIRE(need == 0 || lmi_is_aligned(a->workspace, 16), LMI_ERR_ALIGNMENT, "lmi_class_logprobs: workspace must be 16-byte aligned");
+  const char *result = nullptr, *other = nullptr;
+  LMI_REQUIRE(!overlapping(a, result, other), LMI_ERR_BAD_ARG, "lmi_class_logprobs: %s lies in the memory of %s", result, other);
   Evidence E;
   E.x = a->x;
   E.classes = a->classes;

@@ -765,25 +765,6 @@ def _two_strides(t: torch.Tensor, nd: int):
     return n[0], n[1], st[0], st[1]
 
 
-def _span(t: torch.Tensor):
-    """First byte of t and the one behind its last (t not empty)."""
-    first = t.data_ptr()
-    last = t.numel() - 1 if t.is_contiguous() else sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return first, first + (last + 1) * t.element_size()
-
-
-def _apart(what: str, results: dict, inputs: dict) -> None:
-    """Refuses results that lie in the memory of an input or of one another (None and empty tensors lie nowhere)."""
-    spans = [(name, *_span(t)) for name, t in inputs.items() if t is not None and t.numel()]
-    for name, t in results.items():
-        if t.numel():
-            first, last = _span(t)
-            for other, a, b in spans:
-                if first < b and a < last:
-                    raise ValueError(f"{what}: {name} lies in the memory of {other}")
-            spans.append((name, first, last))
-
-
 def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: int = 0, activation: str = "softmax",
                    index: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None, out: Optional[dict] = None) -> dict:
     """Log probability of given classes, entropy, and the `top` best classes of every row of x (..., C), classes last,
@@ -840,12 +821,10 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
         t = res[key] = out.get(key)
         if t is None or t.shape != size or t.dtype != dtype or t.device != dev or not t.is_contiguous():
             raise ValueError(f"class_logprobs: out[{key!r}] must be a contiguous {dtype} tensor of shape {size} on x's device")
-    given, out = out is not None, res
+    out = res
     rows = math.prod(lead)
     if rows == 0:
         return out
-    if given:
-        _apart("class_logprobs", {f"out[{key!r}]": t for key, t in out.items()}, {"x": x, "labels": labels, "index": index, "count": count})
     if index is not None or count is not None:   # the two leading dimensions mean what they say
         if x.ndim != 3:
             raise ValueError("class_logprobs: count needs x (B,M,C)")
@@ -879,7 +858,7 @@ def class_logprobs(x: torch.Tensor, labels: Optional[torch.Tensor] = None, top: 
         0 if index is None else x.shape[1], 0 if count is None else count.data_ptr(), 0 if labels is None else labels.data_ptr(), l0, l1,
         0 if labels is None else _LABEL_DTYPES[labels.dtype], top, 0 if labels is None else out["logprob"].data_ptr(), out["entropy"].data_ptr(),
         out["top_logprob"].data_ptr() if top else 0, out["top_index"].data_ptr() if top else 0, workspace.data_ptr() if need else 0, need)
-    _launch(_L.lmi_class_logprobs, args, dev)
+    _launch(_L.lmi_class_logprobs, args, dev)   # refuses results over an input or one another, from the addresses it has at hand
     return out
 
 
@@ -1005,6 +984,24 @@ def _mx_common(what, x, weight, bias, act, k):
         raise ValueError(f"{what}: unknown activation {act!r} (None or 'silu')")
 
 
+def _span(t: torch.Tensor):
+    """First byte of t and the one behind its last (t not empty)."""
+    first = t.data_ptr()
+    if t.is_contiguous():
+        return first, first + t.nbytes
+    return first, first + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _apart(what: str, out: torch.Tensor, inputs: dict) -> None:
+    """Refuses a result that lies in the memory of an input (None and empty tensors lie nowhere)."""
+    first, last = _span(out)
+    for name, t in inputs.items():
+        if t is not None and t.numel():
+            a, b = _span(t)
+            if first < b and a < last:
+                raise ValueError(f"{what}: `out` lies in the memory of {name}")
+
+
 def _mx_out(what, out, x, weight, bias, shape, dtype, memory_format=torch.contiguous_format):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=x.device, memory_format=memory_format)
@@ -1012,7 +1009,7 @@ def _mx_out(what, out, x, weight, bias, shape, dtype, memory_format=torch.contig
         raise ValueError(f"{what}: `out` must be a {dtype} tensor of shape {tuple(shape)} in {memory_format} on x's device")
     if out.numel():   # every result needs whole rows of x and of the weights, which others overwrite by then
         parts = {"x": x.packed, "x's scales": x.scales} if isinstance(x, MxTensor) else {"x": x}
-        _apart(what, {"`out`": out}, {**parts, "weight": weight.packed, "weight's scales": weight.scales, "bias": bias})
+        _apart(what, out, {**parts, "weight": weight.packed, "weight's scales": weight.scales, "bias": bias})
     return out
 
 

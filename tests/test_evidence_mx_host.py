@@ -234,3 +234,17 @@ def test_padded_convolutions_stay_as_they_are(monkeypatch):
     monkeypatch.setattr(MxPointwise, "of", classmethod(lambda cls, m: taken.append(m) or torch.nn.Identity()))
     assert net.quantize_pointwise() == len(taken) == len(mine) - 2
     assert mine[0] not in taken and mine[1] not in taken and mine[2] in taken
+
+
+def test_results_over_inputs_at_the_entry_point(L):
+    """Addresses alone decide: nothing is launched."""
+    def status(**kw):
+        return _probs(L, classes=10, n0=2, n1=4, stride0=40, stride1=10, **kw)
+    x, last = 4096, 4096 + 4 * 80                       # fp32 rows of ten, 2 x 4 of them
+    free = last + 4096
+    for bad in (dict(entropy=x), dict(entropy=last - 4), dict(logprob=x - 4 * 8 + 4), dict(top=1, top_index=x + 8), dict(top=1, top_logprob=x),
+                dict(entropy=free, labels=free + 28, label_dtype=4, label_stride0=4, label_stride1=1), dict(entropy=free, count=free + 8),
+                dict(entropy=free, index=free - 28, index_range=3), dict(entropy=free, logprob=free + 4), dict(top=2, top_logprob=free, top_index=free + 60),
+                dict(entropy=free + 4 * 40, index=free + 4096, index_range=1 << 40), dict(entropy=free, labels=free + 64, label_dtype=5, label_stride0=-5, label_stride1=-1)):
+        assert status(**bad) == -1, bad
+        assert b"memory of" in L.load().lmi_last_error(), bad

@@ -300,7 +300,7 @@ __device__ __forceinline__ void store_nan(const Evidence &E, long long row, int 
 }
 
 // 16 lanes per row, class j * 16 + l in value j of lane l.  64 x 300 kept rows of 80 classes (fp32, an anchor plane apart): 28 us
-// for 1.1 million scattered sectors of 64 bytes (68 MB), 2.4 TB/s; one image's 300 rows: 6.7 us, two
+// for 1.1 million scattered sectors of 64 bytes (68 MB), 2.4 TB/s; one image's 300 rows: 6.8 us, two
 // dependent loads and the arithmetic of one wave.  A wave per row took 52 and 17 us: fewer rows, and so sectors, in flight.
 template <typename T, int J, int ACT>
 __device__ __forceinline__ void evidence_team(const Evidence &E, long long row, long long rows) {
@@ -385,9 +385,10 @@ struct alignas(16) PartHead {
   float m, s, t, pad;
 };
 
-// 511 rows of 32001 classes (bf16, top 10): 17.1 us, 1.9 TB/s -- every workgroup's row is in registers at once (two per CU, all of them
+// 511 rows of 32001 classes (bf16, top 10): 17.6 us, 1.9 TB/s -- every workgroup's row is in registers at once (two per CU, all of them
 // resident), so it is the sum of loading (5.3 us), some 11 vector instructions a value (5) and the tail from the row's threshold to its
-// ranked list (5): the two rows of a CU run in step.  2 rows of 200001 (fp32, top 20) in 25 parts: 16.
+// ranked list (5): the two rows of a CU run in step.  2 rows of 200001 (fp32, top 20) in 25 parts: 11 and 5.5
+// for the join.  Probabilities of 16 bits (`none`) spill 132 to 144 bytes a lane, held to four waves per SIMD.
 // V > 1: classes lie side by side and are read in aligned 16-byte groups (the row may start anywhere; the groups at its two ends
 // are read value by value).  V == 1: any class stride.
 template <typename T, int V> struct Group {
@@ -668,9 +669,9 @@ __device__ __forceinline__ void insert2(float (&val)[2], int (&cls)[2], float v,
 
 // A thread per row, for rows side by side: a wave reads neighbouring rows' values of one class at a time.  The lists are kept by float
 // comparisons; a row that holds a NaN (or an infinity that made one) is gone through again in the order that puts NaN first.
-// 64 x 4 x 8400 rows of 16 bins (fp16, top 2): 31 us, 4.4 TB/s of 138 MB; the instructions that keep two best beside the softmax
-// take as long as the loads.  Two rows of a 16-bit type per thread, read as one word, halve the loads and the threads: no better here
-// (35.8 us) and worse for longer lists (64 x 8400 x 80, top 5: 90 us, 71 with one).
+// 64 x 4 x 8400 rows of 16 bins (fp16, top 2): 35 us, 3.9 TB/s of 138 MB; the instructions that keep two best beside the softmax
+// take as long as the loads.  Two rows of a 16-bit type per thread, read as one word, halve the loads and the threads: a tenth slower
+// here and worse for longer lists (64 x 8400 x 80, top 5: 90 us, 74 with one).
 template <typename T, int ACT, int KT>
 __global__ __launch_bounds__(256) void evidence_planes_kernel(const Evidence E) {
   const long long row = (long long)blockIdx.x * 256 + threadIdx.x;

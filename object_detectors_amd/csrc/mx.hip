@@ -72,7 +72,7 @@ template <typename T, bool VEC> __device__ __forceinline__ void load8(const T *p
   }
 }
 
-// Bound by HBM: 409600 x 320 fp16 (331 MB in and out) 64 - 75 us, 4.4 - 5.2 TB/s; 640 x 2560 fp32 4 us.
+// Bound by HBM: 409600 x 320 fp16 (331 MB in and out) 62 us, 5.3 TB/s; 640 x 2560 fp32 4 us.
 // lane = (row of the octet, block of the step, quarter of the block).  The wave reads 8 rows x 128 bytes (16-bit types) per step and writes 8 x 16
 // bytes side by side for either block; the scale bytes of its four steps leave as one word.
 template <typename T, bool VEC>
@@ -386,7 +386,7 @@ __device__ __forceinline__ void store_rows(const Product &P, Y *y, long long p0,
 }
 
 // One wave, 64 positions, k of one step (at most 64), everything in registers: what a lane quantises is its operand.  No LDS, no barrier: the
-// waves of a CU drift apart, so that some load while others multiply.  Bound by HBM: 64 x 64 -> 32 on 160 x 160 58 us, 5.4 TB/s (69 streamed);
+// waves of a CU drift apart, so that some load while others multiply.  Bound by HBM: 64 x 64 -> 32 on 160 x 160 59 us, 5.3 TB/s (69 streamed);
 // 16 x 48 -> 32 on 160 x 160 17.5 and 21.  Two steps held that way stream faster: 16 x 128 -> 64 on 80 x 80 13.6 us, 11 streamed.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256, 4) void mx_wave_planes_kernel(const Product P, int act, long long tiles) {
@@ -434,8 +434,9 @@ template <typename T, bool VEC> void launch_wave_planes(Product P, int act, long
 // Streaming product: 128 positions x up to 64 * NT weight rows per workgroup, k in chunks of two steps.  While the matrix instructions run
 // on one chunk, the next chunk's activations and weights are on their way to registers (loads straight to LDS would be waited for
 // before the next read of any LDS); an activation block is quantised by the thread that loaded it.  Waves are dealt 2 (positions) x 2 (weight rows), each 64 positions x 32 * NT
-// rows of sums in registers: a fragment read from LDS serves 2 or NT matrix instructions.  Bound by HBM: 64 x 1280 -> 320 on 80 x 80 (fp16, 1.31 GB) 270 us, 4.9 TB/s; two
-// workgroups per CU hold 64 KB of loads in flight and stop for each other at every chunk, which costs the rest to 6.2 TB/s.
+// rows of sums in registers: a fragment read from LDS serves 2 or NT matrix instructions.  Bound by HBM: 64 x 1280 -> 320 on 80 x 80 (fp16, 1.31 GB) 273 us, 4.8 TB/s (64 x 320 -> 320: 0.52 GB, 124 us, 4.2); two
+// workgroups per CU hold 64 KB of loads in flight and stop for each other at every chunk, which costs the rest to 6.2 TB/s.  The widest tiles (five per wave, planes of
+// 16 bits) spill 8 to 12 bytes a lane.
 constexpr int kChunkTile = 128;
 
 template <typename T, bool PLANES, bool VEC> struct Chunk;   // what a thread holds of a chunk
@@ -643,11 +644,11 @@ template <typename T, typename Y, bool PLANES, bool VEC> void launch_stream(Prod
 
 // Quantised rows: 64 * WP of them x 32 * NT * 4 / WP weight rows per workgroup, a wave 64 x 32 * NT.  The weights go through LDS; a wave's rows, which
 // at most one other wave needs, come straight into the operands, a chunk of two steps ahead: with both through LDS its traffic (84 KB
-// per chunk for 655 k products of 64) kept it as busy as the matrix units, 8192 x 2560 -> 2560 took 49 us instead of 44.  What
+// per chunk for 655 k products of 64) kept it as busy as the matrix units, 8192 x 2560 -> 2560 took a tenth longer.  It takes 43 us.  What
 // bounds it: the matrix units are busy for half of the time of a deep product (3.8 of the 8.9 PFLOP/s that a loop of
-// nothing else reaches: 8192 x 10240 -> 2560 in 112 us, 1.2 us per chunk), the rest are the waits of two workgroups per CU for
+// nothing else reaches: 8192 x 10240 -> 2560 in 114 us, 1.2 us per chunk), the rest are the waits of two workgroups per CU for
 // each other's loads; touching lines two chunks ahead, chunks in two sets of registers with smaller tiles, and priorities changed
-// nothing or cost; the first loads and 42 MB of results take 15 of the 44 us.
+// nothing or cost; the first loads and 42 MB of results take 19 of the 43 us (the line through k = 2560 and 10240, at k = 0).
 template <typename Y, int NT, int WP>
 __global__ __launch_bounds__(256, 2) void mx_rows_kernel(const Product P, int act, int splits, long long tiles, int vec_y) {
   constexpr int WN = 4 / WP, NG = NT * WN, NF = (NG + 1) / 2, NW = (NG + 3) / 4;
@@ -789,8 +790,8 @@ template <typename Y, int WP> void launch_rows(const Product &P, int act, hipStr
 }
 
 // Few positions: 64 of them x 32 weight rows per workgroup, its eight waves share k.  A wave loads its steps' blocks straight into the
-// operands -- no LDS, no barrier before the sums meet; a workgroup's time is the latency of a load or two: a row of 1280 -> 1000 6.4 us, 640 -> 640
-// on 20 x 20 7.1.
+// operands -- no LDS, no barrier before the sums meet; a workgroup's time is the latency of a load or two: a row of 1280 -> 1000 6.5 us, 640 -> 640
+// on 20 x 20 7.2.  The row forms spill 16 (bf16) to 48 bytes a lane (fp32), held to four waves per SIMD.
 constexpr int kFewWaves = 8;
 // Up to this many pairs of tiles, two workgroups per CU (us here and streamed, fp16: 640 -> 320 on 40 x 40, 25 x 10 of them, 7.9 and 9.9;
 // 320 -> 160 on 80 x 80, 100 x 5, 7.1 and 7.6; 4 x 640 -> 640 on 20 x 20, 28 x 20, 12.6 and 10.7; 4 x 320 -> 320 on 40 x 40, 100 x 10, 12.1 and

@@ -1064,10 +1064,10 @@ def mx_pointwise(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor]
     _mx_common("mx_pointwise", x, weight, bias, act, k)
     n = weight.shape[0]
     sb, sk, sh, sw = x.stride()
-    if b == 1:        # strides of dimensions of one element say nothing, however large
-        sb = k * h * w
+    if b == 1:        # strides of dimensions of one element say nothing, however large or odd
+        sb = 0
     if k == 1:
-        sk = h * w
+        sk = 0
     planes = (w == 1 or sw == 1) and (h == 1 or sh == w * (sw if w > 1 else 1)) and h * w > 1
     if planes and w == 1 and h > 1:
         planes = sh == 1

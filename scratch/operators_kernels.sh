@@ -1,9 +1,9 @@
 #!/bin/bash
-# rocprofv3 over every case of scratch/operators_kernels.py -> gpurun_out/operators_kernels.csv (kept as profiles/operators/kernels.csv)
-R=${GRAFT_REPO_ROOT:-$(cd "$(dirname "$0")/.." && pwd)}
+# rocprofv3 over every case of scratch/operators_kernels.py -> the file named (kept as profiles/operators/kernels.csv)
+R=$(cd "$(dirname "$0")/.." && pwd)
+OUT=$(realpath "${1:?file to write}")
 cd /tmp && export TMPDIR=/tmp
-OUT=$R/gpurun_out/operators_kernels.csv
-mkdir -p $R/gpurun_out && echo "case,kernel,launches,median_us,min_us" > $OUT
+echo "case,kernel,launches,median_us,min_us" > $OUT
 python3 $R/scratch/operators_kernels.py names > /tmp/op_names 2>/dev/null || exit 1
 while read -r c; do
   rm -rf /tmp/op_prof

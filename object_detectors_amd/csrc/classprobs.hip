@@ -56,10 +56,10 @@ __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
 __device__ __forceinline__ float to_float(__bf16 v) { return (float)v; }
 
-// monotonic bits: larger value -> larger number; -0 = +0; NaN above everything; never 0
+// monotonic bits: larger value -> larger number; -0 = +0; NaN above everything; never 0, never all ones (no key is ~0, from which the rounds start)
 __device__ __forceinline__ unsigned order_bits(float v) {
   unsigned b = __float_as_uint(v + 0.0f);
-  b = v != v ? 0x7fffffffu : b;
+  b = v != v ? 0x7ffffffeu : b;
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float order_value(unsigned o) {

@@ -471,3 +471,21 @@ def test_results_over_inputs_are_refused():
     with pytest.raises(ValueError, match="memory of"):
         ops.class_logprobs(x[:1, :1], top=1, count=one, out={"entropy": torch.zeros(1, 1).cuda(), "top_logprob": torch.zeros(1, 1, 1).cuda(),
                                                             "top_index": one.view(1, 1, 1)})
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["rows", "planes"])
+@pytest.mark.parametrize("c,top", [(100, 3), (131, 1), (600, 5), (5000, 32), (20001, 8), (70001, 32)])
+def test_nan_of_the_first_class_among_many_equal_values(c, top, layout, dtype):
+    """More candidates than the table holds, the best of them a NaN at class 0."""
+    x = torch.full((4, c), -float("inf"))
+    x[0, 0] = float("nan")
+    x[1] = 0.5
+    x[1, [0, c - 1]] = float("nan")
+    x[2] = float("nan")
+    x[3, 0] = float("inf")
+    x = x.to(DTYPES[dtype]).cuda()
+    if layout == "planes":
+        x = x.t().contiguous().t()
+    labels = torch.tensor([0, 1, 2, 0]).cuda()
+    _check(_ops().class_logprobs(x, labels, top=top), x, labels, top, "softmax")
